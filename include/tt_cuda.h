@@ -12,8 +12,9 @@
  * status back into std::runtime_error(ttc_last_error()), which keeps the
  * reference's error behaviour for tt_lazy users.
  *
- * Data: fp32 only, row-major, rank <= 4 -- the reference's only dtype and
- * rank limit (src/core/Tensor.hpp:111-114).
+ * Data: fp32, row-major, rank <= 4 -- the reference's only dtype and rank
+ * limit (src/core/Tensor.hpp:111-114). The feed-forward operators at the end
+ * (ttc_rms_norm, ttc_linear, ttc_gated_linear) take 16-bit and 8-bit types too.
  *
  * Threading: one process drives one GPU; calls come from one host thread
  * (the reference's Context/EvaluationManager are unsynchronised singletons,
@@ -313,6 +314,185 @@ typedef struct {
 int ttc_gemm(const ttc_gemm_desc* desc);
 /* Which path ttc_gemm would take for this descriptor (TTC_GEMM_FFMA/TF32/TF32X3). */
 int ttc_gemm_select_path(const ttc_gemm_desc* desc);
+
+/* ------------------------------------------- feed-forward block operators
+ * The operators of a language model's feed-forward block beside the fused
+ * MLP above, in the types such models run in; no counterpart in the
+ * reference (fp32, inference on the CPU):
+ *
+ *   ttc_rms_norm       h = x + residual;  y = h * rsqrt(mean(h^2) + eps) * weight
+ *   ttc_linear         y = act(x W + bias) + residual
+ *   ttc_gated_linear   y = act(x Wg) * (x Wu)       (one kernel)
+ *
+ * with their gradients (_backward). A block is the three in a row: the norm,
+ * the gated pair, and ttc_linear back to the model's width with the residual.
+ *
+ * Types. dtype is the operands' type. The norm takes F32, F16 and BF16 and can
+ * write e4m3 with one scale per row, which is the form the 8-bit products
+ * read. The products take F16, BF16 and (forward only) E4M3 operands; fp32
+ * products are ttc_gemm's. Every sum, norm and activation is computed in fp32
+ * and rounded once, where a value is stored in its tensor's type.
+ *
+ * Layout. Matrices are row-major with a leading dimension in elements. With
+ * trans_w = 0 a weight is stored [K, N] as for ttc_gemm, with trans_w = 1
+ * [N, K]; E4M3 weights have trans_w = 1. Any size, leading dimension and
+ * element-aligned address is accepted. A matrix operand of a product whose
+ * address or row pitch is not a multiple of 16 bytes is first copied into the
+ * workspace with padded rows.
+ *
+ * Memory and streams. The calls allocate nothing: scratch memory is the
+ * caller's `workspace` (256-byte aligned, of at least the bytes that the
+ * matching _workspace function returns for the same descriptor; 0 for most
+ * forward calls). It is used until the call's kernels have run on the library
+ * stream and holds nothing between calls. Calls that may overlap (different
+ * streams, or captured graphs that are replayed side by side) take different
+ * workspaces. Results do not depend on scheduling: no floating-point atomics.
+ *
+ * Zero rows (rows or M = 0) are a valid call: gradients of weights and biases
+ * are then zeros, everything else is left as it is. Descriptors are checked
+ * before anything runs, also without a device. Fields that are not described
+ * as optional must be set; a pointer that is optional may be NULL, and its
+ * leading dimension is then ignored. */
+typedef enum { TTC_F32 = 0, TTC_F16 = 1, TTC_BF16 = 2, TTC_E4M3 = 3 } ttc_dtype;
+
+/* Activations: z; max(z, 0) (NaN stays NaN); z / (1 + e^-z); z Phi(z) with the
+ * normal distribution function; its tanh form z (1 + tanh(sqrt(2/pi) (z +
+ * 0.044715 z^3))) / 2. The gradient of max(z, 0) at 0 is 0. */
+typedef enum {
+    TTC_ACT_NONE = 0,
+    TTC_ACT_RELU = 1,
+    TTC_ACT_SILU = 2,
+    TTC_ACT_GELU = 3,
+    TTC_ACT_GELU_TANH = 4
+} ttc_activation;
+
+/* Root-mean-square norm over the last dimension of x [rows, cols], with the
+ * residual stream's addition in front. The norm is of the fp32 sum
+ * x + residual; `hidden` receives that sum rounded to dtype.
+ * y_dtype is dtype, or E4M3: then scales[r] = max(max_c |y(r, c)| / 448, 2^-126)
+ * and y holds e4m3(y(r, c) * (1 / scales[r])), rounded to nearest even and
+ * saturated at +-448 (NaN stays NaN).
+ * `hidden` and `y` may be `x` or `residual` themselves (same address and
+ * leading dimension, same type); no other overlap is allowed. */
+typedef struct {
+    int64_t rows;
+    int32_t cols; /* >= 1 */
+    int32_t dtype, weight_dtype, y_dtype; /* weight_dtype: dtype or F32 */
+    float eps;                            /* >= 0 */
+    const void* x; int64_t ldx;
+    const void* residual; int64_t ldr; /* optional, dtype */
+    const void* weight;                /* [cols] */
+    void* y; int64_t ldy;
+    void* hidden; int64_t ldh;         /* optional, dtype */
+    float* scales;                     /* [rows], with y_dtype E4M3 only */
+} ttc_rms_norm_desc;
+int ttc_rms_norm(const ttc_rms_norm_desc* desc);
+
+/* Gradients of ttc_rms_norm from dy and the forward call's `hidden` (its `x`
+ * where it had no residual):
+ *   dx = rstd (dy weight - hidden rstd^2 mean(dy weight hidden)) + dhidden
+ *   dweight[c] = sum_r dy(r, c) hidden(r, c) rstd(r)
+ * dhidden, optional, is the gradient that reaches `hidden` by another way (the
+ * residual stream); dx is then the gradient of both x and residual. dx may be
+ * dy or dhidden themselves. */
+typedef struct {
+    int64_t rows;
+    int32_t cols;
+    int32_t dtype, weight_dtype;
+    float eps;
+    const void* dy; int64_t lddy;
+    const void* hidden; int64_t ldh;
+    const void* weight;
+    const void* dhidden; int64_t lddh; /* optional */
+    void* dx; int64_t lddx;
+    void* dweight; /* optional, [cols], weight_dtype */
+    void* workspace; size_t workspace_bytes;
+} ttc_rms_norm_backward_desc;
+int ttc_rms_norm_backward(const ttc_rms_norm_backward_desc* desc);
+int ttc_rms_norm_backward_workspace(const ttc_rms_norm_backward_desc* desc, size_t* bytes);
+
+/* y [M, N] = act(x [M, K] W + bias) + residual. With dtype E4M3 the product is
+ * scaled before the bias: x_scales[m] * w_scales[n] * (x W)(m, n).
+ * y, bias, residual and pre have y_dtype: dtype or F32 for 16-bit operands;
+ * F16, BF16 or F32 for E4M3. y may be `residual` itself. */
+typedef struct {
+    int32_t M, N, K; /* M >= 0, N >= 1, K >= 1 */
+    int32_t dtype, y_dtype, trans_w, act;
+    const void* x; int64_t ldx;
+    const void* w; int64_t ldw;
+    void* y; int64_t ldy;
+    const void* bias;                  /* optional, [N] */
+    const void* residual; int64_t ldr; /* optional, [M, N] */
+    void* pre; int64_t ldp;            /* optional, [M, N]: x W + bias, for the backward pass */
+    const float* x_scales;             /* [M] and [N], with E4M3 only */
+    const float* w_scales;
+    void* workspace; size_t workspace_bytes;
+} ttc_linear_desc;
+int ttc_linear(const ttc_linear_desc* desc);
+int ttc_linear_workspace(const ttc_linear_desc* desc, size_t* bytes);
+
+/* Gradients of ttc_linear (F16, BF16): with dz = dy act'(pre), rounded to
+ * dtype for the products,
+ *   dx = dz W^T,  dw = x^T dz (stored as W is),  dbias = sum over rows of dz.
+ * The residual's gradient is dy itself. Each of dx, dw, dbias is optional; x is
+ * read for dw, w for dx, pre for act != NONE. */
+typedef struct {
+    int32_t M, N, K;
+    int32_t dtype, trans_w, act;
+    const void* dy; int64_t lddy;
+    const void* x; int64_t ldx;
+    const void* w; int64_t ldw;
+    const void* pre; int64_t ldp;
+    void* dx; int64_t lddx;
+    void* dw; int64_t lddw;
+    void* dbias;
+    void* workspace; size_t workspace_bytes;
+} ttc_linear_backward_desc;
+int ttc_linear_backward(const ttc_linear_backward_desc* desc);
+int ttc_linear_backward_workspace(const ttc_linear_backward_desc* desc, size_t* bytes);
+
+/* y [M, N] = act(x Wg) * (x Wu): both products, the activation and the product
+ * of the two in one kernel. gate and up, optional (both or neither), receive
+ * x Wg and x Wu for the backward pass. Types as for ttc_linear, with one scale
+ * vector for each weight. */
+typedef struct {
+    int32_t M, N, K;
+    int32_t dtype, y_dtype, trans_w, act;
+    const void* x; int64_t ldx;
+    const void* wg;
+    const void* wu; int64_t ldw; /* of both weights */
+    void* y; int64_t ldy;
+    void* gate;
+    void* up; int64_t ldp; /* of both */
+    const float* x_scales;
+    const float* wg_scales;
+    const float* wu_scales;
+    void* workspace; size_t workspace_bytes;
+} ttc_gated_linear_desc;
+int ttc_gated_linear(const ttc_gated_linear_desc* desc);
+int ttc_gated_linear_workspace(const ttc_gated_linear_desc* desc, size_t* bytes);
+
+/* Gradients of ttc_gated_linear (F16, BF16) from the saved gate and up: with
+ * dg = dy up act'(gate) and du = dy act(gate), rounded to dtype for the
+ * products,
+ *   dx = dg Wg^T + du Wu^T,  dwg = x^T dg,  dwu = x^T du (stored as W is).
+ * dx is optional, and dwg with dwu (both or neither). */
+typedef struct {
+    int32_t M, N, K;
+    int32_t dtype, trans_w, act;
+    const void* dy; int64_t lddy;
+    const void* x; int64_t ldx;
+    const void* wg;
+    const void* wu; int64_t ldw;
+    const void* gate;
+    const void* up; int64_t ldp;
+    void* dx; int64_t lddx;
+    void* dwg;
+    void* dwu; int64_t lddw;
+    void* workspace; size_t workspace_bytes;
+} ttc_gated_linear_backward_desc;
+int ttc_gated_linear_backward(const ttc_gated_linear_backward_desc* desc);
+int ttc_gated_linear_backward_workspace(const ttc_gated_linear_backward_desc* desc, size_t* bytes);
 
 /* ------------------------------------------------ collective (multi-GPU)
  * Row-sharded data parallelism: every rank holds the same weights and a

@@ -37,7 +37,11 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + ["-O3", "-lineinfo", "-std=c++17", "-fmad=false", "-Xcompiler", "-fPIC",
                      "--expt-relaxed-constexpr", "-I" + INCLUDE, "-I" + CSRC, "-I" + OBJ]
 
-CUDA_SOURCES = ["runtime.cu", "chain.cu", "chain_tma.cu", "chain_jit.cu", "transpose.cu", "gemm_ffma.cu", "gemm_tc.cu"]
+CUDA_SOURCES = ["runtime.cu", "chain.cu", "chain_tma.cu", "chain_jit.cu", "transpose.cu", "gemm_ffma.cu", "gemm_tc.cu", "norm.cu",
+                "linear.cu"]
+# Nothing in these is compared bit for bit with another implementation: the
+# compiler may contract multiply-adds.
+FMAD_SOURCES = {"norm.cu", "linear.cu"}
 CPP_SOURCES = ["comm.cpp"]
 
 
@@ -95,7 +99,8 @@ def build_cuda(verbose=False) -> str:
         s = os.path.join(CSRC, src)
         o = os.path.join(OBJ, src + ".o")
         if _stale(o, [s] + hdrs):
-            _run([NVCC] + NVCC_FLAGS + ["-c", s, "-o", o + ".tmp"], verbose)
+            flags = [f for f in NVCC_FLAGS if f != "-fmad=false"] if src in FMAD_SOURCES else NVCC_FLAGS
+            _run([NVCC] + flags + ["-c", s, "-o", o + ".tmp"], verbose)
             os.replace(o + ".tmp", o)
         objs.append(o)
     for src in CPP_SOURCES:

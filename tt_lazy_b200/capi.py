@@ -28,6 +28,12 @@ SRC_ACC, SRC_INPUT, SRC_SLOT = range(3)
 REDUCE_NONE, REDUCE_ALL, REDUCE_ROWS, REDUCE_COLS = range(4)
 # ttc_gemm_path
 GEMM_AUTO, GEMM_FFMA, GEMM_TF32, GEMM_TF32X3 = range(4)
+# ttc_dtype
+F32, F16, BF16, E4M3 = range(4)
+DTYPES = {"f32": F32, "f16": F16, "bf16": BF16, "e4m3": E4M3}
+# ttc_activation
+ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU, ACT_GELU_TANH = range(5)
+ACTIVATIONS = {"none": ACT_NONE, "relu": ACT_RELU, "silu": ACT_SILU, "gelu": ACT_GELU, "gelu_tanh": ACT_GELU_TANH}
 
 
 class Instr(C.Structure):
@@ -61,6 +67,61 @@ class GemmDesc(C.Structure):
                 ("epilogue", ChainDesc)]
 
 
+class RmsNormDesc(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("cols", C.c_int32),
+                ("dtype", C.c_int32), ("weight_dtype", C.c_int32), ("y_dtype", C.c_int32), ("eps", C.c_float),
+                ("x", C.c_void_p), ("ldx", C.c_int64), ("residual", C.c_void_p), ("ldr", C.c_int64),
+                ("weight", C.c_void_p), ("y", C.c_void_p), ("ldy", C.c_int64),
+                ("hidden", C.c_void_p), ("ldh", C.c_int64), ("scales", C.c_void_p)]
+
+
+class RmsNormBackwardDesc(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("cols", C.c_int32),
+                ("dtype", C.c_int32), ("weight_dtype", C.c_int32), ("eps", C.c_float),
+                ("dy", C.c_void_p), ("lddy", C.c_int64), ("hidden", C.c_void_p), ("ldh", C.c_int64),
+                ("weight", C.c_void_p), ("dhidden", C.c_void_p), ("lddh", C.c_int64),
+                ("dx", C.c_void_p), ("lddx", C.c_int64), ("dweight", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class LinearDesc(C.Structure):
+    _fields_ = [("M", C.c_int32), ("N", C.c_int32), ("K", C.c_int32),
+                ("dtype", C.c_int32), ("y_dtype", C.c_int32), ("trans_w", C.c_int32), ("act", C.c_int32),
+                ("x", C.c_void_p), ("ldx", C.c_int64), ("w", C.c_void_p), ("ldw", C.c_int64),
+                ("y", C.c_void_p), ("ldy", C.c_int64), ("bias", C.c_void_p),
+                ("residual", C.c_void_p), ("ldr", C.c_int64), ("pre", C.c_void_p), ("ldp", C.c_int64),
+                ("x_scales", C.c_void_p), ("w_scales", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class LinearBackwardDesc(C.Structure):
+    _fields_ = [("M", C.c_int32), ("N", C.c_int32), ("K", C.c_int32),
+                ("dtype", C.c_int32), ("trans_w", C.c_int32), ("act", C.c_int32),
+                ("dy", C.c_void_p), ("lddy", C.c_int64), ("x", C.c_void_p), ("ldx", C.c_int64),
+                ("w", C.c_void_p), ("ldw", C.c_int64), ("pre", C.c_void_p), ("ldp", C.c_int64),
+                ("dx", C.c_void_p), ("lddx", C.c_int64), ("dw", C.c_void_p), ("lddw", C.c_int64),
+                ("dbias", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class GatedLinearDesc(C.Structure):
+    _fields_ = [("M", C.c_int32), ("N", C.c_int32), ("K", C.c_int32),
+                ("dtype", C.c_int32), ("y_dtype", C.c_int32), ("trans_w", C.c_int32), ("act", C.c_int32),
+                ("x", C.c_void_p), ("ldx", C.c_int64), ("wg", C.c_void_p), ("wu", C.c_void_p), ("ldw", C.c_int64),
+                ("y", C.c_void_p), ("ldy", C.c_int64), ("gate", C.c_void_p), ("up", C.c_void_p), ("ldp", C.c_int64),
+                ("x_scales", C.c_void_p), ("wg_scales", C.c_void_p), ("wu_scales", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class GatedLinearBackwardDesc(C.Structure):
+    _fields_ = [("M", C.c_int32), ("N", C.c_int32), ("K", C.c_int32),
+                ("dtype", C.c_int32), ("trans_w", C.c_int32), ("act", C.c_int32),
+                ("dy", C.c_void_p), ("lddy", C.c_int64), ("x", C.c_void_p), ("ldx", C.c_int64),
+                ("wg", C.c_void_p), ("wu", C.c_void_p), ("ldw", C.c_int64),
+                ("gate", C.c_void_p), ("up", C.c_void_p), ("ldp", C.c_int64),
+                ("dx", C.c_void_p), ("lddx", C.c_int64), ("dwg", C.c_void_p), ("dwu", C.c_void_p),
+                ("lddw", C.c_int64), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
 class MemoryStats(C.Structure):
     _fields_ = [("bytes_in_use", C.c_size_t), ("peak_bytes", C.c_size_t), ("workspace_bytes", C.c_size_t),
                 ("kernels_launched", C.c_uint64)]
@@ -71,7 +132,17 @@ EXPORTS = ["ttc_last_error", "ttc_init", "ttc_shutdown", "ttc_device_count", "tt
            "ttc_set_stream", "ttc_synchronize", "ttc_malloc", "ttc_free", "ttc_memcpy_h2d", "ttc_memcpy_d2h", "ttc_h2d_prefetch", "ttc_wait_ticket", "ttc_capture_begin", "ttc_capture_end", "ttc_graph_launch", "ttc_graph_destroy", "ttc_range_push", "ttc_range_pop", "ttc_timer_mark", "ttc_timer_elapsed",
            "ttc_memcpy_d2d", "ttc_memset_zero", "ttc_host_alloc", "ttc_host_free", "ttc_get_memory_stats",
            "ttc_eltwise_chain", "ttc_eltwise_chain_noalloc", "ttc_chain_jit_source", "ttc_reduce", "ttc_transpose", "ttc_copy2d", "ttc_gemm", "ttc_gemm_select_path",
+           "ttc_rms_norm", "ttc_rms_norm_backward", "ttc_rms_norm_backward_workspace",
+           "ttc_linear", "ttc_linear_workspace", "ttc_linear_backward", "ttc_linear_backward_workspace",
+           "ttc_gated_linear", "ttc_gated_linear_workspace",
+           "ttc_gated_linear_backward", "ttc_gated_linear_backward_workspace",
            "ttc_comm_unique_id", "ttc_comm_init", "ttc_allreduce_sum", "ttc_comm_destroy"]
+
+
+# Descriptors whose calls take a workspace, and those calls.
+_WITH_WORKSPACE = {RmsNormBackwardDesc: "ttc_rms_norm_backward", LinearDesc: "ttc_linear",
+                   LinearBackwardDesc: "ttc_linear_backward", GatedLinearDesc: "ttc_gated_linear",
+                   GatedLinearBackwardDesc: "ttc_gated_linear_backward"}
 
 
 class TTCError(RuntimeError):
@@ -113,6 +184,10 @@ def lib():
         L.ttc_chain_jit_source.argtypes = [C.POINTER(ChainDesc), C.c_char_p, C.c_size_t, C.POINTER(C.c_size_t)]
         L.ttc_gemm.argtypes = [C.POINTER(GemmDesc)]
         L.ttc_gemm_select_path.argtypes = [C.POINTER(GemmDesc)]
+        L.ttc_rms_norm.argtypes = [C.POINTER(RmsNormDesc)]
+        for desc, fn in _WITH_WORKSPACE.items():
+            getattr(L, fn).argtypes = [C.POINTER(desc)]
+            getattr(L, fn + "_workspace").argtypes = [C.POINTER(desc), C.POINTER(C.c_size_t)]
         L.ttc_reduce.argtypes = [C.c_void_p, C.POINTER(C.c_uint32), C.c_int, C.POINTER(C.c_int32), C.c_int,
                                  C.c_int, C.c_void_p]
         L.ttc_transpose.argtypes = [C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_int64]
@@ -135,6 +210,14 @@ def init(device=0):
     check(lib().ttc_init(device))
 
 
+def set_stream(stream=None):
+    """Run the library's calls on `stream`, a CUDA stream handle (an int, as in
+    torch.cuda.Stream.cuda_stream); None restores the library's own stream.
+    Handle 0, CUDA's legacy default stream, is passed on by its other name,
+    since 0 means the library's own stream to ttc_set_stream."""
+    check(lib().ttc_set_stream(None if stream is None else (stream or 1)))
+
+
 def synchronize():
     check(lib().ttc_synchronize())
 
@@ -150,12 +233,15 @@ def kernels_launched() -> int:
 
 
 class DeviceArray:
-    """A float32 buffer in device memory, owned through ttc_malloc/ttc_free."""
+    """A buffer in device memory, owned through ttc_malloc/ttc_free: float32,
+    or another numpy type of the same bits as its elements (float16; uint16
+    for bf16 and uint8 for e4m3, which numpy does not have)."""
 
-    def __init__(self, shape, ptr=None, owner=True):
+    def __init__(self, shape, ptr=None, owner=True, dtype=np.float32):
         self.shape = tuple(int(s) for s in shape)
         self.size = int(np.prod(self.shape)) if self.shape else 1
-        self.nbytes = self.size * 4
+        self.dtype = np.dtype(dtype)
+        self.nbytes = self.size * self.dtype.itemsize
         if ptr is None:
             p = C.c_void_p()
             check(lib().ttc_malloc(self.nbytes, C.byref(p)))
@@ -164,30 +250,30 @@ class DeviceArray:
         self._owner = owner
 
     @classmethod
-    def from_numpy(cls, a):
-        a = np.ascontiguousarray(a, dtype=np.float32)
-        d = cls(a.shape)
+    def from_numpy(cls, a, dtype=np.float32):
+        a = np.ascontiguousarray(a, dtype=dtype)
+        d = cls(a.shape, dtype=dtype)
         check(lib().ttc_memcpy_h2d(d.ptr, a.ctypes.data, d.nbytes))
         return d
 
     @classmethod
-    def empty(cls, shape):
-        return cls(shape)
+    def empty(cls, shape, dtype=np.float32):
+        return cls(shape, dtype=dtype)
 
     @classmethod
-    def zeros(cls, shape):
-        d = cls(shape)
+    def zeros(cls, shape, dtype=np.float32):
+        d = cls(shape, dtype=dtype)
         check(lib().ttc_memset_zero(d.ptr, d.nbytes))
         return d
 
     def numpy(self):
-        out = np.empty(self.shape, dtype=np.float32)
+        out = np.empty(self.shape, dtype=self.dtype)
         check(lib().ttc_memcpy_d2h(out.ctypes.data, self.ptr, self.nbytes))
         return out
 
     def at(self, elem_offset):
         """Pointer to element `elem_offset` (a view; no ownership)."""
-        return (self.ptr or 0) + 4 * int(elem_offset)
+        return (self.ptr or 0) + self.dtype.itemsize * int(elem_offset)
 
     def free(self):
         if self._owner and self.ptr:
@@ -274,3 +360,83 @@ def transpose(in_ptr, out_ptr, batch, rows, cols):
 
 def copy2d(in_ptr, in_ld, out_ptr, out_ld, rows, cols):
     check(lib().ttc_copy2d(in_ptr, in_ld, out_ptr, out_ld, rows, cols))
+
+
+# ------------------------------------------------- feed-forward block operators
+# Each operator has a descriptor builder, like chain_desc, and a call that takes
+# the descriptor. Pointers are device addresses (ints); dtype and y_dtype are
+# F32 / F16 / BF16 / E4M3. See include/tt_cuda.h for the formulas and rules.
+def rms_norm_desc(rows, cols, x, ldx, weight, y, ldy, dtype, y_dtype=None, weight_dtype=None, eps=1e-6,
+                  residual=None, ldr=0, hidden=None, ldh=0, scales=None):
+    return RmsNormDesc(rows, cols, dtype, dtype if weight_dtype is None else weight_dtype,
+                       dtype if y_dtype is None else y_dtype, eps, x, ldx, residual, ldr, weight, y, ldy, hidden, ldh,
+                       scales)
+
+
+def rms_norm_backward_desc(rows, cols, dy, lddy, hidden, ldh, weight, dx, lddx, dweight, dtype, weight_dtype=None,
+                           eps=1e-6, dhidden=None, lddh=0):
+    return RmsNormBackwardDesc(rows, cols, dtype, dtype if weight_dtype is None else weight_dtype, eps, dy, lddy,
+                               hidden, ldh, weight, dhidden, lddh, dx, lddx, dweight)
+
+
+def linear_desc(M, N, K, x, ldx, w, ldw, y, ldy, dtype, y_dtype=None, trans_w=False, act=ACT_NONE, bias=None,
+                residual=None, ldr=0, pre=None, ldp=0, x_scales=None, w_scales=None):
+    return LinearDesc(M, N, K, dtype, dtype if y_dtype is None else y_dtype, trans_w, act, x, ldx, w, ldw, y, ldy,
+                      bias, residual, ldr, pre, ldp, x_scales, w_scales)
+
+
+def linear_backward_desc(M, N, K, dy, lddy, x, ldx, w, ldw, dtype, trans_w=False, act=ACT_NONE, pre=None, ldp=0,
+                         dx=None, lddx=0, dw=None, lddw=0, dbias=None):
+    return LinearBackwardDesc(M, N, K, dtype, trans_w, act, dy, lddy, x, ldx, w, ldw, pre, ldp, dx, lddx, dw, lddw,
+                              dbias)
+
+
+def gated_linear_desc(M, N, K, x, ldx, wg, wu, ldw, y, ldy, dtype, y_dtype=None, trans_w=False, act=ACT_SILU,
+                      gate=None, up=None, ldp=0, x_scales=None, wg_scales=None, wu_scales=None):
+    return GatedLinearDesc(M, N, K, dtype, dtype if y_dtype is None else y_dtype, trans_w, act, x, ldx, wg, wu, ldw,
+                           y, ldy, gate, up, ldp, x_scales, wg_scales, wu_scales)
+
+
+def gated_linear_backward_desc(M, N, K, dy, lddy, x, ldx, wg, wu, ldw, gate, up, ldp, dtype, trans_w=False,
+                               act=ACT_SILU, dx=None, lddx=0, dwg=None, dwu=None, lddw=0):
+    return GatedLinearBackwardDesc(M, N, K, dtype, trans_w, act, dy, lddy, x, ldx, wg, wu, ldw, gate, up, ldp, dx,
+                                   lddx, dwg, dwu, lddw)
+
+
+def workspace_size(desc) -> int:
+    """Bytes of workspace that the call with this descriptor needs (0: none)."""
+    n = C.c_size_t(0)
+    check(getattr(lib(), _WITH_WORKSPACE[type(desc)] + "_workspace")(C.byref(desc), C.byref(n)))
+    return n.value
+
+
+def _call(desc, workspace):
+    """`workspace`: None, a DeviceArray or a torch CUDA tensor."""
+    if workspace is not None:
+        desc.workspace = workspace.ptr if isinstance(workspace, DeviceArray) else workspace.data_ptr()
+        desc.workspace_bytes = workspace.nbytes
+    check(getattr(lib(), _WITH_WORKSPACE[type(desc)])(C.byref(desc)))
+
+
+def rms_norm(desc):
+    check(lib().ttc_rms_norm(C.byref(desc)))
+
+
+def rms_norm_backward(desc, workspace=None):
+    _call(desc, workspace)
+
+
+def linear(desc, workspace=None):
+    _call(desc, workspace)
+
+
+def linear_backward(desc, workspace=None):
+    _call(desc, workspace)
+
+
+def gated_linear(desc, workspace=None):
+    _call(desc, workspace)
+
+
+def gated_linear_backward(desc, workspace=None):
+    _call(desc, workspace)

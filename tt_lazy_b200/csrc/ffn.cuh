@@ -1,0 +1,328 @@
+// ffn.cuh -- shared parts of the feed-forward operators (norm.cu, linear.cu):
+// element types, 8-element vector access, activations and their derivatives.
+// The translation units that include it are compiled with multiply-add
+// contraction on (their results are rounded once, to a stored type; nothing
+// here is held to another implementation bit for bit).
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "ttc_internal.cuh"
+
+namespace ttc {
+
+inline int dtype_size(int dtype) {
+    return dtype == TTC_F32 ? 4 : dtype == TTC_F16 || dtype == TTC_BF16 ? 2 : dtype == TTC_E4M3 ? 1 : 0;
+}
+inline const char* dtype_name(int dtype) {
+    return dtype == TTC_F32 ? "f32" : dtype == TTC_F16 ? "f16" : dtype == TTC_BF16 ? "bf16" : dtype == TTC_E4M3 ? "e4m3" : "?";
+}
+
+// The library launches on its own device whatever device the caller has
+// current, and leaves the caller's device as it found it.
+class DeviceGuard {
+   public:
+    DeviceGuard() {
+        if (cudaGetDevice(&prev_) != cudaSuccess) prev_ = -1;
+        if (prev_ != rt().device) cudaSetDevice(rt().device);
+    }
+    ~DeviceGuard() {
+        if (prev_ >= 0 && prev_ != rt().device) cudaSetDevice(prev_);
+    }
+
+   private:
+    int prev_ = -1;
+};
+
+// Checks of one tensor argument: set (or optional), aligned to its elements,
+// rows that do not overlap. Status code, with the message in ttc_last_error().
+inline int check_tensor(const char* op, const char* name, const void* p, int dtype, long long ld, long long width,
+                        bool needed) {
+    if (!p)
+        return needed ? set_error(TTC_ERR_INVALID_ARGUMENT, "tt_cuda: %s: %s is NULL", op, name) : TTC_OK;
+    if ((uintptr_t)p % dtype_size(dtype))
+        return set_error(TTC_ERR_INVALID_ARGUMENT, "tt_cuda: %s: %s (%p) is not aligned to its %d-byte elements", op,
+                         name, p, dtype_size(dtype));
+    if (ld < width)
+        return set_error(TTC_ERR_INVALID_ARGUMENT, "tt_cuda: %s: leading dimension %lld of %s is below its width %lld",
+                         op, ld, name, width);
+    return TTC_OK;
+}
+
+inline size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
+
+// True when rows of 8 elements of `p` can be read with 16-byte accesses (two
+// for fp32): address and row pitch on 16-byte boundaries (8 for e4m3, whose
+// 8 elements are one 8-byte access).
+inline bool vec8_ok(const void* p, int dtype, long long ld) {
+    const int a = dtype == TTC_E4M3 ? 8 : 16;
+    return p == nullptr || ((uintptr_t)p % a == 0 && (ld * dtype_size(dtype)) % a == 0);
+}
+
+int check_workspace(const char* op, const void* ws, size_t have, size_t need);
+// out[c] = sum over b < n of partials[b][c], in a fixed order, stored as dtype.
+int launch_sum_partials(const float* partials, int n, int cols, void* out, int dtype, cudaStream_t st);
+
+// ------------------------------------------------------------------ products
+// One product C [M, N] = sum over `segs` segments of A_s [M, K] B_s [K, N], or
+// (gated) the two products A B_0 and A B_1, with what happens to it on the way
+// out. mn_major: stored with the M (A) or N (B) index contiguous.
+struct Operand {
+    const void* ptr;
+    long long ld;
+};
+struct ProductEpilogue {
+    void* out;
+    void* out2;       // with split: the part of the output from `split` on
+    long long ldo;
+    int out_dtype;    // of out, bias, residual, pre
+    int act;
+    const void* bias;
+    const void* residual;
+    long long ldr;
+    void* pre;        // linear: the value before the activation
+    void* gate;       // gated: the two products
+    void* up;
+    long long ldp;    // of pre, gate and up
+    const float* row_scales;
+    const float* col_scales[2];
+    int split_rows;   // > 0: rows from here on go to out2 ...
+    int split_cols;   // (or columns, with > 0 here)
+    int split_skip;   // ... after this many that go nowhere
+    unsigned vec;     // bit i: 16-byte accesses (kVec*)
+};
+enum { kVecOut = 1, kVecOut2 = 2, kVecBias = 4, kVecResidual = 8, kVecPre = 16, kVecGate = 32, kVecUp = 64 };
+struct Product {
+    int M, N, K;
+    int dtype;  // of A and B
+    int segs, gated;
+    int a_mn, b_mn;
+    Operand a[2], b[2];
+    ProductEpilogue epi;
+};
+// Runs it on the library stream. `scratch` (256-byte aligned) holds the padded
+// copies of operands that cannot be read in place, of product_scratch() bytes.
+int run_product(const Product& p, void* scratch);
+size_t product_scratch(const Product& p);
+
+#ifdef __CUDACC__
+
+template <class T>
+__device__ __forceinline__ float to_f32(T v);
+template <>
+__device__ __forceinline__ float to_f32<float>(float v) {
+    return v;
+}
+template <>
+__device__ __forceinline__ float to_f32<__half>(__half v) {
+    return __half2float(v);
+}
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) {
+    return __bfloat162float(v);
+}
+template <>
+__device__ __forceinline__ float to_f32<__nv_fp8_e4m3>(__nv_fp8_e4m3 v) {
+    return (float)v;
+}
+template <class T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) {
+    return v;
+}
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) {
+    return __float2half_rn(v);
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
+    return __float2bfloat16_rn(v);
+}
+template <>
+__device__ __forceinline__ __nv_fp8_e4m3 from_f32<__nv_fp8_e4m3>(float v) {
+    return __nv_fp8_e4m3(v);  // nearest even, saturating at +-448, NaN stays NaN
+}
+
+// Eight consecutive elements; n < 8 or `vec` false takes them one by one
+// (elements past n read as 0 and are not stored).
+template <class T>
+__device__ __forceinline__ void load8(const T* p, int n, bool vec, float (&v)[8]) {
+    if (vec && n >= 8) {
+        if constexpr (sizeof(T) == 4) {
+            const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        } else if constexpr (sizeof(T) == 2) {
+            const uint4 a = *reinterpret_cast<const uint4*>(p);
+            const T* e = reinterpret_cast<const T*>(&a);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(e[i]);
+        } else {
+            const uint2 a = *reinterpret_cast<const uint2*>(p);
+            const T* e = reinterpret_cast<const T*>(&a);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(e[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32<T>(p[i]) : 0.0f;
+    }
+}
+template <class T>
+__device__ __forceinline__ void store8(T* p, int n, bool vec, const float (&v)[8]) {
+    if (vec && n >= 8) {
+        if constexpr (sizeof(T) == 4) {
+            *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+            alignas(16) T e[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(v[i]);
+            if constexpr (sizeof(T) == 2)
+                *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(e);
+            else
+                *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(e);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) p[i] = from_f32<T>(v[i]);
+    }
+}
+
+// The same with the type chosen at run time (one branch per 8 elements, the
+// same way for every thread of a launch).
+__device__ __forceinline__ void load8_as(int dtype, const void* base, long long i, int n, bool vec, float (&v)[8]) {
+    if (dtype == TTC_BF16)
+        load8(static_cast<const __nv_bfloat16*>(base) + i, n, vec, v);
+    else if (dtype == TTC_F16)
+        load8(static_cast<const __half*>(base) + i, n, vec, v);
+    else
+        load8(static_cast<const float*>(base) + i, n, vec, v);
+}
+__device__ __forceinline__ void store8_as(int dtype, void* base, long long i, int n, bool vec, const float (&v)[8]) {
+    if (dtype == TTC_BF16)
+        store8(static_cast<__nv_bfloat16*>(base) + i, n, vec, v);
+    else if (dtype == TTC_F16)
+        store8(static_cast<__half*>(base) + i, n, vec, v);
+    else
+        store8(static_cast<float*>(base) + i, n, vec, v);
+}
+
+// Activations in fp32. __expf and __fdividef are good to a few 2^-23, far
+// below the 2^-8 .. 2^-11 of the types the results are rounded to; an fp32
+// result of the products carries their accumulation error already.
+__device__ __forceinline__ float sigmoid_f32(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
+constexpr float kGeluTanhScale = 1.5957691216057308f;  // 2 sqrt(2 / pi): (1 + tanh t) / 2 = sigmoid(2 t)
+__device__ __forceinline__ float activate(int act, float z) {
+    switch (act) {
+        case TTC_ACT_RELU: return z < 0.0f ? 0.0f : z;
+        case TTC_ACT_SILU: return z * sigmoid_f32(z);
+        case TTC_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+        case TTC_ACT_GELU_TANH: return z * sigmoid_f32(kGeluTanhScale * (z + 0.044715f * z * z * z));
+        default: return z;
+    }
+}
+// The activation and its derivative.
+__device__ __forceinline__ void activate_grad(int act, float z, float& a, float& da) {
+    switch (act) {
+        case TTC_ACT_RELU:
+            a = z < 0.0f ? 0.0f : z;
+            da = z > 0.0f ? 1.0f : 0.0f;
+            break;
+        case TTC_ACT_SILU: {
+            const float p = sigmoid_f32(z);
+            a = z * p;
+            da = p + a * (1.0f - p);
+            break;
+        }
+        case TTC_ACT_GELU: {
+            const float cdf = 0.5f * (1.0f + erff(z * 0.70710678118654752f));
+            a = z * cdf;
+            da = cdf + z * 0.39894228040143268f * __expf(-0.5f * z * z);
+            break;
+        }
+        case TTC_ACT_GELU_TANH: {
+            const float p = sigmoid_f32(kGeluTanhScale * (z + 0.044715f * z * z * z));
+            a = z * p;
+            // p (1 - p) is 0 in fp32 long before |z| = 16; past that z^2 would
+            // overflow and 0 * inf make a NaN of a slope that is 0 or 1.
+            const float zc = fminf(fmaxf(z, -16.0f), 16.0f);
+            da = p + zc * p * (1.0f - p) * kGeluTanhScale * (1.0f + 0.134145f * zc * zc);
+            break;
+        }
+        default:
+            a = z;
+            da = 1.0f;
+    }
+}
+
+// Eight consecutive columns of one row of a product, col < N, n = columns left.
+__device__ __forceinline__ void finish_linear(const ProductEpilogue& e, int row, int col, int N, float (&v)[8]) {
+    int n = N - col < 8 ? N - col : 8;
+    if (e.row_scales) {
+        const float rs = __ldg(e.row_scales + row);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) v[i] = v[i] * rs * __ldg(e.col_scales[0] + col + i);
+    }
+    float t[8];
+    if (e.bias) {
+        load8_as(e.out_dtype, e.bias, col, n, e.vec & kVecBias, t);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += t[i];
+    }
+    if (e.pre) store8_as(e.out_dtype, e.pre, row * e.ldp + col, n, e.vec & kVecPre, v);
+    if (e.act != TTC_ACT_NONE) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = activate(e.act, v[i]);
+    }
+    if (e.residual) {
+        load8_as(e.out_dtype, e.residual, row * e.ldr + col, n, e.vec & kVecResidual, t);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += t[i];
+    }
+    void* out = e.out;
+    bool vec = e.vec & kVecOut;
+    long long r = row, c = col;
+    if (e.split_rows > 0 && row >= e.split_rows) {
+        r -= e.split_rows + e.split_skip;
+        if (r < 0) return;
+        out = e.out2;
+        vec = e.vec & kVecOut2;
+    } else if (e.split_cols > 0) {  // split_cols + split_skip is a multiple of 8: no group straddles it
+        if (col >= e.split_cols + e.split_skip) {
+            out = e.out2;
+            vec = e.vec & kVecOut2;
+            c -= e.split_cols + e.split_skip;
+        } else if (col + n > e.split_cols) {
+            n = e.split_cols - col;
+        }
+    }
+    store8_as(e.out_dtype, out, r * e.ldo + c, n, vec, v);
+}
+// The same columns of the two products of a gated pair.
+__device__ __forceinline__ void finish_gated(const ProductEpilogue& e, int row, int col, int N, float (&g)[8],
+                                             float (&u)[8]) {
+    const int n = N - col < 8 ? N - col : 8;
+    if (e.row_scales) {
+        const float rs = __ldg(e.row_scales + row);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) {
+                g[i] = g[i] * rs * __ldg(e.col_scales[0] + col + i);
+                u[i] = u[i] * rs * __ldg(e.col_scales[1] + col + i);
+            }
+    }
+    if (e.gate) {
+        store8_as(e.out_dtype, e.gate, row * e.ldp + col, n, e.vec & kVecGate, g);
+        store8_as(e.out_dtype, e.up, row * e.ldp + col, n, e.vec & kVecUp, u);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) g[i] = activate(e.act, g[i]) * u[i];
+    store8_as(e.out_dtype, e.out, row * e.ldo + col, n, e.vec & kVecOut, g);
+}
+#endif  // __CUDACC__
+
+}  // namespace ttc
