@@ -292,7 +292,7 @@ def test_rms_norm_gradient_against_differences(lib):
 # --------------------------------------------------------------------------------------------------- products
 SHAPES = [(1, 64, 64), (1, 1024, 512), (3, 8, 8), (2, 136, 1000), (16, 256, 320), (17, 200, 72), (33, 129, 257),
           (64, 512, 128), (77, 1000, 264), (130, 384, 520), (256, 1024, 512), (300, 1, 1), (1, 1, 4096), (513, 264, 136),
-          (1000, 776, 200)]
+          (1000, 776, 200), (1300, 4104, 136), (2304, 2080, 72)]
 
 
 def product_inputs(g, M, N, K, dtype, trans_w, pad, shift, weights=("w",), scale=None):
@@ -762,6 +762,30 @@ def test_results_do_not_change_from_call_to_call(lib):
         again = run_block(lib, t, M, D, H, {})
         for k, v in first.items():
             assert torch.equal(again[k], v), k
+
+
+@pytest.mark.parametrize("M,N,K", [(4, 256, 512), (2048, 2560, 256)])
+@pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
+def test_wait_expiry_is_reported_and_the_context_stays_usable(lib, monkeypatch, M, N, K, dtype):
+    """Both product kernels with their loads left out (TTC_TEST_STALL=linear: nothing
+    is ever in flight): the bounded waits run out after about a millisecond, the
+    next synchronisation reports it, and the same call then runs."""
+    g = gen(6)
+    x, (w,), xv, (wv,), xs, (ws,) = product_inputs(g, M, N, K, dtype, True, 0, 0)
+    y = Mat(M, N, "bf16")
+    d = lib.linear_desc(M, N, K, x.ptr, K, w.ptr, K, y.ptr, N, lib.DTYPES[dtype], y_dtype=lib.BF16, trans_w=True,
+                        x_scales=ptr(xs), w_scales=ptr(ws))
+    torch.cuda.synchronize()
+    monkeypatch.setenv("TTC_TEST_STALL", "linear")
+    lib.linear(d)
+    with pytest.raises(lib.TTCError) as e:
+        lib.synchronize()
+    assert e.value.code == lib.ERR_TIMEOUT and "bounded wait expired" in str(e.value)
+    monkeypatch.delenv("TTC_TEST_STALL")
+    lib.synchronize()
+    lib.linear(d)
+    z, dz = product64(xv, wv)
+    within(y.t, z, (U["bf16"] + 2.0 ** -23) * z.abs() + dz + TINY["bf16"], "y")
 
 
 def test_library_buffers_in_sixteen_bits(ttc):

@@ -38,10 +38,10 @@ NVCC_FLAGS = ARCH + ["-O3", "-lineinfo", "-std=c++17", "-fmad=false", "-Xcompile
                      "--expt-relaxed-constexpr", "-I" + INCLUDE, "-I" + CSRC, "-I" + OBJ]
 
 CUDA_SOURCES = ["runtime.cu", "chain.cu", "chain_tma.cu", "chain_jit.cu", "transpose.cu", "gemm_ffma.cu", "gemm_tc.cu", "norm.cu",
-                "linear.cu"]
+                "linear.cu", "linear_tc.cu"]
 # Nothing in these is compared bit for bit with another implementation: the
 # compiler may contract multiply-adds.
-FMAD_SOURCES = {"norm.cu", "linear.cu"}
+FMAD_SOURCES = {"norm.cu", "linear.cu", "linear_tc.cu"}
 CPP_SOURCES = ["comm.cpp"]
 
 

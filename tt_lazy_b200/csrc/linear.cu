@@ -1,6 +1,7 @@
 // linear.cu -- the products of a feed-forward block (ttc_linear,
 // ttc_gated_linear) and their gradients: argument checks, the element-wise
-// half of the backward passes, and the products each call is made of.
+// half of the backward passes, and the products each call is made of (the
+// products themselves: linear_tc.cu).
 #include <algorithm>
 #include <cstring>
 
@@ -424,87 +425,7 @@ int plan_gated_backward(const ttc_gated_linear_backward_desc& d, void* ws, size_
     return d.dwg ? run_product(pw, scratch) : TTC_OK;
 }
 
-// ------------------------------------------------------------------ product
-// 64 x 64 tile, 16 deep, 4 x 4 results a thread, fp32.
-constexpr int kTile = 64, kDeep = 16;
-
-__device__ __forceinline__ float element(int dtype, const void* p, long long i) {
-    if (dtype == TTC_BF16) return to_f32(static_cast<const __nv_bfloat16*>(p)[i]);
-    if (dtype == TTC_F16) return to_f32(static_cast<const __half*>(p)[i]);
-    return to_f32(static_cast<const __nv_fp8_e4m3*>(p)[i]);
-}
-
-__global__ void __launch_bounds__(256) product_kernel(const __grid_constant__ Product p) {
-    __shared__ float as[kDeep][kTile + 1], bs[2][kDeep][kTile + 1];
-    __shared__ float cs[2][kTile][kTile + 1];
-    const long long m0 = (long long)blockIdx.y * kTile, n0 = (long long)blockIdx.x * kTile;
-    const int tm = threadIdx.x / 16, tn = threadIdx.x % 16;
-    float acc[2][4][4] = {};
-    const int nb = p.gated ? 2 : 1;
-    for (int s = 0; s < p.segs; ++s)
-        for (int k0 = 0; k0 < p.K; k0 += kDeep) {
-            for (int i = threadIdx.x; i < kDeep * kTile; i += 256) {
-                const int kk = p.a_mn ? i / kTile : i % kDeep, mm = p.a_mn ? i % kTile : i / kDeep;
-                const long long m = m0 + mm, k = k0 + kk;
-                as[kk][mm] = m < p.M && k < p.K
-                                 ? element(p.dtype, p.a[s].ptr, p.a_mn ? k * p.a[s].ld + m : m * p.a[s].ld + k)
-                                 : 0.0f;
-            }
-            for (int b = 0; b < nb; ++b) {
-                const Operand& o = p.b[p.gated ? b : s];
-                for (int i = threadIdx.x; i < kDeep * kTile; i += 256) {
-                    const int kk = p.b_mn ? i / kTile : i % kDeep, nn = p.b_mn ? i % kTile : i / kDeep;
-                    const long long n = n0 + nn, k = k0 + kk;
-                    bs[b][kk][nn] = n < p.N && k < p.K
-                                        ? element(p.dtype, o.ptr, p.b_mn ? k * o.ld + n : n * o.ld + k)
-                                        : 0.0f;
-                }
-            }
-            __syncthreads();
-            for (int b = 0; b < nb; ++b)
-                for (int kk = 0; kk < kDeep; ++kk)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            acc[b][i][j] += as[kk][tm * 4 + i] * bs[b][kk][tn * 4 + j];
-            __syncthreads();
-        }
-    for (int b = 0; b < nb; ++b)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) cs[b][tm * 4 + i][tn * 4 + j] = acc[b][i][j];
-    __syncthreads();
-    for (int i = threadIdx.x; i < kTile * kTile / 8; i += 256) {
-        const int mm = i / (kTile / 8), nn = i % (kTile / 8) * 8;
-        const long long m = m0 + mm, n = n0 + nn;
-        if (m >= p.M || n >= p.N) continue;
-        float v[8], u[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            v[j] = cs[0][mm][nn + j];
-            u[j] = cs[1][mm][nn + j];
-        }
-        if (p.gated)
-            finish_gated(p.epi, (int)m, (int)n, p.N, v, u);
-        else
-            finish_linear(p.epi, (int)m, (int)n, p.N, v);
-    }
-}
-
 }  // namespace
-
-size_t product_scratch(const Product&) { return 0; }
-
-int run_product(const Product& p, void*) {
-    const long long my = ((long long)p.M + kTile - 1) / kTile;
-    if (my > 65535) return set_error(TTC_ERR_UNSUPPORTED, "tt_cuda: too many rows");
-    product_kernel<<<dim3((unsigned)((p.N + kTile - 1) / kTile), (unsigned)my), 256, 0, rt().stream>>>(p);
-    count_launch();
-    return check_cuda(cudaGetLastError(), "product launch");
-}
-
 }  // namespace ttc
 
 using namespace ttc;

@@ -1,0 +1,707 @@
+// linear_tc.cu -- the matrix products of ttc_linear, ttc_gated_linear and their
+// gradients on the 5th-generation tensor cores: tcgen05.mma kind::f16 (F16 and
+// BF16 operands) or kind::f8f6f4 (E4M3), fp32 accumulators in tensor memory,
+// operands staged by TMA, the epilogue on the way out.
+//
+// Two kernels:
+//   pair_kernel   large products: persistent CTA pairs (cta_group::2), one
+//                 256 x 256 tile a pair, operands in a ring of 6 stages.
+//   tile_kernel   few rows of x (single tokens, small batches): one 128-wide
+//                 tile of the weight's output columns against up to 256 rows,
+//                 the weight as the 128-row operand of the instruction, the
+//                 sum over K split over the CTAs of a cluster and joined
+//                 through distributed shared memory.
+//
+// Both stage 128 bytes of K a row (64 16-bit or 128 8-bit elements), in the
+// 128-byte swizzle, four instructions a stage. An operand whose rows are
+// contiguous along K comes as one box; one that is contiguous along M or N (a
+// transposed 16-bit operand) as boxes of 64 columns x 64 k-rows.
+//
+// The gated product is one kernel: the tile's columns are half gate and half
+// up columns of the same outputs, so both accumulators of an output are in the
+// same tile and the activation and the product happen in the epilogue. A
+// product over two segments (dx = dg Wg^T + du Wu^T) runs the k-blocks of the
+// second pair of operands after the first's into the same accumulator.
+//
+// Every wait is bounded, as in the TF32 kernels: an expired one is recorded in
+// the status word, the other roles run out too, and the kernel frees what it
+// holds and returns. No TMA load is multicast.
+#include <algorithm>
+#include <cstring>
+
+#include "ffn.cuh"
+#include "tc_util.cuh"
+
+namespace ttc {
+namespace {
+
+constexpr int kThreads = 192;  // warp 0: TMA, warp 1: MMA, warps 2-5: epilogue
+constexpr int kRow = 128;      // bytes of K a stage holds of each row
+constexpr int kBox = 64 * kRow;  // an MN-major box: 64 k-rows of 64 16-bit columns
+
+struct alignas(64) ProductParams {
+    CUtensorMap a[2], b[2];
+    Product p;
+    int kb_seg, kb_total;  // k-blocks of one segment, of all segments
+    int m_tiles, n_tiles;
+    int tok, stages, splits;  // tile_kernel: rows of x a tile, ring stages, CTAs that share a tile
+    unsigned idesc;
+    int* status;
+    long long wait_limit;
+    int stall;
+};
+
+template <int GROUP, bool F8>
+__device__ __forceinline__ void mma(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                    uint32_t accumulate) {
+#define TTC_MMA(GROUP_TEXT, KIND_TEXT)                                                                          \
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma." GROUP_TEXT "." KIND_TEXT         \
+                 " [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),                                                  \
+                 "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)                                            \
+                 : "memory")
+    if constexpr (GROUP == 2 && F8)
+        TTC_MMA("cta_group::2", "kind::f8f6f4");
+    else if constexpr (GROUP == 2)
+        TTC_MMA("cta_group::2", "kind::f16");
+    else if constexpr (F8)
+        TTC_MMA("cta_group::1", "kind::f8f6f4");
+    else
+        TTC_MMA("cta_group::1", "kind::f16");
+#undef TTC_MMA
+}
+
+__device__ __forceinline__ void tc_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+
+// How the four instructions of a stage walk an operand's tile. K-major: groups
+// of 8 rows every 1024 bytes, each instruction 32 bytes further along the row.
+// MN-major: boxes of 64 columns (leading offset kBox), groups of 8 k-rows every
+// 1024 bytes, each instruction 16 k-rows = 2048 bytes further.
+struct Walk {
+    uint32_t lbo, step;
+};
+__device__ __forceinline__ Walk walk_of(int mn) { return mn ? Walk{kBox, 2048} : Walk{16, 32}; }
+__device__ __forceinline__ uint64_t walk_desc(uint32_t base, const Walk& w, int i) {
+    return make_desc(base + i * w.step, w.lbo, 1024, kLayoutSW128);
+}
+
+// `rows` rows (an operand's M or N index, from row0) of k-block kb.
+__device__ __forceinline__ void load_rows(uint32_t dst, const CUtensorMap* map, uint32_t bar, int mn, int kb, int bk,
+                                          int row0, int rows) {
+    if (!mn) {
+        tma_load_2d(dst, map, bar, kb * bk, row0);
+    } else {
+        for (int j = 0; j < rows; j += 64) tma_load_2d(dst + j * kRow, map, bar, row0 + j, kb * bk);
+    }
+}
+
+// ---------------------------------------------------------------- pair kernel
+constexpr int kStages = 6;
+constexpr int kHalf = 128 * kRow;       // one CTA's rows of A, or of B: 16 KB
+constexpr int kStageBytes = 2 * kHalf;  // 32 KB
+constexpr int kStaging = 32 * 64 * 4;   // one epilogue warp's 32 rows x 64 fp32
+constexpr int kPairSmem = kStages * kStageBytes + 4 * kStaging + 1024 + 256;
+static_assert(kPairSmem <= 232448, "pair kernel: shared memory");
+constexpr int kGroupM = 8;  // pair tiles of M that are walked together, so that their operands stay in L2
+
+__device__ __forceinline__ void pair_coords(int tile, int m_tiles, int n_tiles, int& mt, int& nt) {
+    const int per_group = kGroupM * n_tiles;
+    const int group = tile / per_group, first = group * kGroupM;
+    const int rows = min(kGroupM, m_tiles - first), local = tile - group * per_group;
+    mt = first + local % rows;
+    nt = local / rows;
+}
+
+// CTA r of a pair holds rows 128 r .. of the A tile and columns 128 r .. of the
+// B tile (gated: the gate columns for r = 0, the up columns for r = 1) and gets
+// its 128 rows x 256 columns of the result in its own tensor memory, two
+// accumulators deep, so that the epilogue of one tile runs under the next.
+//
+// Epilogue: tensor memory hands each lane one row; the rows go through shared
+// memory (16-byte chunks xored with the row, conflict-free both ways), so that
+// a warp reads the residual and writes the output in whole 128-byte lines.
+template <bool F8>
+__global__ void __launch_bounds__(kThreads, 1) pair_kernel(const __grid_constant__ ProductParams q) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint8_t* staging = smem + kStages * kStageBytes;
+    uint64_t* bars = (uint64_t*)(staging + 4 * kStaging);
+    uint32_t* tmem_slot = (uint32_t*)(bars + 2 * kStages + 4);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    const uint32_t sbase = smem_u32(smem), bar0 = smem_u32(bars);
+    auto full_bar = [&](int s) { return bar0 + 8u * s; };
+    auto empty_bar = [&](int s) { return bar0 + 8u * (kStages + s); };
+    auto tfull_bar = [&](int b) { return bar0 + 8u * (2 * kStages + b); };
+    auto tempty_bar = [&](int b) { return bar0 + 8u * (2 * kStages + 2 + b); };
+    const Product& p = q.p;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(full_bar(s), rank == 0 ? 2 : 1);  // CTA 0: its own producer and the peer's forward
+            mbar_init(empty_bar(s), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(tfull_bar(b), 1);
+            mbar_init(tempty_bar(b), 8);
+        }
+        mbar_fence_init();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                     "r"(512)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();  // both CTAs' barriers are initialised before anyone signals across
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const int num_tiles = q.m_tiles * q.n_tiles;
+    const int cluster_id = blockIdx.x >> 1, nclusters = gridDim.x >> 1;
+    bool failed = false;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            constexpr int bk = F8 ? 128 : 64;
+            int stage = 0;
+            uint32_t phase = 0;
+            long long issued = 0;
+            for (int tile = cluster_id; tile < num_tiles && !failed && !q.stall; tile += nclusters) {
+                int mt, nt;
+                pair_coords(tile, q.m_tiles, q.n_tiles, mt, nt);
+                const int row0 = mt * 256 + (int)rank * 128;
+                const int col0 = p.gated ? nt * 128 : nt * 256 + (int)rank * 128;
+                for (int kb = 0; kb < q.kb_total; ++kb) {
+                    if (!mbar_wait(empty_bar(stage), phase ^ 1, q.wait_limit)) {
+                        failed = true;
+                        break;
+                    }
+                    const int seg = kb >= q.kb_seg, k = kb - (seg ? q.kb_seg : 0);
+                    mbar_arrive_expect_tx(full_bar(stage), kStageBytes);
+                    const uint32_t a_dst = sbase + stage * kStageBytes;
+                    load_rows(a_dst, &q.a[seg], full_bar(stage), p.a_mn, k, bk, row0, 128);
+                    load_rows(a_dst + kHalf, &q.b[p.gated ? rank : seg], full_bar(stage), p.b_mn, k, bk, col0, 128);
+                    ++issued;
+                    if (++stage == kStages) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                }
+            }
+            // Never leave with loads in flight.
+            const long long last = issued < kStages ? issued : kStages;
+            for (long long i = 0; i < last; ++i) {
+                const long long n = issued - 1 - i;
+                if (!mbar_wait(full_bar((int)(n % kStages)), (uint32_t)((n / kStages) & 1), q.wait_limit)) failed = true;
+            }
+        }
+    } else if (warp == 1 && rank == 1) {
+        if (lane == 0) {
+            // forward every completed stage of this CTA to CTA 0's full barrier
+            int stage = 0;
+            uint32_t phase = 0;
+            for (int tile = cluster_id; tile < num_tiles && !failed; tile += nclusters) {
+                for (int kb = 0; kb < q.kb_total; ++kb) {
+                    if (!mbar_wait(full_bar(stage), phase, q.wait_limit)) {
+                        failed = true;
+                        break;
+                    }
+                    mbar_arrive_cluster_relaxed(cluster_addr(full_bar(stage), 0));
+                    if (++stage == kStages) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            const Walk wa = walk_of(p.a_mn), wb = walk_of(p.b_mn);
+            int stage = 0;
+            uint32_t phase = 0;
+            int t = 0;
+            for (int tile = cluster_id; tile < num_tiles && !failed; tile += nclusters, ++t) {
+                const int b = t & 1;
+                if (!mbar_wait(tempty_bar(b), ((t >> 1) & 1) ^ 1, q.wait_limit)) {
+                    failed = true;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t d_tmem = tmem_base + (uint32_t)(b * 256);
+                for (int kb = 0; kb < q.kb_total; ++kb) {
+                    if (!mbar_wait(full_bar(stage), phase, q.wait_limit)) {
+                        failed = true;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t a_s = sbase + stage * kStageBytes, b_s = a_s + kHalf;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        mma<2, F8>(d_tmem, walk_desc(a_s, wa, i), walk_desc(b_s, wb, i), q.idesc, (kb | i) != 0);
+                    tc2_commit(cluster_addr(empty_bar(stage), 0));
+                    tc2_commit(cluster_addr(empty_bar(stage), 1));
+                    if (++stage == kStages) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                }
+                if (failed) break;
+                tc2_commit(cluster_addr(tfull_bar(b), 0));
+                tc2_commit(cluster_addr(tfull_bar(b), 1));
+            }
+        }
+    } else {
+        const int quarter = warp & 3;  // this warp's quarter of the 128 tensor-memory lanes
+        float4* const mine = reinterpret_cast<float4*>(staging + quarter * kStaging);
+        auto chunk = [&](int row, int c) -> float4& { return mine[row * 16 + (c ^ (row & 7))]; };
+        // two 16-byte chunks from c on, in the order that keeps 8 lanes on 8 different banks
+        auto take8 = [&](int row, int c, int flip, float (&v)[8]) {
+            const float4 x = chunk(row, c + flip), y = chunk(row, c + (flip ^ 1));
+            const float4 lo = flip ? y : x, hi = flip ? x : y;
+            v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w, v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
+        };
+        int t = 0;
+        for (int tile = cluster_id; tile < num_tiles; tile += nclusters, ++t) {
+            int mt, nt;
+            pair_coords(tile, q.m_tiles, q.n_tiles, mt, nt);
+            const int b = t & 1;
+            if (!__all_sync(0xffffffffu, mbar_wait(tfull_bar(b), (t >> 1) & 1, q.wait_limit))) {
+                failed = true;
+                break;
+            }
+            tc_fence_after();
+            const int row0 = mt * 256 + (int)rank * 128 + quarter * 32;
+            const int col0 = nt * (p.gated ? 128 : 256);
+            const uint32_t acc = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(b * 256);
+            for (int c = 0; c < 4; ++c) {
+                uint32_t r[2][32];
+                tc_ld_32x32b_x32(acc + (p.gated ? c * 32 : c * 64), r[0]);
+                tc_ld_32x32b_x32(acc + (p.gated ? 128 + c * 32 : c * 64 + 32), r[1]);
+                tc_wait_ld();
+                if (c == 3) {  // the accumulator is read: the MMA warp may start the tile after next
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(cluster_addr(tempty_bar(b), 0));
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        chunk(lane, h * 8 + j) =
+                            make_float4(__uint_as_float(r[h][4 * j]), __uint_as_float(r[h][4 * j + 1]),
+                                        __uint_as_float(r[h][4 * j + 2]), __uint_as_float(r[h][4 * j + 3]));
+                __syncwarp();
+                if (p.gated) {
+                    const int j = lane & 3, col = col0 + c * 32 + j * 8;
+#pragma unroll 1
+                    for (int i = 0; i < 4; ++i) {
+                        const int lr = i * 8 + (lane >> 2), row = row0 + lr;
+                        if (row < p.M && col < p.N) {
+                            float g[8], u[8];
+                            take8(lr, 2 * j, 0, g);
+                            take8(lr, 8 + 2 * j, 0, u);
+                            finish_gated(p.epi, row, col, p.N, g, u);
+                        }
+                    }
+                } else {
+                    const int j = lane & 7, col = col0 + c * 64 + j * 8;
+#pragma unroll 1
+                    for (int i = 0; i < 8; ++i) {
+                        const int lr = i * 4 + (lane >> 3), row = row0 + lr;
+                        if (row < p.M && col < p.N) {
+                            float v[8];
+                            take8(lr, 2 * j, j >> 2, v);
+                            finish_linear(p.epi, row, col, p.N, v);
+                        }
+                    }
+                }
+                __syncwarp();
+            }
+        }
+    }
+
+    if (failed) *(volatile int*)q.status = 1;
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();  // the pair's MMAs and signals are done before TMEM is freed or a CTA exits
+    tc_fence_after();
+    if (warp == 1)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512) : "memory");
+}
+
+// ---------------------------------------------------------------- tile kernel
+// One CTA: 128 output columns (gated: 64 outputs, their gate columns in the
+// first half and their up columns in the second) against `tok` rows of x, over
+// its share of the k-blocks. The accumulator's lanes are output columns and its
+// columns rows of x; it goes to shared memory as [row of x][128] over the ring,
+// where the CTAs of the cluster add up each other's shares in rank order, a
+// contiguous share of the outputs each.
+__device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
+
+template <bool F8>
+__global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ ProductParams q) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    const int stage_bytes = kHalf + q.tok * kRow, stages = q.stages;
+    uint64_t* bars = (uint64_t*)(smem + stages * stage_bytes);
+    uint32_t* tmem_slot = (uint32_t*)(bars + 2 * stages + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t sbase = smem_u32(smem), bar0 = smem_u32(bars);
+    auto full_bar = [&](int s) { return bar0 + 8u * s; };
+    auto empty_bar = [&](int s) { return bar0 + 8u * (stages + s); };
+    const uint32_t done_bar = bar0 + 8u * (2 * stages);
+    const Product& p = q.p;
+    const int splits = q.splits, split = splits > 1 ? (int)cluster_rank() : 0;
+    const int tile = blockIdx.x / splits;
+    const int m0 = tile % q.m_tiles * q.tok, n0 = tile / q.m_tiles * (p.gated ? 64 : 128);
+    const int kb0 = (int)((long long)q.kb_total * split / splits);
+    const int kb1 = (int)((long long)q.kb_total * (split + 1) / splits);
+    const uint32_t tmem_cols = q.tok < 32 ? 32 : q.tok;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < stages; ++s) {
+            mbar_init(full_bar(s), 1);
+            mbar_init(empty_bar(s), 1);
+        }
+        mbar_init(done_bar, 1);
+        mbar_fence_init();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                     "r"(tmem_cols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    bool failed = false;
+
+    if (warp == 0) {
+        if (lane == 0 && !q.stall) {
+            constexpr int bk = F8 ? 128 : 64;
+            int stage = 0;
+            uint32_t phase = 0;
+            int issued = 0;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!mbar_wait(empty_bar(stage), phase ^ 1, q.wait_limit)) {
+                    failed = true;
+                    break;
+                }
+                const int seg = kb >= q.kb_seg, k = kb - (seg ? q.kb_seg : 0);
+                const uint32_t dst = sbase + stage * stage_bytes, bar = full_bar(stage);
+                mbar_arrive_expect_tx(bar, stage_bytes);
+                if (p.gated) {
+                    load_rows(dst, &q.b[0], bar, p.b_mn, k, bk, n0, 64);
+                    load_rows(dst + kHalf / 2, &q.b[1], bar, p.b_mn, k, bk, n0, 64);
+                } else {
+                    load_rows(dst, &q.b[seg], bar, p.b_mn, k, bk, n0, 128);
+                }
+                load_rows(dst + kHalf, &q.a[seg], bar, p.a_mn, k, bk, m0, q.tok);
+                ++issued;
+                if (++stage == stages) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+            }
+            const int last = issued < stages ? issued : stages;  // never leave with loads in flight
+            for (int i = 0; i < last; ++i) {
+                const int n = issued - 1 - i;
+                if (!mbar_wait(full_bar(n % stages), (uint32_t)((n / stages) & 1), q.wait_limit)) failed = true;
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            const Walk ww = walk_of(p.b_mn), wx = walk_of(p.a_mn);
+            int stage = 0;
+            uint32_t phase = 0;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!mbar_wait(full_bar(stage), phase, q.wait_limit)) {
+                    failed = true;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t w_s = sbase + stage * stage_bytes, x_s = w_s + kHalf;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    mma<1, F8>(tmem_base, walk_desc(w_s, ww, i), walk_desc(x_s, wx, i), q.idesc, kb > kb0 || i > 0);
+                tc_commit(empty_bar(stage));
+                if (++stage == stages) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+            }
+            if (!failed) tc_commit(done_bar);
+        }
+    }
+    const int rows = min(q.tok, p.M - m0);
+    float* const part = reinterpret_cast<float*>(smem);
+    if (warp >= 2) {
+        const int quarter = warp & 3;
+        if (__all_sync(0xffffffffu, mbar_wait(done_bar, 0, q.wait_limit))) {
+            // every load has landed and every instruction has read its stage: the ring is free
+            tc_fence_after();
+            for (int c = 0; c < rows; c += 16) {
+                uint32_t r[16];
+                tc_ld_32x32b_x16(tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)c, r);
+                tc_wait_ld();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) part[(c + j) * 128 + quarter * 32 + lane] = __uint_as_float(r[j]);
+            }
+        } else {
+            failed = true;
+        }
+    }
+    if (failed) *(volatile int*)q.status = 1;
+    tc_fence_before();
+    __syncthreads();
+    if (splits > 1) cluster_sync();
+    tc_fence_after();
+    if (warp == 1)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(tmem_cols)
+                     : "memory");
+
+    const int groups = p.gated ? 8 : 16;  // of 8 columns
+    const int items = rows * groups, share = (items + splits - 1) / splits;
+    const int last = min(items, (split + 1) * share);
+    // 8 consecutive values of a row, added over the cluster's CTAs in rank order
+    auto take8 = [&](int row, int col, float (&v)[8]) {
+        if (splits == 1) {
+            const float4 lo = *reinterpret_cast<const float4*>(part + row * 128 + col);
+            const float4 hi = *reinterpret_cast<const float4*>(part + row * 128 + col + 4);
+            v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w, v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
+            return;
+        }
+        const uint32_t at = sbase + (uint32_t)(row * 128 + col) * 4u;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+#pragma unroll 4
+        for (int s = 0; s < splits; ++s) {
+            const uint32_t a = cluster_addr(at, s);
+            const float4 lo = ld_cluster(a), hi = ld_cluster(a + 16);
+            v[0] += lo.x, v[1] += lo.y, v[2] += lo.z, v[3] += lo.w, v[4] += hi.x, v[5] += hi.y, v[6] += hi.z, v[7] += hi.w;
+        }
+    };
+    for (int it = split * share + threadIdx.x; it < last; it += kThreads) {
+        const int row = it / groups, j = it % groups, col = n0 + j * 8;
+        if (col >= p.N) continue;
+        float v[8], u[8];
+        take8(row, j * 8, v);
+        if (p.gated) {
+            take8(row, 64 + j * 8, u);
+            finish_gated(p.epi, m0 + row, col, p.N, v, u);
+        } else {
+            finish_linear(p.epi, m0 + row, col, p.N, v);
+        }
+    }
+    if (splits > 1) {  // nobody leaves while its shared memory is still read
+        __syncwarp();
+        cluster_sync();
+    }
+}
+
+// ------------------------------------------------------------ padded operands
+// TMA wants 16-byte aligned addresses and row pitches. Other operands are
+// copied once per call, rows padded to 16 bytes (the padding is never read).
+bool aligned16(const Operand& o, int es) { return (uintptr_t)o.ptr % 16 == 0 && (o.ld * es) % 16 == 0; }
+
+struct Copy {
+    const void* src;
+    void* dst;
+    long long rows, cols, lds, ldd;
+};
+
+template <class T>
+__global__ void __launch_bounds__(256) pad_rows_kernel(const __grid_constant__ Copy c) {
+    for (long long r = blockIdx.x; r < c.rows; r += gridDim.x) {
+        const T* s = static_cast<const T*>(c.src) + r * c.lds;
+        T* d = static_cast<T*>(c.dst) + r * c.ldd;
+        for (long long i = threadIdx.x; i < c.cols; i += 256) d[i] = s[i];
+    }
+}
+
+// The operands of a product with their stored shapes.
+struct Stored {
+    const Operand* o;
+    long long rows, cols;  // as stored
+};
+int stored_operands(const Product& p, Stored (&s)[4]) {
+    int n = 0;
+    for (int i = 0; i < p.segs; ++i) s[n++] = {&p.a[i], p.a_mn ? p.K : p.M, p.a_mn ? p.M : p.K};
+    for (int i = 0; i < (p.gated ? 2 : p.segs); ++i) s[n++] = {&p.b[i], p.b_mn ? p.K : p.N, p.b_mn ? p.N : p.K};
+    return n;
+}
+long long padded_ld(long long cols, int es) { return (cols * es + 15) / 16 * 16 / es; }
+
+int make_map(CUtensorMap* map, const Product& p, const Operand& o, int width, bool mn, int box_rows) {
+    const bool f8 = p.dtype == TTC_E4M3;
+    const int es = dtype_size(p.dtype);
+    const unsigned long long dims[2] = {(unsigned long long)(mn ? width : p.K), (unsigned long long)(mn ? p.K : width)};
+    const unsigned long long strides[1] = {(unsigned long long)o.ld};
+    const unsigned box[2] = {(unsigned)(kRow / es), (unsigned)(mn ? 64 : box_rows)};
+    const CUtensorMapDataType type = f8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
+    return encode_tensor_map(map, type, es, o.ptr, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+unsigned instruction(const Product& p, bool a_mn, bool b_mn, int m, int n) {
+    const unsigned fmt = p.dtype == TTC_BF16 ? 1u : 0u;  // kind::f16: f16 0, bf16 1; kind::f8f6f4: e4m3 0
+    return (1u << 4) | (fmt << 7) | (fmt << 10) | ((unsigned)a_mn << 15) | ((unsigned)b_mn << 16) |
+           ((unsigned)(n >> 3) << 17) | ((unsigned)(m >> 4) << 24);
+}
+
+bool first_on_device(bool (&seen)[kMaxDevices]) {
+    bool& s = seen[rt().device];
+    const bool first = !s;
+    s = true;
+    return first;
+}
+
+template <bool F8>
+int launch_pair(ProductParams& q) {
+    static bool seen[kMaxDevices] = {};
+    static int most[kMaxDevices] = {};
+    cudaLaunchConfig_t cfg;
+    std::memset(&cfg, 0, sizeof cfg);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.dynamicSmemBytes = kPairSmem;
+    cfg.stream = rt().stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int& clusters = most[rt().device];
+    if (first_on_device(seen)) {
+        TTC_CUDA(cudaFuncSetAttribute(pair_kernel<F8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
+        cfg.gridDim = dim3(2 * (rt().sm_count / 2), 1, 1);
+        if (cudaOccupancyMaxActiveClusters(&clusters, pair_kernel<F8>, &cfg) != cudaSuccess || clusters < 1) {
+            cudaGetLastError();
+            clusters = rt().sm_count / 2;
+        }
+    }
+    const long long tiles = (long long)q.m_tiles * q.n_tiles;
+    cfg.gridDim = dim3(2u * (unsigned)std::min<long long>(tiles, clusters), 1, 1);
+    TTC_CUDA(cudaLaunchKernelEx(&cfg, pair_kernel<F8>, q));
+    count_launch();
+    return TTC_OK;
+}
+
+template <bool F8>
+int launch_tile(ProductParams& q) {
+    static bool seen[kMaxDevices] = {};
+    const int ring = q.stages * (kHalf + q.tok * kRow);
+    if (first_on_device(seen))
+        TTC_CUDA(cudaFuncSetAttribute(tile_kernel<F8>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448));
+    cudaLaunchConfig_t cfg;
+    std::memset(&cfg, 0, sizeof cfg);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)q.splits;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.dynamicSmemBytes = (size_t)ring + 1024 + 256;
+    cfg.stream = rt().stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = q.splits > 1 ? 1 : 0;
+    cfg.gridDim = dim3((unsigned)((long long)q.m_tiles * q.n_tiles * q.splits), 1, 1);
+    TTC_CUDA(cudaLaunchKernelEx(&cfg, tile_kernel<F8>, q));
+    count_launch();
+    return TTC_OK;
+}
+
+}  // namespace
+
+size_t product_scratch(const Product& p) {
+    Stored s[4];
+    const int n = stored_operands(p, s), es = dtype_size(p.dtype);
+    size_t bytes = 0;
+    for (int i = 0; i < n; ++i)
+        if (!aligned16(*s[i].o, es)) bytes += align256((size_t)s[i].rows * padded_ld(s[i].cols, es) * es);
+    return bytes;
+}
+
+int run_product(const Product& given, void* scratch) {
+    if (rt().device < 0 || rt().device >= kMaxDevices)
+        return set_error(TTC_ERR_UNSUPPORTED, "tt_cuda: device %d", rt().device);
+    ProductParams q;
+    std::memset(&q, 0, sizeof q);
+    Product& p = q.p;
+    p = given;
+    const int es = dtype_size(p.dtype), sms = rt().sm_count;
+    const bool f8 = p.dtype == TTC_E4M3;
+    Stored s[4];
+    const int n = stored_operands(p, s);
+    char* room = (char*)scratch;
+    for (int i = 0; i < n; ++i) {
+        if (aligned16(*s[i].o, es)) continue;
+        Operand& o = const_cast<Operand&>(*s[i].o);
+        const Copy c{o.ptr, room, s[i].rows, s[i].cols, o.ld, padded_ld(s[i].cols, es)};
+        const unsigned grid = (unsigned)std::min<long long>(c.rows, 16ll * sms);
+        if (f8)
+            pad_rows_kernel<uint8_t><<<grid, 256, 0, rt().stream>>>(c);
+        else
+            pad_rows_kernel<uint16_t><<<grid, 256, 0, rt().stream>>>(c);
+        count_launch();
+        if (int rc = check_cuda(cudaGetLastError(), "operand copy launch")) return rc;
+        o = {room, c.ldd};
+        room += align256((size_t)c.rows * c.ldd * es);
+    }
+    const int bk = kRow / es;
+    q.kb_seg = (p.K + bk - 1) / bk;
+    q.kb_total = q.kb_seg * p.segs;
+    if (int rc = device_status_ptr(&q.status)) return rc;
+    q.stall = stall_test("linear") ? 1 : 0;
+    q.wait_limit = q.stall ? kStallTestLimitCycles : kWaitLimitCycles;
+    const int nb = p.gated ? 2 : p.segs;
+
+    const long long pair_m = ((long long)p.M + 255) / 256, pair_n = ((long long)p.N + (p.gated ? 127 : 255)) / (p.gated ? 128 : 256);
+    if (pair_m * pair_n > INT32_MAX / 2) return set_error(TTC_ERR_UNSUPPORTED, "tt_cuda: too many output tiles");
+    if (p.M > 256 && pair_m * pair_n >= sms / 2) {
+        q.m_tiles = (int)pair_m;
+        q.n_tiles = (int)pair_n;
+        q.idesc = instruction(p, p.a_mn, p.b_mn, 256, 256);
+        for (int i = 0; i < p.segs; ++i)
+            if (int rc = make_map(&q.a[i], p, p.a[i], p.M, p.a_mn, 128)) return rc;
+        for (int i = 0; i < nb; ++i)
+            if (int rc = make_map(&q.b[i], p, p.b[i], p.N, p.b_mn, 128)) return rc;
+        return f8 ? launch_pair<true>(q) : launch_pair<false>(q);
+    }
+
+    q.tok = p.a_mn ? 64 : 16;
+    while (q.tok < p.M && q.tok < 256) q.tok *= 2;
+    q.n_tiles = (p.N + (p.gated ? 63 : 127)) / (p.gated ? 64 : 128);
+    q.m_tiles = (p.M + q.tok - 1) / q.tok;
+    const long long tiles = (long long)q.m_tiles * q.n_tiles;
+    q.splits = 1;
+    while (q.splits < 8 && tiles * q.splits * 2 <= 2 * sms && q.kb_total >= 4 * q.splits) q.splits *= 2;
+    // two CTAs an SM up to 64 rows, one above
+    const int stage_bytes = kHalf + q.tok * kRow;
+    q.stages = (q.tok <= 64 ? 96 * 1024 : 192 * 1024) / stage_bytes;
+    q.idesc = instruction(p, p.b_mn, p.a_mn, 128, q.tok);
+    for (int i = 0; i < p.segs; ++i)
+        if (int rc = make_map(&q.a[i], p, p.a[i], p.M, p.a_mn, q.tok)) return rc;
+    for (int i = 0; i < nb; ++i)
+        if (int rc = make_map(&q.b[i], p, p.b[i], p.N, p.b_mn, p.gated ? 64 : 128)) return rc;
+    return f8 ? launch_tile<true>(q) : launch_tile<false>(q);
+}
+
+}  // namespace ttc

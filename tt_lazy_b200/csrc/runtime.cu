@@ -60,8 +60,9 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-int encode_tensor_map_f32(CUtensorMap* map, const void* ptr, int rank, const unsigned long long* dims,
-                          const unsigned long long* strides_elems, const unsigned* box, CUtensorMapSwizzle swizzle) {
+int encode_tensor_map(CUtensorMap* map, CUtensorMapDataType type, int elem_bytes, const void* ptr, int rank,
+                      const unsigned long long* dims, const unsigned long long* strides_elems, const unsigned* box,
+                      CUtensorMapSwizzle swizzle) {
     static EncodeTiledFn fn = nullptr;
     if (!fn) {
         void* p = nullptr;
@@ -80,15 +81,20 @@ int encode_tensor_map_f32(CUtensorMap* map, const void* ptr, int rank, const uns
         d[i] = dims[i];
         b[i] = box[i];
         e[i] = 1;
-        if (i + 1 < rank) s[i] = strides_elems[i] * 4;
+        if (i + 1 < rank) s[i] = strides_elems[i] * elem_bytes;
     }
-    CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, (cuuint32_t)rank, const_cast<void*>(ptr), d, s, b, e,
+    CUresult r = fn(map, type, (cuuint32_t)rank, const_cast<void*>(ptr), d, s, b, e,
                     CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS)
         return set_error(TTC_ERR_CUDA, "tt_cuda: cuTensorMapEncodeTiled failed (%d): rank %d, dims %llu x %llu", (int)r,
                          rank, (unsigned long long)d[0], rank > 1 ? (unsigned long long)d[1] : 1ull);
     return TTC_OK;
+}
+
+int encode_tensor_map_f32(CUtensorMap* map, const void* ptr, int rank, const unsigned long long* dims,
+                          const unsigned long long* strides_elems, const unsigned* box, CUtensorMapSwizzle swizzle) {
+    return encode_tensor_map(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, ptr, rank, dims, strides_elems, box, swizzle);
 }
 
 // A host-mapped status word that kernels with bounded waits set when a wait

@@ -12,7 +12,10 @@
 namespace ttc {
 
 // cuTensorMapEncodeTiled through the runtime's driver entry point (no -lcuda).
-// dims / strides in elements of 4 bytes; strides[i] is the pitch of dim i+1.
+// dims / strides in elements; strides[i] is the pitch of dim i+1.
+int encode_tensor_map(CUtensorMap* map, CUtensorMapDataType type, int elem_bytes, const void* ptr, int rank,
+                      const unsigned long long* dims, const unsigned long long* strides_elems, const unsigned* box,
+                      CUtensorMapSwizzle swizzle);
 int encode_tensor_map_f32(CUtensorMap* map, const void* ptr, int rank, const unsigned long long* dims,
                           const unsigned long long* strides_elems, const unsigned* box, CUtensorMapSwizzle swizzle);
 // Host-mapped status word a kernel sets when one of its bounded waits expires.
@@ -20,8 +23,8 @@ int device_status_ptr(int** dptr);
 
 constexpr long long kWaitLimitCycles = 4000000000ll;  // ~2 s at 1.9 GHz
 // Failure-detection test switch, read at every launch: TTC_TEST_STALL=gemm
-// (the TF32 GEMM kernels) or =chain (the TMA-staged chain kernel) makes the
-// kernel's TMA producer issue no loads at all, so nothing is ever in flight
+// (the TF32 GEMM kernels), =linear (the 16- and 8-bit products) or =chain (the
+// TMA-staged chain kernel) makes the kernel's TMA producer issue no loads at all, so nothing is ever in flight
 // and the consumers' waits run out after kStallTestLimitCycles (~1 ms); they
 // set the status word, free what they hold and return, and the next
 // synchronisation reports TTC_ERR_TIMEOUT. Returns whether `family` stalls.
