@@ -143,6 +143,7 @@ EXPORTS = ["ttc_last_error", "ttc_init", "ttc_shutdown", "ttc_device_count", "tt
 _WITH_WORKSPACE = {RmsNormBackwardDesc: "ttc_rms_norm_backward", LinearDesc: "ttc_linear",
                    LinearBackwardDesc: "ttc_linear_backward", GatedLinearDesc: "ttc_gated_linear",
                    GatedLinearBackwardDesc: "ttc_gated_linear_backward"}
+_calls = {}  # descriptor type -> (the call, its _workspace function), filled when the library is loaded
 
 
 class TTCError(RuntimeError):
@@ -186,8 +187,10 @@ def lib():
         L.ttc_gemm_select_path.argtypes = [C.POINTER(GemmDesc)]
         L.ttc_rms_norm.argtypes = [C.POINTER(RmsNormDesc)]
         for desc, fn in _WITH_WORKSPACE.items():
-            getattr(L, fn).argtypes = [C.POINTER(desc)]
-            getattr(L, fn + "_workspace").argtypes = [C.POINTER(desc), C.POINTER(C.c_size_t)]
+            call, size = getattr(L, fn), getattr(L, fn + "_workspace")
+            call.argtypes = [C.POINTER(desc)]
+            size.argtypes = [C.POINTER(desc), C.POINTER(C.c_size_t)]
+            _calls[desc] = call, size
         L.ttc_reduce.argtypes = [C.c_void_p, C.POINTER(C.c_uint32), C.c_int, C.POINTER(C.c_int32), C.c_int,
                                  C.c_int, C.c_void_p]
         L.ttc_transpose.argtypes = [C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_int64]
@@ -405,8 +408,9 @@ def gated_linear_backward_desc(M, N, K, dy, lddy, x, ldx, wg, wu, ldw, gate, up,
 
 def workspace_size(desc) -> int:
     """Bytes of workspace that the call with this descriptor needs (0: none)."""
-    n = C.c_size_t(0)
-    check(getattr(lib(), _WITH_WORKSPACE[type(desc)] + "_workspace")(C.byref(desc), C.byref(n)))
+    lib()
+    n = C.c_size_t()
+    check(_calls[type(desc)][1](desc, n))
     return n.value
 
 
@@ -415,11 +419,12 @@ def _call(desc, workspace):
     if workspace is not None:
         desc.workspace = workspace.ptr if isinstance(workspace, DeviceArray) else workspace.data_ptr()
         desc.workspace_bytes = workspace.nbytes
-    check(getattr(lib(), _WITH_WORKSPACE[type(desc)])(C.byref(desc)))
+    lib()
+    check(_calls[type(desc)][0](desc))
 
 
 def rms_norm(desc):
-    check(lib().ttc_rms_norm(C.byref(desc)))
+    check(lib().ttc_rms_norm(desc))
 
 
 def rms_norm_backward(desc, workspace=None):

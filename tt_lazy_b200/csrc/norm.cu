@@ -1,13 +1,166 @@
 // norm.cu -- root-mean-square norm with the residual's addition
 // (ttc_rms_norm) and its gradients (ttc_rms_norm_backward).
 #include <algorithm>
+#include <cstring>
 
 #include "ffn.cuh"
+#include "tc_util.cuh"
 
 namespace ttc {
 namespace {
 
-constexpr int kThreads = 256;
+// Both kernels hold a row in registers: it is read once, its sums go over the
+// row's threads, and the results are written from the registers. The next
+// row's loads are issued before this row's reduction, so memory is busy while
+// the threads wait for their sums.
+//
+// A thread holds C chunks of 16 bytes of a row. Rows of up to 128 chunks
+// belong to one warp; longer ones to a block of up to 256 threads with two
+// chunks each, and above 512 chunks to the 2, 4 or 8 blocks of a cluster that
+// exchange their sums through distributed shared memory.
+//
+// A chunk is one 16-byte access where every tensor's rows are 16-byte aligned
+// and whole chunks long (VEC), else its elements lie 32 apart, so that a warp
+// still touches consecutive elements.
+template <class T>
+constexpr int kPer = 16 / (int)sizeof(T);  // elements of a chunk
+
+// Thread t of the row's tpr threads.
+struct Lane {
+    int t, tpr;
+};
+template <class T, bool VEC>
+__device__ __forceinline__ int column(int c, int i, Lane l) {
+    return VEC ? (c * l.tpr + l.t) * kPer<T> + i : (c * l.tpr + (l.t & ~31)) * kPer<T> + i * 32 + (l.t & 31);
+}
+
+// A chunk's elements in the four registers that they fill, whichever way they came.
+template <class T>
+__device__ __forceinline__ void unpack(const uint4& u, float (&v)[kPer<T>]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) {
+            v[i] = __uint_as_float(w[i]);
+        } else {
+            const T *lo = reinterpret_cast<const T*>(&w[i]);
+            v[2 * i] = to_f32<T>(lo[0]);
+            v[2 * i + 1] = to_f32<T>(lo[1]);
+        }
+    }
+}
+
+template <class T, bool VEC, int C>
+__device__ __forceinline__ void load_row(const T* row, int cols, Lane l, uint4 (&r)[C]) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        if constexpr (VEC) {
+            const int k = column<T, VEC>(c, 0, l);
+            r[c] = k < cols ? *reinterpret_cast<const uint4*>(row + k) : make_uint4(0, 0, 0, 0);
+        } else {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                w[i] = 0;
+#pragma unroll
+                for (int e = 0; e < kPer<T> / 4; ++e) {
+                    const int k = column<T, VEC>(c, i * (kPer<T> / 4) + e, l);
+                    if constexpr (sizeof(T) == 4) {
+                        if (k < cols) w[i] = __float_as_uint(row[k]);
+                    } else {
+                        if (k < cols) w[i] |= (uint32_t)reinterpret_cast<const uint16_t*>(row)[k] << (16 * e);
+                    }
+                }
+            }
+            r[c] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+}
+
+// T is the type whose chunks the row is divided into, Y the type stored.
+template <class T, class Y, bool VEC, int C>
+__device__ __forceinline__ void store_row(Y* row, int cols, Lane l, const float (&v)[C][kPer<T>]) {
+    struct alignas(sizeof(Y) * kPer<T>) Out {
+        Y e[kPer<T>];
+    };
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        if constexpr (VEC) {
+            Out o;
+#pragma unroll
+            for (int i = 0; i < kPer<T>; ++i) o.e[i] = from_f32<Y>(v[c][i]);
+            if (column<T, VEC>(c, 0, l) < cols)
+                *reinterpret_cast<Out*>(row + column<T, VEC>(c, 0, l)) = o;
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPer<T>; ++i) {
+                const int k = column<T, VEC>(c, i, l);
+                if (k < cols) row[k] = from_f32<Y>(v[c][i]);
+            }
+        }
+    }
+}
+
+template <class T, bool VEC, int C>
+__device__ __forceinline__ void load_weight(const void* weight, bool f32, int cols, Lane l, float (&w)[C][kPer<T>]) {
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int i = 0; i < kPer<T>; ++i) {
+            const int k = column<T, VEC>(c, i, l);
+            w[c][i] = k >= cols ? 0.0f
+                      : f32     ? static_cast<const float*>(weight)[k]
+                                : to_f32<T>(static_cast<const T*>(weight)[k]);
+        }
+}
+
+// Reduces a and b over a row's threads, in a fixed order; MAX: b is a maximum.
+// ONE: the row is one warp's. Else `slots` is one of two buffers that the rows
+// use in turn, so that one barrier a row is enough; in a cluster of more than
+// one block every warp writes its pair into the buffer of each block.
+constexpr int kSlots = 64;  // 8 blocks of 8 warps
+template <bool ONE, bool MAX>
+__device__ __forceinline__ void reduce_row(float& a, float& b, float2* slots, int blocks) {
+    auto warp = [&] {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            a += __shfl_xor_sync(0xffffffffu, a, o);
+            const float x = __shfl_xor_sync(0xffffffffu, b, o);
+            b = MAX ? fmaxf(b, x) : b + x;
+        }
+    };
+    warp();
+    if constexpr (!ONE) {
+        const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, warps = blockDim.x >> 5;
+        if (blocks == 1) {
+            if (lane == 0) slots[w] = make_float2(a, b);
+            __syncthreads();
+            a = slots[0].x;
+            b = slots[0].y;
+            for (int i = 1; i < warps; ++i) {
+                const float2 s = slots[i];
+                a += s.x;
+                b = MAX ? fmaxf(b, s.y) : b + s.y;
+            }
+        } else {
+            if (lane < blocks)
+                asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(
+                                 cluster_addr(smem_u32(slots + cluster_rank() * warps + w), lane)),
+                             "f"(a), "f"(b)
+                             : "memory");
+            __syncwarp();
+            cluster_sync();
+            const int n = warps * blocks;
+            const float2 s = lane < n ? slots[lane] : make_float2(0.0f, 0.0f);
+            const float2 s2 = lane + 32 < n ? slots[lane + 32] : make_float2(0.0f, 0.0f);
+            a = s.x + s2.x;
+            b = MAX ? fmaxf(s.y, s2.y) : s.y + s2.y;
+            warp();
+        }
+    }
+}
+
+constexpr float kMinScale = 1.17549435e-38f;  // 2^-126
 
 struct NormParams {
     long long rows;
@@ -18,62 +171,79 @@ struct NormParams {
     float* scales;
     long long ldx, ldr, ldy, ldh;
     int weight_f32;
+    int cluster;  // blocks of a row
 };
 
-// Sum and maximum over the block, in a fixed order, to every thread.
-__device__ __forceinline__ float2 block_sum_max(float s, float m) {
-    __shared__ float2 part[kThreads / 32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// Which row a thread starts at, how far it is to its next one, and its place in a row.
+struct RowPlace {
+    Lane lane;
+    long long row, step;
+};
+template <bool ONE>
+__device__ __forceinline__ RowPlace row_place(int cluster) {
+    if (ONE) {
+        const long long rows = blockDim.x / 32;
+        return {{(int)threadIdx.x % 32, 32}, blockIdx.x * rows + threadIdx.x / 32, gridDim.x * rows};
+    }
+    const int rank = cluster > 1 ? (int)cluster_rank() : 0;
+    if (cluster > 1) cluster_sync();  // every block of the row is there before one writes into another
+    return {{rank * (int)blockDim.x + (int)threadIdx.x, cluster * (int)blockDim.x},
+            (long long)(blockIdx.x / cluster), (long long)(gridDim.x / cluster)};
+}
+
+constexpr int kWarpRows = 4;  // rows of a block whose rows are one warp's
+constexpr int kMaxBlock = 256;
+
+template <class T, class Y, bool VEC, bool ONE, int C>
+__global__ void __launch_bounds__(ONE ? 32 * kWarpRows : kMaxBlock) rms_norm_kernel(const __grid_constant__ NormParams p) {
+    __shared__ float2 slots[2][kSlots];
+    const RowPlace at = row_place<ONE>(p.cluster);
+    const Lane l = at.lane;
+    float w[C][kPer<T>];
+    load_weight<T, VEC, C>(p.weight, p.weight_f32, p.cols, l, w);
+    const T *x = static_cast<const T*>(p.x), *res = static_cast<const T*>(p.residual);
+    const long long step = at.step;
+    long long r = at.row;
+    uint4 xs[C], rs[C];
+    auto fetch = [&](long long row) {
+        if (row >= p.rows) return;
+        load_row<T, VEC, C>(x + row * p.ldx, p.cols, l, xs);
+        if (res) load_row<T, VEC, C>(res + row * p.ldr, p.cols, l, rs);
+    };
+    fetch(r);
+    for (int parity = 0; r < p.rows; r += step, parity ^= 1) {
+        float h[C][kPer<T>], sum = 0.0f, top = 0.0f;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        s += __shfl_xor_sync(0xffffffffu, s, o);
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    }
-    if (lane == 0) part[warp] = make_float2(s, m);
-    __syncthreads();
-    float2 t = part[0];
-    for (int w = 1; w < kThreads / 32; ++w) {
-        t.x += part[w].x;
-        t.y = fmaxf(t.y, part[w].y);
-    }
-    return t;
-}
-
-constexpr float kMinScale = 1.17549435e-38f;  // 2^-126
-
-template <class T>
-__device__ __forceinline__ float weight_at(const NormParams& p, int c) {
-    return p.weight_f32 ? static_cast<const float*>(p.weight)[c] : to_f32<T>(static_cast<const T*>(p.weight)[c]);
-}
-
-// One block per row, two passes over it.
-template <class T, class Y>
-__global__ void __launch_bounds__(kThreads) rms_norm_kernel(const __grid_constant__ NormParams p) {
-    const long long r = blockIdx.x;
-    const T* x = static_cast<const T*>(p.x) + r * p.ldx;
-    const T* res = p.residual ? static_cast<const T*>(p.residual) + r * p.ldr : nullptr;
-    float sum = 0.0f, top = 0.0f;
-    for (int c = threadIdx.x; c < p.cols; c += kThreads) {
-        float h = to_f32<T>(x[c]);
-        if (res) h += to_f32<T>(res[c]);
-        sum += h * h;
-        top = fmaxf(top, fabsf(h * weight_at<T>(p, c)));
-    }
-    const float2 t = block_sum_max(sum, top);
-    const float rstd = rsqrtf(t.x / (float)p.cols + p.eps);
-    float inv = 1.0f;
-    if (sizeof(Y) == 1) {
-        const float scale = fmaxf(t.y * rstd * (1.0f / 448.0f), kMinScale);
-        inv = 1.0f / scale;
-        if (threadIdx.x == 0) p.scales[r] = scale;
-    }
-    Y* y = static_cast<Y*>(p.y) + r * p.ldy;
-    T* hid = p.hidden ? static_cast<T*>(p.hidden) + r * p.ldh : nullptr;
-    for (int c = threadIdx.x; c < p.cols; c += kThreads) {
-        float h = to_f32<T>(x[c]);
-        if (res) h += to_f32<T>(res[c]);
-        if (hid) hid[c] = from_f32<T>(h);
-        y[c] = from_f32<Y>(h * rstd * weight_at<T>(p, c) * inv);
+        for (int c = 0; c < C; ++c) {
+            unpack<T>(xs[c], h[c]);
+            if (res) {
+                float v[kPer<T>];
+                unpack<T>(rs[c], v);
+#pragma unroll
+                for (int i = 0; i < kPer<T>; ++i) h[c][i] += v[i];
+            }
+#pragma unroll
+            for (int i = 0; i < kPer<T>; ++i) {
+                sum += h[c][i] * h[c][i];
+                if (sizeof(Y) == 1) top = fmaxf(top, fabsf(h[c][i] * w[c][i]));
+            }
+        }
+        fetch(r + step);
+        reduce_row<ONE, true>(sum, top, slots[parity], p.cluster);
+        // All of the row is in registers now: x, residual, hidden and y may be the same memory.
+        if (p.hidden) store_row<T, T, VEC, C>(static_cast<T*>(p.hidden) + r * p.ldh, p.cols, l, h);
+        float k = rsqrtf(sum / (float)p.cols + p.eps);
+        float inv = 1.0f;
+        if (sizeof(Y) == 1) {
+            const float scale = fmaxf(top * k * (1.0f / 448.0f), kMinScale);
+            inv = 1.0f / scale;
+            if (l.t == 0) p.scales[r] = scale;
+        }
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < kPer<T>; ++i) h[c][i] = h[c][i] * k * w[c][i] * inv;
+        store_row<T, Y, VEC, C>(static_cast<Y*>(p.y) + r * p.ldy, p.cols, l, h);
     }
 }
 
@@ -83,47 +253,170 @@ struct NormBackwardParams {
     float eps;
     const void *dy, *hidden, *weight, *dhidden;
     void* dx;
-    float* partials;  // [gridDim.x, cols] sums of dy * hidden * rstd, or NULL
+    float* partials;  // [blocks or clusters, cols] sums of dy * hidden * rstd, or NULL
     long long lddy, ldh, lddh, lddx;
     int weight_f32;
+    int cluster;
 };
 
-// Block b takes rows b, b + gridDim.x, ...; a thread owns the same columns of
-// every row, so its running weight gradients sit in the block's own row of
-// the partials without atomics.
-template <class T>
-__global__ void __launch_bounds__(kThreads) rms_norm_backward_kernel(const __grid_constant__ NormBackwardParams p) {
-    float* part = p.partials ? p.partials + (long long)blockIdx.x * p.cols : nullptr;
-    if (part)
-        for (int c = threadIdx.x; c < p.cols; c += kThreads) part[c] = 0.0f;
+// The weight's gradient stays in registers over all of a block's rows and goes
+// out once as the block's row of the partials; no atomics.
+// Registers for 512 threads an SM (one row a warp: 512, 256 with four chunks).
+template <class T, bool VEC, bool ONE, int C>
+__global__ void __launch_bounds__(ONE ? 32 * kWarpRows : kMaxBlock, ONE ? (C == 4 ? 2 : 4) : 2)
+    rms_norm_backward_kernel(const __grid_constant__ NormBackwardParams p) {
+    __shared__ float2 slots[2][kSlots];
+    const RowPlace at = row_place<ONE>(p.cluster);
+    const Lane l = at.lane;
+    float w[C][kPer<T>], dw[C][kPer<T>] = {};
+    load_weight<T, VEC, C>(p.weight, p.weight_f32, p.cols, l, w);
+    const T *dy = static_cast<const T*>(p.dy), *hid = static_cast<const T*>(p.hidden);
+    const T* dh = static_cast<const T*>(p.dhidden);
+    const long long step = at.step;
+    long long r = at.row;
+    uint4 gs[C], hs[C], ds[C];
+    auto fetch = [&](long long row) {
+        if (row >= p.rows) return;
+        load_row<T, VEC, C>(dy + row * p.lddy, p.cols, l, gs);
+        load_row<T, VEC, C>(hid + row * p.ldh, p.cols, l, hs);
+        if (dh) load_row<T, VEC, C>(dh + row * p.lddh, p.cols, l, ds);
+    };
+    fetch(r);
+    for (int parity = 0; r < p.rows; r += step, parity ^= 1) {
+        float sum = 0.0f, dot = 0.0f;
+        uint4 g[C], h[C], d[C];
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            g[c] = gs[c];
+            h[c] = hs[c];
+            if (dh) d[c] = ds[c];
+            float hv[kPer<T>], gv[kPer<T>];
+            unpack<T>(h[c], hv);
+            unpack<T>(g[c], gv);
+#pragma unroll
+            for (int i = 0; i < kPer<T>; ++i) {
+                sum += hv[i] * hv[i];
+                dot += gv[i] * w[c][i] * hv[i];
+            }
+        }
+        fetch(r + step);
+        reduce_row<ONE, false>(sum, dot, slots[parity], p.cluster);
+        const float rstd = rsqrtf(sum / (float)p.cols + p.eps);
+        const float k = dot * rstd * rstd / (float)p.cols;
+        float out[C][kPer<T>];
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            float hv[kPer<T>], gv[kPer<T>];
+            unpack<T>(h[c], hv);
+            unpack<T>(g[c], gv);
+#pragma unroll
+            for (int i = 0; i < kPer<T>; ++i) {
+                out[c][i] = rstd * (gv[i] * w[c][i] - hv[i] * k);
+                dw[c][i] += gv[i] * hv[i] * rstd;
+            }
+            if (dh) {
+                unpack<T>(d[c], gv);
+#pragma unroll
+                for (int i = 0; i < kPer<T>; ++i) out[c][i] += gv[i];
+            }
+        }
+        store_row<T, T, VEC, C>(static_cast<T*>(p.dx) + r * p.lddx, p.cols, l, out);
+    }
+    if (!p.partials) return;
+    float* part = p.partials + (long long)(blockIdx.x / p.cluster) * p.cols;
+    if constexpr (!ONE) {
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < kPer<T>; ++i) {
+                const int col = column<T, VEC>(c, i, l);
+                if (col < p.cols) part[col] = dw[c][i];
+            }
+    } else {  // the block's warps side by side, added in order
+        __shared__ float rows[kWarpRows][32 * C * kPer<T>];
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < kPer<T>; ++i) rows[threadIdx.x / 32][column<T, VEC>(c, i, l)] = dw[c][i];
+        __syncthreads();
+        for (int col = threadIdx.x; col < p.cols; col += 32 * kWarpRows) {
+            float s = rows[0][col];
+#pragma unroll
+            for (int k = 1; k < kWarpRows; ++k) s += rows[k][col];
+            part[col] = s;
+        }
+    }
+}
+
+// Rows that do not fit in registers: one block a row, two passes over it (the
+// second finds it in L2).
+constexpr int kWide = 1024;
+
+template <class T, class Y>
+__global__ void __launch_bounds__(kWide) rms_norm_wide_kernel(const __grid_constant__ NormParams p) {
+    __shared__ float2 slots[2][kSlots];
     auto weight = [&](int c) {
         return p.weight_f32 ? static_cast<const float*>(p.weight)[c] : to_f32<T>(static_cast<const T*>(p.weight)[c]);
     };
-    for (long long r = blockIdx.x; r < p.rows; r += gridDim.x) {
+    int parity = 0;
+    for (long long r = blockIdx.x; r < p.rows; r += gridDim.x, parity ^= 1) {
+        const T* x = static_cast<const T*>(p.x) + r * p.ldx;
+        const T* res = p.residual ? static_cast<const T*>(p.residual) + r * p.ldr : nullptr;
+        float sum = 0.0f, top = 0.0f;
+#pragma unroll 4
+        for (int c = threadIdx.x; c < p.cols; c += kWide) {
+            float h = to_f32<T>(x[c]);
+            if (res) h += to_f32<T>(res[c]);
+            sum += h * h;
+            if (sizeof(Y) == 1) top = fmaxf(top, fabsf(h * weight(c)));
+        }
+        reduce_row<false, true>(sum, top, slots[parity], 1);
+        const float k = rsqrtf(sum / (float)p.cols + p.eps);
+        float inv = 1.0f;
+        if (sizeof(Y) == 1) {
+            const float scale = fmaxf(top * k * (1.0f / 448.0f), kMinScale);
+            inv = 1.0f / scale;
+            if (threadIdx.x == 0) p.scales[r] = scale;
+        }
+        Y* y = static_cast<Y*>(p.y) + r * p.ldy;
+        T* hid = p.hidden ? static_cast<T*>(p.hidden) + r * p.ldh : nullptr;
+#pragma unroll 4
+        for (int c = threadIdx.x; c < p.cols; c += kWide) {  // an element is read before it may be written over
+            float h = to_f32<T>(x[c]);
+            if (res) h += to_f32<T>(res[c]);
+            if (hid) hid[c] = from_f32<T>(h);
+            y[c] = from_f32<Y>(h * k * weight(c) * inv);
+        }
+    }
+}
+
+template <class T>
+__global__ void __launch_bounds__(kWide) rms_norm_backward_wide_kernel(const __grid_constant__ NormBackwardParams p) {
+    __shared__ float2 slots[2][kSlots];
+    float* part = p.partials ? p.partials + (long long)blockIdx.x * p.cols : nullptr;
+    if (part)
+        for (int c = threadIdx.x; c < p.cols; c += kWide) part[c] = 0.0f;  // a thread owns its columns throughout
+    auto weight = [&](int c) {
+        return p.weight_f32 ? static_cast<const float*>(p.weight)[c] : to_f32<T>(static_cast<const T*>(p.weight)[c]);
+    };
+    int parity = 0;
+    for (long long r = blockIdx.x; r < p.rows; r += gridDim.x, parity ^= 1) {
         const T* dy = static_cast<const T*>(p.dy) + r * p.lddy;
         const T* hid = static_cast<const T*>(p.hidden) + r * p.ldh;
         const T* dh = p.dhidden ? static_cast<const T*>(p.dhidden) + r * p.lddh : nullptr;
         T* dx = static_cast<T*>(p.dx) + r * p.lddx;
         float sum = 0.0f, dot = 0.0f;
-        for (int c = threadIdx.x; c < p.cols; c += kThreads) {
+#pragma unroll 4
+        for (int c = threadIdx.x; c < p.cols; c += kWide) {
             const float h = to_f32<T>(hid[c]);
             sum += h * h;
             dot += to_f32<T>(dy[c]) * weight(c) * h;
         }
-        __shared__ float2 red[kThreads / 32];
-        sum = warp_sum(sum);
-        dot = warp_sum(dot);
-        __syncthreads();
-        if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = make_float2(sum, dot);
-        __syncthreads();
-        sum = dot = 0.0f;
-        for (int w = 0; w < kThreads / 32; ++w) {
-            sum += red[w].x;
-            dot += red[w].y;
-        }
+        reduce_row<false, false>(sum, dot, slots[parity], 1);
         const float rstd = rsqrtf(sum / (float)p.cols + p.eps);
         const float k = dot * rstd * rstd / (float)p.cols;
-        for (int c = threadIdx.x; c < p.cols; c += kThreads) {
+#pragma unroll 4
+        for (int c = threadIdx.x; c < p.cols; c += kWide) {
             const float h = to_f32<T>(hid[c]), g = to_f32<T>(dy[c]);
             float d = rstd * (g * weight(c) - h * k);
             if (dh) d += to_f32<T>(dh[c]);
@@ -133,13 +426,23 @@ __global__ void __launch_bounds__(kThreads) rms_norm_backward_kernel(const __gri
     }
 }
 
-// out[c] = sum over b < n of partials[b][c], in order.
-__global__ void __launch_bounds__(kThreads) sum_partials_kernel(const float* partials, int n, int cols, void* out,
-                                                                int dtype) {
-    const int c = blockIdx.x * kThreads + threadIdx.x;
-    if (c >= cols) return;
+// out[c] = sum over b < n of partials[b][c]: 32 columns a block, 32 threads a
+// column that each add every 32nd partial, then the 32 in order.
+__global__ void __launch_bounds__(1024) sum_partials_kernel(const float* partials, int n, int cols, void* out,
+                                                            int dtype) {
+    __shared__ float part[32][33];
+    const int lane = threadIdx.x & 31, g = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
     float s = 0.0f;
-    for (int b = 0; b < n; ++b) s += partials[(long long)b * cols + c];
+    if (c < cols) {
+#pragma unroll 8
+        for (int b = g; b < n; b += 32) s += partials[(long long)b * cols + c];
+    }
+    part[g][lane] = s;
+    __syncthreads();
+    if (g != 0 || c >= cols) return;
+    s = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 32; ++k) s += part[k][lane];
     if (dtype == TTC_BF16)
         static_cast<__nv_bfloat16*>(out)[c] = from_f32<__nv_bfloat16>(s);
     else if (dtype == TTC_F16)
@@ -192,20 +495,121 @@ int check_norm_backward(const ttc_rms_norm_backward_desc& d) {
     return check_tensor(op, "dweight", d.dweight, d.weight_dtype, d.cols, d.cols, false);
 }
 
-// Blocks of the backward kernel. Fixed by the shape alone, so that the
-// workspace size needs no device and results are the same on every call.
-int backward_blocks(long long rows) { return (int)std::min<long long>(rows, 148 * 4); }
+// How a row is divided: threads of a block, blocks of a cluster and chunks a
+// thread; one: a warp has the row; block 0: the row does not fit.
+struct RowShape {
+    int block, cluster, chunks, one;
+};
+RowShape row_shape(int cols, int dtype) {
+    const long long n = ((long long)cols * dtype_size(dtype) + 15) / 16;
+    if (n <= 128) return {32 * kWarpRows, 1, n <= 32 ? 1 : n <= 64 ? 2 : 4, 1};
+    for (int cluster = 1; cluster <= 8; cluster *= 2)
+        if (n <= 2ll * kMaxBlock * cluster) return {(int)((n + 64 * cluster - 1) / (64 * cluster)) * 32, cluster, 2, 0};
+    return {0, 1, 0, 0};
+}
+
+// Clusters (of one block mostly) of the backward kernel at most: what 148 SMs
+// hold at 512 threads each, from the shape alone, so that the workspace size
+// needs no device.
+int backward_clusters(long long rows, const RowShape& s) {
+    if (s.block == 0) return (int)std::min<long long>(rows, 148 * 2);
+    if (s.one) return (int)std::min<long long>((rows + kWarpRows - 1) / kWarpRows, 148 * (s.chunks == 4 ? 2 : 4));
+    return (int)std::min<long long>(rows, std::max(1, 148 * 512 / (s.block * s.cluster)));
+}
 
 size_t backward_bytes(const ttc_rms_norm_backward_desc& d) {
-    return d.dweight ? align256((size_t)backward_blocks(d.rows) * d.cols * sizeof(float)) : 0;
+    const int n = backward_clusters(d.rows, row_shape(d.cols, d.dtype));
+    return d.dweight ? align256((size_t)n * d.cols * sizeof(float)) : 0;
+}
+
+// Launches `clusters` clusters, or as many as the GPU holds at once: a few more
+// than that would take a second round as long as the first.
+template <class Params>
+int launch_rows(void (*kernel)(const Params), const Params& p, const RowShape& s, long long clusters,
+                int* launched = nullptr) {
+    struct Seen {
+        const void* kernel;
+        int device, block, cluster, most;
+    };
+    static Seen seen[64] = {};  // one launch shape an entry; a full table starts over
+    static int used = 0;
+    cudaLaunchConfig_t cfg;
+    std::memset(&cfg, 0, sizeof cfg);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)s.cluster;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)(clusters * s.cluster), 1, 1);
+    cfg.blockDim = dim3((unsigned)s.block, 1, 1);
+    cfg.stream = rt().stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = s.cluster > 1 ? 1 : 0;
+    int most = 0;
+    for (int i = 0; i < used && !most; ++i)
+        if (seen[i].kernel == (const void*)kernel && seen[i].device == rt().device && seen[i].block == s.block &&
+            seen[i].cluster == s.cluster)
+            most = seen[i].most;
+    if (!most) {
+        if (s.cluster > 1) {
+            TTC_CUDA(cudaOccupancyMaxActiveClusters(&most, kernel, &cfg));
+        } else {
+            TTC_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&most, kernel, s.block, 0));
+            most *= rt().sm_count;
+        }
+        if (most < 1) return set_error(TTC_ERR_CUDA, "tt_cuda: rms_norm: a block of %d threads does not fit", s.block);
+        if (used == 64) used = 0;
+        seen[used++] = {(const void*)kernel, rt().device, s.block, s.cluster, most};
+    }
+    clusters = std::min<long long>(clusters, most);
+    if (launched) *launched = (int)clusters;
+    cfg.gridDim.x = (unsigned)(clusters * s.cluster);
+    TTC_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
+    return TTC_OK;
+}
+
+template <class T, class Y, bool VEC>
+int launch_norm(const NormParams& p, const RowShape& s) {
+    if (s.block == 0) {
+        const long long n = std::min<long long>(p.rows, 2ll * rt().sm_count);
+        rms_norm_wide_kernel<T, Y><<<(unsigned)n, kWide, 0, rt().stream>>>(p);
+        return TTC_OK;
+    }
+    if (s.one) {
+        const long long n = (p.rows + kWarpRows - 1) / kWarpRows;
+        return launch_rows(s.chunks == 1   ? rms_norm_kernel<T, Y, VEC, true, 1>
+                           : s.chunks == 2 ? rms_norm_kernel<T, Y, VEC, true, 2>
+                                           : rms_norm_kernel<T, Y, VEC, true, 4>,
+                           p, s, n);
+    }
+    // 768 threads an SM rather than the 1024 that fit: 88 us against 97 for 16384 rows of 4096 in bf16
+    const long long n = s.cluster > 1 ? p.rows : std::min<long long>(p.rows, 768ll * rt().sm_count / s.block);
+    return launch_rows(rms_norm_kernel<T, Y, VEC, false, 2>, p, s, n);
 }
 
 template <class T>
-void launch_norm(const NormParams& p, int y_dtype, cudaStream_t st) {
+int launch_norm_type(const NormParams& p, int y_dtype, const RowShape& s, bool vec) {
     if (y_dtype == TTC_E4M3)
-        rms_norm_kernel<T, __nv_fp8_e4m3><<<(unsigned)p.rows, kThreads, 0, st>>>(p);
-    else
-        rms_norm_kernel<T, T><<<(unsigned)p.rows, kThreads, 0, st>>>(p);
+        return vec ? launch_norm<T, __nv_fp8_e4m3, true>(p, s) : launch_norm<T, __nv_fp8_e4m3, false>(p, s);
+    return vec ? launch_norm<T, T, true>(p, s) : launch_norm<T, T, false>(p, s);
+}
+
+template <class T, bool VEC>
+int launch_norm_backward(const NormBackwardParams& p, const RowShape& s, int& clusters) {
+    if (s.block == 0) {
+        rms_norm_backward_wide_kernel<T><<<clusters, kWide, 0, rt().stream>>>(p);
+        return TTC_OK;
+    }
+    return launch_rows(!s.one          ? rms_norm_backward_kernel<T, VEC, false, 2>
+                       : s.chunks == 1 ? rms_norm_backward_kernel<T, VEC, true, 1>
+                       : s.chunks == 2 ? rms_norm_backward_kernel<T, VEC, true, 2>
+                                       : rms_norm_backward_kernel<T, VEC, true, 4>,
+                       p, s, clusters, &clusters);
+}
+
+// Rows of `p` start on boundaries of a whole chunk's elements.
+bool rows_aligned(const void* p, int elem_bytes, int per_chunk, long long ld) {
+    return !p || ((uintptr_t)p % (elem_bytes * per_chunk) == 0 && ld % per_chunk == 0);
 }
 
 }  // namespace
@@ -221,7 +625,7 @@ int check_workspace(const char* op, const void* ws, size_t have, size_t need) {
 }
 
 int launch_sum_partials(const float* partials, int n, int cols, void* out, int dtype, cudaStream_t st) {
-    sum_partials_kernel<<<(cols + kThreads - 1) / kThreads, kThreads, 0, st>>>(partials, n, cols, out, dtype);
+    sum_partials_kernel<<<(cols + 31) / 32, 1024, 0, st>>>(partials, n, cols, out, dtype);
     count_launch();
     return check_cuda(cudaGetLastError(), "partial sums launch");
 }
@@ -239,14 +643,16 @@ int ttc_rms_norm(const ttc_rms_norm_desc* desc) {
     TTC_REQUIRE_INIT();
     if (d.rows == 0) return TTC_OK;
     DeviceGuard guard;
-    NormParams p{d.rows, d.cols,   d.eps, d.x,   d.residual, d.weight, d.y, d.hidden,
-                 d.scales, d.ldx, d.ldr, d.ldy, d.ldh,      d.weight_dtype == TTC_F32};
-    if (d.dtype == TTC_BF16)
-        launch_norm<__nv_bfloat16>(p, d.y_dtype, rt().stream);
-    else if (d.dtype == TTC_F16)
-        launch_norm<__half>(p, d.y_dtype, rt().stream);
-    else
-        launch_norm<float>(p, d.y_dtype, rt().stream);
+    const RowShape s = row_shape(d.cols, d.dtype);
+    const NormParams p{d.rows,   d.cols, d.eps, d.x,   d.residual, d.weight,                  d.y,      d.hidden,
+                       d.scales, d.ldx,  d.ldr, d.ldy, d.ldh,      d.weight_dtype == TTC_F32, s.cluster};
+    const int es = dtype_size(d.dtype), per = 16 / es;
+    const bool vec = d.cols % per == 0 && rows_aligned(d.x, es, per, d.ldx) && rows_aligned(d.residual, es, per, d.ldr) &&
+                     rows_aligned(d.y, dtype_size(d.y_dtype), per, d.ldy) && rows_aligned(d.hidden, es, per, d.ldh);
+    if (int rc = d.dtype == TTC_BF16  ? launch_norm_type<__nv_bfloat16>(p, d.y_dtype, s, vec)
+                 : d.dtype == TTC_F16 ? launch_norm_type<__half>(p, d.y_dtype, s, vec)
+                                      : launch_norm_type<float>(p, d.y_dtype, s, vec))
+        return rc;
     count_launch();
     return check_cuda(cudaGetLastError(), "rms_norm launch");
 }
@@ -272,19 +678,25 @@ int ttc_rms_norm_backward(const ttc_rms_norm_backward_desc* desc) {
         if (d.dweight) TTC_CUDA(cudaMemsetAsync(d.dweight, 0, (size_t)d.cols * dtype_size(d.weight_dtype), st));
         return TTC_OK;
     }
-    const int blocks = backward_blocks(d.rows);
-    NormBackwardParams p{d.rows, d.cols, d.eps,  d.dy,  d.hidden, d.weight, d.dhidden, d.dx,
-                         d.dweight ? (float*)d.workspace : nullptr,
-                         d.lddy, d.ldh,  d.lddh, d.lddx, d.weight_dtype == TTC_F32};
-    if (d.dtype == TTC_BF16)
-        rms_norm_backward_kernel<__nv_bfloat16><<<blocks, kThreads, 0, st>>>(p);
-    else if (d.dtype == TTC_F16)
-        rms_norm_backward_kernel<__half><<<blocks, kThreads, 0, st>>>(p);
-    else
-        rms_norm_backward_kernel<float><<<blocks, kThreads, 0, st>>>(p);
+    const RowShape s = row_shape(d.cols, d.dtype);
+    int clusters = backward_clusters(d.rows, s);
+    const NormBackwardParams p{d.rows, d.cols, d.eps, d.dy, d.hidden, d.weight, d.dhidden, d.dx,
+                               d.dweight ? (float*)d.workspace : nullptr,
+                               d.lddy, d.ldh, d.lddh, d.lddx, d.weight_dtype == TTC_F32, s.cluster};
+    const int es = dtype_size(d.dtype), per = 16 / es;
+    const bool vec = d.cols % per == 0 && rows_aligned(d.dy, es, per, d.lddy) && rows_aligned(d.hidden, es, per, d.ldh) &&
+                     rows_aligned(d.dhidden, es, per, d.lddh) && rows_aligned(d.dx, es, per, d.lddx);
+    auto launch = [&](auto type) {
+        using T = decltype(type);
+        return vec ? launch_norm_backward<T, true>(p, s, clusters) : launch_norm_backward<T, false>(p, s, clusters);
+    };
+    if (int rc = d.dtype == TTC_BF16  ? launch(__nv_bfloat16())
+                 : d.dtype == TTC_F16 ? launch(__half())
+                                      : launch(0.0f))
+        return rc;
     count_launch();
     if (int rc = check_cuda(cudaGetLastError(), "rms_norm_backward launch")) return rc;
-    return d.dweight ? launch_sum_partials(p.partials, blocks, d.cols, d.dweight, d.weight_dtype, st) : TTC_OK;
+    return d.dweight ? launch_sum_partials(p.partials, clusters, d.cols, d.dweight, d.weight_dtype, st) : TTC_OK;
 }
 
 }  // extern "C"
