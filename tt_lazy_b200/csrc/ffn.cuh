@@ -106,7 +106,26 @@ struct Product {
 int run_product(const Product& p, void* scratch);
 size_t product_scratch(const Product& p);
 
+// Launch attributes of these operators' kernels: a cluster where there is one,
+// and leave to be launched while the kernel before it in the stream still runs
+// (each kernel calls grid_wait() before it touches memory). Returns their number.
+inline int launch_attributes(cudaLaunchAttribute (&attr)[2], int cluster) {
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    if (cluster == 1) return 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    return 2;
+}
+
 #ifdef __CUDACC__
+
+// Waits until the kernels before this one in the stream have finished and their
+// writes are visible; lets the kernel after this one start to be launched.
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 template <class T>
 __device__ __forceinline__ float to_f32(T v);

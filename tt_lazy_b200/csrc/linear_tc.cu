@@ -35,7 +35,8 @@
 namespace ttc {
 namespace {
 
-constexpr int kThreads = 192;  // warp 0: TMA, warp 1: MMA, warps 2-5: epilogue
+constexpr int kThreads = 192;      // warp 0: TMA, warp 1: MMA, warps 2-5: epilogue
+constexpr int kTileThreads = 320;  // tile kernel: warps 2-9 empty the accumulator, all of them finish the outputs
 constexpr int kRow = 128;      // bytes of K a stage holds of each row
 constexpr int kBox = 64 * kRow;  // an MN-major box: 64 k-rows of 64 16-bit columns
 
@@ -164,6 +165,8 @@ __global__ void __launch_bounds__(kThreads, 1) pair_kernel(const __grid_constant
     cluster_sync();  // both CTAs' barriers are initialised before anyone signals across
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
+    grid_wait();
+    grid_trigger();
     const int num_tiles = q.m_tiles * q.n_tiles;
     const int cluster_id = blockIdx.x >> 1, nclusters = gridDim.x >> 1;
     bool failed = false;
@@ -354,7 +357,7 @@ __device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
 }
 
 template <bool F8>
-__global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ ProductParams q) {
+__global__ void __launch_bounds__(kTileThreads) tile_kernel(const __grid_constant__ ProductParams q) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     const int stage_bytes = kHalf + q.tok * kRow, stages = q.stages;
@@ -371,8 +374,25 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ 
     const int m0 = tile % q.m_tiles * q.tok, n0 = tile / q.m_tiles * (p.gated ? 64 : 128);
     const int kb0 = (int)((long long)q.kb_total * split / splits);
     const int kb1 = (int)((long long)q.kb_total * (split + 1) / splits);
-    const uint32_t tmem_cols = q.tok < 32 ? 32 : q.tok;
+    const uint32_t tmem_cols = q.tok <= 32 ? 32 : q.tok <= 64 ? 64 : q.tok <= 128 ? 128 : 256;
+    bool failed = false;
 
+    // The first loads go out before the block has met: the barriers they need
+    // are this thread's own.
+    constexpr int bk = F8 ? 128 : 64;
+    auto load = [&](int kb, int stage) {
+        const int seg = kb >= q.kb_seg, k = kb - (seg ? q.kb_seg : 0);
+        const uint32_t dst = sbase + stage * stage_bytes, bar = full_bar(stage);
+        mbar_arrive_expect_tx(bar, stage_bytes);
+        if (p.gated) {
+            load_rows(dst, &q.b[0], bar, p.b_mn, k, bk, n0, 64);
+            load_rows(dst + kHalf / 2, &q.b[1], bar, p.b_mn, k, bk, n0, 64);
+        } else {
+            load_rows(dst, &q.b[seg], bar, p.b_mn, k, bk, n0, 128);
+        }
+        load_rows(dst + kHalf, &q.a[seg], bar, p.a_mn, k, bk, m0, q.tok);
+    };
+    int issued = 0;
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; ++s) {
             mbar_init(full_bar(s), 1);
@@ -380,6 +400,9 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ 
         }
         mbar_init(done_bar, 1);
         mbar_fence_init();
+        grid_wait();
+        if (!q.stall)
+            for (; issued < stages && kb0 + issued < kb1; ++issued) load(kb0 + issued, issued);
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
@@ -391,29 +414,18 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ 
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    bool failed = false;
+    grid_trigger();
 
     if (warp == 0) {
         if (lane == 0 && !q.stall) {
-            constexpr int bk = F8 ? 128 : 64;
-            int stage = 0;
+            int stage = 0;  // the ring is full, or everything is on its way
             uint32_t phase = 0;
-            int issued = 0;
-            for (int kb = kb0; kb < kb1; ++kb) {
-                if (!mbar_wait(empty_bar(stage), phase ^ 1, q.wait_limit)) {
+            for (int kb = kb0 + issued; kb < kb1; ++kb) {
+                if (!mbar_wait(empty_bar(stage), phase, q.wait_limit)) {
                     failed = true;
                     break;
                 }
-                const int seg = kb >= q.kb_seg, k = kb - (seg ? q.kb_seg : 0);
-                const uint32_t dst = sbase + stage * stage_bytes, bar = full_bar(stage);
-                mbar_arrive_expect_tx(bar, stage_bytes);
-                if (p.gated) {
-                    load_rows(dst, &q.b[0], bar, p.b_mn, k, bk, n0, 64);
-                    load_rows(dst + kHalf / 2, &q.b[1], bar, p.b_mn, k, bk, n0, 64);
-                } else {
-                    load_rows(dst, &q.b[seg], bar, p.b_mn, k, bk, n0, 128);
-                }
-                load_rows(dst + kHalf, &q.a[seg], bar, p.a_mn, k, bk, m0, q.tok);
+                load(kb, stage);
                 ++issued;
                 if (++stage == stages) {
                     stage = 0;
@@ -457,7 +469,7 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ 
         if (__all_sync(0xffffffffu, mbar_wait(done_bar, 0, q.wait_limit))) {
             // every load has landed and every instruction has read its stage: the ring is free
             tc_fence_after();
-            for (int c = 0; c < rows; c += 16) {
+            for (int c = (warp - 2) / 4 * 16; c < rows; c += 32) {
                 uint32_t r[16];
                 tc_ld_32x32b_x16(tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)c, r);
                 tc_wait_ld();
@@ -468,6 +480,7 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ 
             failed = true;
         }
     }
+    grid_wait();
     if (failed) *(volatile int*)q.status = 1;
     tc_fence_before();
     __syncthreads();
@@ -498,7 +511,7 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ 
             v[0] += lo.x, v[1] += lo.y, v[2] += lo.z, v[3] += lo.w, v[4] += hi.x, v[5] += hi.y, v[6] += hi.z, v[7] += hi.w;
         }
     };
-    for (int it = split * share + threadIdx.x; it < last; it += kThreads) {
+    for (int it = split * share + threadIdx.x; it < last; it += kTileThreads) {
         const int row = it / groups, j = it % groups, col = n0 + j * 8;
         if (col >= p.N) continue;
         float v[8], u[8];
@@ -578,16 +591,12 @@ int launch_pair(ProductParams& q) {
     static int most[kMaxDevices] = {};
     cudaLaunchConfig_t cfg;
     std::memset(&cfg, 0, sizeof cfg);
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
+    cfg.attrs = attr;
+    cfg.numAttrs = launch_attributes(attr, 2);
     cfg.blockDim = dim3(kThreads, 1, 1);
     cfg.dynamicSmemBytes = kPairSmem;
     cfg.stream = rt().stream;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
     int& clusters = most[rt().device];
     if (first_on_device(seen)) {
         TTC_CUDA(cudaFuncSetAttribute(pair_kernel<F8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
@@ -612,16 +621,12 @@ int launch_tile(ProductParams& q) {
         TTC_CUDA(cudaFuncSetAttribute(tile_kernel<F8>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448));
     cudaLaunchConfig_t cfg;
     std::memset(&cfg, 0, sizeof cfg);
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)q.splits;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.blockDim = dim3(kThreads, 1, 1);
+    cudaLaunchAttribute attr[2];
+    cfg.attrs = attr;
+    cfg.numAttrs = launch_attributes(attr, q.splits);
+    cfg.blockDim = dim3(kTileThreads, 1, 1);
     cfg.dynamicSmemBytes = (size_t)ring + 1024 + 256;
     cfg.stream = rt().stream;
-    cfg.attrs = attr;
-    cfg.numAttrs = q.splits > 1 ? 1 : 0;
     cfg.gridDim = dim3((unsigned)((long long)q.m_tiles * q.n_tiles * q.splits), 1, 1);
     TTC_CUDA(cudaLaunchKernelEx(&cfg, tile_kernel<F8>, q));
     count_launch();
@@ -686,16 +691,29 @@ int run_product(const Product& given, void* scratch) {
         return f8 ? launch_pair<true>(q) : launch_pair<false>(q);
     }
 
-    q.tok = p.a_mn ? 64 : 16;
-    while (q.tok < p.M && q.tok < 256) q.tok *= 2;
-    q.n_tiles = (p.N + (p.gated ? 63 : 127)) / (p.gated ? 64 : 128);
+    // Rows a tile: all of x up to 256; fewer where even eight CTAs a tile would
+    // leave SMs idle (256 x 1024 x 512: 18.3 us with 8 tiles of 256 rows, 6.2
+    // with 64 tiles of 32). CTAs a tile: until the SMs have one each, and two
+    // each for few rows, whose CTAs spend their time waiting for the weight
+    // (1 x 4096 x 16384: 24.2 us with 256 CTAs, 28.0 with 128; 64 x 4096 x
+    // 4096: 13.1 us with 128, 15.8 with 256), while every share has at least
+    // four k-blocks (two for a few rows, where joining the shares is quick).
+    const int unit = p.a_mn ? 64 : 16, width = p.gated ? 64 : 128;
+    const int least = p.M <= 16 ? 2 : 4;
+    q.n_tiles = (p.N + width - 1) / width;
+    int most_splits = 1;
+    while (most_splits < 8 && q.kb_total >= 2 * most_splits * least) most_splits *= 2;
+    q.tok = std::min(256, (p.M + unit - 1) / unit * unit);
+    auto tiles = [&] { return ((long long)p.M + q.tok - 1) / q.tok * q.n_tiles; };
+    while (q.tok > std::max(32, unit) && tiles() * most_splits < sms) q.tok = (q.tok / 2 + unit - 1) / unit * unit;
     q.m_tiles = (p.M + q.tok - 1) / q.tok;
-    const long long tiles = (long long)q.m_tiles * q.n_tiles;
     q.splits = 1;
-    while (q.splits < 8 && tiles * q.splits * 2 <= 2 * sms && q.kb_total >= 4 * q.splits) q.splits *= 2;
-    // two CTAs an SM up to 64 rows, one above
+    while (q.splits < most_splits && tiles() * q.splits * 2 <= (q.tok <= 32 ? 2 * sms : sms)) q.splits *= 2;
+    // The ring: half an SM's shared memory where that holds three stages, so
+    // that one CTA's loads run under the other's start and end (4 x 16384 x
+    // 4096 gated: 45 us, 51 with the whole of it).
     const int stage_bytes = kHalf + q.tok * kRow;
-    q.stages = (q.tok <= 64 ? 96 * 1024 : 192 * 1024) / stage_bytes;
+    q.stages = (3 * stage_bytes <= 104 * 1024 ? 104 * 1024 : 200 * 1024) / stage_bytes;
     q.idesc = instruction(p, p.b_mn, p.a_mn, 128, q.tok);
     for (int i = 0; i < p.segs; ++i)
         if (int rc = make_map(&q.a[i], p, p.a[i], p.M, p.a_mn, q.tok)) return rc;
