@@ -52,12 +52,10 @@ inline int check_tensor(const char* op, const char* name, const void* p, int dty
 
 inline size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
 
-// True when rows of 8 elements of `p` can be read with 16-byte accesses (two
-// for fp32): address and row pitch on 16-byte boundaries (8 for e4m3, whose
-// 8 elements are one 8-byte access).
+// True when groups of 8 elements of `p` can be read with 16-byte accesses (two
+// for fp32): address and row pitch on 16-byte boundaries.
 inline bool vec8_ok(const void* p, int dtype, long long ld) {
-    const int a = dtype == TTC_E4M3 ? 8 : 16;
-    return p == nullptr || ((uintptr_t)p % a == 0 && (ld * dtype_size(dtype)) % a == 0);
+    return p == nullptr || ((uintptr_t)p % 16 == 0 && (ld * dtype_size(dtype)) % 16 == 0);
 }
 
 int check_workspace(const char* op, const void* ws, size_t have, size_t need);
@@ -90,9 +88,8 @@ struct ProductEpilogue {
     int split_rows;   // > 0: rows from here on go to out2 ...
     int split_cols;   // (or columns, with > 0 here)
     int split_skip;   // ... after this many that go nowhere
-    unsigned vec;     // bit i: 16-byte accesses (kVec*)
+    bool vec;         // every tensor here can be read and written 8 elements at a time
 };
-enum { kVecOut = 1, kVecOut2 = 2, kVecBias = 4, kVecResidual = 8, kVecPre = 16, kVecGate = 32, kVecUp = 64 };
 struct Product {
     int M, N, K;
     int dtype;  // of A and B
@@ -164,6 +161,29 @@ __device__ __forceinline__ __nv_fp8_e4m3 from_f32<__nv_fp8_e4m3>(float v) {
     return __nv_fp8_e4m3(v);  // nearest even, saturating at +-448, NaN stays NaN
 }
 
+// Eight 16-bit elements in four registers, as floats.
+template <class T>
+__device__ __forceinline__ void unpack8(const uint4& a, float (&v)[8]) {
+    static_assert(sizeof(T) == 2, "16-bit elements");
+    const T* e = reinterpret_cast<const T*>(&a);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(e[i]);
+}
+
+// Two values in one register, each rounded to nearest even.
+template <class T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
 // Eight consecutive elements; n < 8 or `vec` false takes them one by one
 // (elements past n read as 0 and are not stored).
 template <class T>
@@ -172,16 +192,8 @@ __device__ __forceinline__ void load8(const T* p, int n, bool vec, float (&v)[8]
         if constexpr (sizeof(T) == 4) {
             const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
             v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        } else if constexpr (sizeof(T) == 2) {
-            const uint4 a = *reinterpret_cast<const uint4*>(p);
-            const T* e = reinterpret_cast<const T*>(&a);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(e[i]);
         } else {
-            const uint2 a = *reinterpret_cast<const uint2*>(p);
-            const T* e = reinterpret_cast<const T*>(&a);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(e[i]);
+            unpack8<T>(*reinterpret_cast<const uint4*>(p), v);
         }
     } else {
 #pragma unroll
@@ -195,13 +207,9 @@ __device__ __forceinline__ void store8(T* p, int n, bool vec, const float (&v)[8
             *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
             *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
         } else {
-            alignas(16) T e[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(v[i]);
-            if constexpr (sizeof(T) == 2)
-                *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(e);
-            else
-                *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(e);
+            static_assert(sizeof(T) == 2, "8 elements are 16 or 32 bytes");
+            *reinterpret_cast<uint4*>(p) = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]),
+                                                      pack2<T>(v[6], v[7]));
         }
     } else {
 #pragma unroll
@@ -210,37 +218,85 @@ __device__ __forceinline__ void store8(T* p, int n, bool vec, const float (&v)[8
     }
 }
 
-// The same with the type chosen at run time (one branch per 8 elements, the
-// same way for every thread of a launch).
+// The same for a type known to the compiler (DT >= 0) or chosen at run time, one
+// branch per 8 elements. FULL: all eight, vector accesses.
+template <int DT, bool FULL>
 __device__ __forceinline__ void load8_as(int dtype, const void* base, long long i, int n, bool vec, float (&v)[8]) {
-    if (dtype == TTC_BF16)
-        load8(static_cast<const __nv_bfloat16*>(base) + i, n, vec, v);
-    else if (dtype == TTC_F16)
-        load8(static_cast<const __half*>(base) + i, n, vec, v);
+    const int d = DT >= 0 ? DT : dtype;
+    const int m = FULL ? 8 : n;
+    if (d == TTC_BF16)
+        load8(static_cast<const __nv_bfloat16*>(base) + i, m, FULL || vec, v);
+    else if (d == TTC_F16)
+        load8(static_cast<const __half*>(base) + i, m, FULL || vec, v);
     else
-        load8(static_cast<const float*>(base) + i, n, vec, v);
+        load8(static_cast<const float*>(base) + i, m, FULL || vec, v);
 }
+template <int DT, bool FULL>
 __device__ __forceinline__ void store8_as(int dtype, void* base, long long i, int n, bool vec, const float (&v)[8]) {
-    if (dtype == TTC_BF16)
-        store8(static_cast<__nv_bfloat16*>(base) + i, n, vec, v);
-    else if (dtype == TTC_F16)
-        store8(static_cast<__half*>(base) + i, n, vec, v);
+    const int d = DT >= 0 ? DT : dtype;
+    const int m = FULL ? 8 : n;
+    if (d == TTC_BF16)
+        store8(static_cast<__nv_bfloat16*>(base) + i, m, FULL || vec, v);
+    else if (d == TTC_F16)
+        store8(static_cast<__half*>(base) + i, m, FULL || vec, v);
     else
-        store8(static_cast<float*>(base) + i, n, vec, v);
+        store8(static_cast<float*>(base) + i, m, FULL || vec, v);
 }
 
-// Activations in fp32. __expf and __fdividef are good to a few 2^-23, far
-// below the 2^-8 .. 2^-11 of the types the results are rounded to; an fp32
-// result of the products carries their accumulation error already.
-__device__ __forceinline__ float sigmoid_f32(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
+// Activations in fp32, with the hardware's approximate 2^x and 1 / x (good to
+// 2^-22; 2^x takes the rounding of its argument besides), far below the 2^-8
+// .. 2^-11 of the types the results are rounded to; an fp32 result of the
+// products carries their accumulation error already.
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+constexpr float kLog2E = 1.4426950408889634f;
+__device__ __forceinline__ float sigmoid_f32(float z) { return rcp_approx(1.0f + exp2_approx(-kLog2E * z)); }
+// The normal distribution function at z by Abramowitz and Stegun 7.1.26,
+// erfc(x) = (a1 t + ... + a5 t^5) e^(-x^2) + 1.5e-7 at most, t = 1 / (1 + p x):
+// one exponential, which the density needs too, and one reciprocal: half the
+// instructions of erff with a separate exponential.
+__device__ __forceinline__ float normal_cdf(float z, float& e) {
+    const float t = rcp_approx(fmaf(0.3275911f * 0.70710678118654752f, fabsf(z), 1.0f));
+    e = exp2_approx(-0.5f * kLog2E * z * z);
+    float q = fmaf(t, 1.061405429f, -1.453152027f);
+    q = fmaf(t, q, 1.421413741f);
+    q = fmaf(t, q, -0.284496736f);
+    q = fmaf(t, q, 0.254829592f);
+    q = 0.5f * t * q * e;
+    return z < 0.0f ? q : 1.0f - q;
+}
 constexpr float kGeluTanhScale = 1.5957691216057308f;  // 2 sqrt(2 / pi): (1 + tanh t) / 2 = sigmoid(2 t)
 __device__ __forceinline__ float activate(int act, float z) {
     switch (act) {
         case TTC_ACT_RELU: return z < 0.0f ? 0.0f : z;
         case TTC_ACT_SILU: return z * sigmoid_f32(z);
-        case TTC_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+        case TTC_ACT_GELU: {
+            float e;
+            return z * normal_cdf(z, e);
+        }
         case TTC_ACT_GELU_TANH: return z * sigmoid_f32(kGeluTanhScale * (z + 0.044715f * z * z * z));
         default: return z;
+    }
+}
+__device__ __forceinline__ void activate8(int act, float (&v)[8]) {
+    auto all = [&](auto one) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = one(v[i]);
+    };
+    switch (act) {
+        case TTC_ACT_RELU: all([](float z) { return activate(TTC_ACT_RELU, z); }); break;
+        case TTC_ACT_SILU: all([](float z) { return activate(TTC_ACT_SILU, z); }); break;
+        case TTC_ACT_GELU: all([](float z) { return activate(TTC_ACT_GELU, z); }); break;
+        case TTC_ACT_GELU_TANH: all([](float z) { return activate(TTC_ACT_GELU_TANH, z); }); break;
+        default: break;
     }
 }
 // The activation and its derivative.
@@ -257,9 +313,10 @@ __device__ __forceinline__ void activate_grad(int act, float z, float& a, float&
             break;
         }
         case TTC_ACT_GELU: {
-            const float cdf = 0.5f * (1.0f + erff(z * 0.70710678118654752f));
+            float e;
+            const float cdf = normal_cdf(z, e);
             a = z * cdf;
-            da = cdf + z * 0.39894228040143268f * __expf(-0.5f * z * z);
+            da = fmaf(z * 0.39894228040143268f, e, cdf);
             break;
         }
         case TTC_ACT_GELU_TANH: {
@@ -277,70 +334,115 @@ __device__ __forceinline__ void activate_grad(int act, float z, float& a, float&
     }
 }
 
-// Eight consecutive columns of one row of a product, col < N, n = columns left.
-__device__ __forceinline__ void finish_linear(const ProductEpilogue& e, int row, int col, int N, float (&v)[8]) {
-    int n = N - col < 8 ? N - col : 8;
+// What eight consecutive columns (from col < N on) have in common over all rows.
+struct Columns {
+    int col, n;  // n of the eight are inside
+    float scale[2][8];
+    float bias[8];
+};
+__device__ __forceinline__ Columns load_columns(const ProductEpilogue& e, int col, int N) {
+    Columns c;
+    c.col = col;
+    c.n = N - col < 8 ? N - col : 8;
     if (e.row_scales) {
-        const float rs = __ldg(e.row_scales + row);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < n) v[i] = v[i] * rs * __ldg(e.col_scales[0] + col + i);
+        for (int s = 0; s < 2; ++s)
+            if (e.col_scales[s]) load8(e.col_scales[s] + col, c.n, e.vec, c.scale[s]);
     }
-    float t[8];
-    if (e.bias) {
-        load8_as(e.out_dtype, e.bias, col, n, e.vec & kVecBias, t);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] += t[i];
-    }
-    if (e.pre) store8_as(e.out_dtype, e.pre, row * e.ldp + col, n, e.vec & kVecPre, v);
-    if (e.act != TTC_ACT_NONE) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = activate(e.act, v[i]);
-    }
-    if (e.residual) {
-        load8_as(e.out_dtype, e.residual, row * e.ldr + col, n, e.vec & kVecResidual, t);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] += t[i];
-    }
-    void* out = e.out;
-    bool vec = e.vec & kVecOut;
-    long long r = row, c = col;
-    if (e.split_rows > 0 && row >= e.split_rows) {
-        r -= e.split_rows + e.split_skip;
-        if (r < 0) return;
-        out = e.out2;
-        vec = e.vec & kVecOut2;
-    } else if (e.split_cols > 0) {  // split_cols + split_skip is a multiple of 8: no group straddles it
-        if (col >= e.split_cols + e.split_skip) {
-            out = e.out2;
-            vec = e.vec & kVecOut2;
-            c -= e.split_cols + e.split_skip;
-        } else if (col + n > e.split_cols) {
-            n = e.split_cols - col;
-        }
-    }
-    store8_as(e.out_dtype, out, r * e.ldo + c, n, vec, v);
+    if (e.bias) load8_as<-1, false>(e.out_dtype, e.bias, col, c.n, e.vec, c.bias);
+    return c;
 }
-// The same columns of the two products of a gated pair.
-__device__ __forceinline__ void finish_gated(const ProductEpilogue& e, int row, int col, int N, float (&g)[8],
-                                             float (&u)[8]) {
-    const int n = N - col < 8 ? N - col : 8;
-    if (e.row_scales) {
-        const float rs = __ldg(e.row_scales + row);
+
+// The rest of the epilogue for one row of such columns. FULL (all eight inside,
+// e.vec) and the type DT are known to the compiler on the path that matters: the
+// general form, with its predicated single elements, ran 24 instructions a value.
+template <int DT, bool FULL>
+struct Finish {
+    const ProductEpilogue& e;
+    const Columns& c;
+    __device__ __forceinline__ void load(const void* base, long long i, float (&v)[8]) const {
+        load8_as<DT, FULL>(e.out_dtype, base, i, c.n, e.vec, v);
+    }
+    __device__ __forceinline__ void store(void* base, long long i, int n, const float (&v)[8]) const {
+        store8_as<DT, FULL>(e.out_dtype, base, i, n, e.vec, v);
+    }
+    // The residual of a row; issued ahead of the row's values.
+    __device__ __forceinline__ void residual(int row, float (&t)[8]) const {
+        if (e.residual) load(e.residual, row * e.ldr + c.col, t);
+    }
+    // The same from registers, for 16-bit types.
+    __device__ __forceinline__ void unpack(const uint4& a, float (&t)[8]) const {
+        if (DT == TTC_BF16)
+            unpack8<__nv_bfloat16>(a, t);
+        else
+            unpack8<__half>(a, t);
+    }
+    // v holds the product, res what residual() gave.
+    __device__ __forceinline__ void linear(int row, float (&v)[8], const float (&res)[8]) const {
+        int n = c.n;
+        if (e.row_scales) {
+            const float rs = __ldg(e.row_scales + row);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < n) {
-                g[i] = g[i] * rs * __ldg(e.col_scales[0] + col + i);
-                u[i] = u[i] * rs * __ldg(e.col_scales[1] + col + i);
+            for (int i = 0; i < 8; ++i) v[i] = v[i] * rs * c.scale[0][i];
+        }
+        if (e.bias) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] += c.bias[i];
+        }
+        if (e.pre) store(e.pre, row * e.ldp + c.col, n, v);
+        activate8(e.act, v);
+        if (e.residual) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] += res[i];
+        }
+        void* out = e.out;
+        int r = row, k = c.col;
+        if (e.split_rows > 0 && row >= e.split_rows) {
+            r -= e.split_rows + e.split_skip;
+            if (r < 0) return;
+            out = e.out2;
+        } else if (e.split_cols > 0) {  // split_cols + split_skip is a multiple of 8: no group straddles it
+            if (k >= e.split_cols + e.split_skip) {
+                out = e.out2;
+                k -= e.split_cols + e.split_skip;
+            } else if (!FULL && k + n > e.split_cols) {
+                n = e.split_cols - k;
             }
+        }
+        store(out, r * e.ldo + k, n, v);
     }
-    if (e.gate) {
-        store8_as(e.out_dtype, e.gate, row * e.ldp + col, n, e.vec & kVecGate, g);
-        store8_as(e.out_dtype, e.up, row * e.ldp + col, n, e.vec & kVecUp, u);
-    }
+    // The same columns of the two products of a gated pair.
+    __device__ __forceinline__ void gated(int row, float (&g)[8], float (&u)[8]) const {
+        if (e.row_scales) {
+            const float rs = __ldg(e.row_scales + row);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) g[i] = activate(e.act, g[i]) * u[i];
-    store8_as(e.out_dtype, e.out, row * e.ldo + col, n, e.vec & kVecOut, g);
+            for (int i = 0; i < 8; ++i) {
+                g[i] = g[i] * rs * c.scale[0][i];
+                u[i] = u[i] * rs * c.scale[1][i];
+            }
+        }
+        if (e.gate) {
+            store(e.gate, row * e.ldp + c.col, c.n, g);
+            store(e.up, row * e.ldp + c.col, c.n, u);
+        }
+        activate8(e.act, g);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g[i] *= u[i];
+        store(e.out, row * e.ldo + c.col, c.n, g);
+    }
+};
+
+// f(Finish) for the columns c; `full` is the same for the whole warp.
+template <class F>
+__device__ __forceinline__ void with_finish(const ProductEpilogue& e, const Columns& c, bool full, F&& f) {
+    if (!full)
+        f(Finish<-1, false>{e, c});
+    else if (e.out_dtype == TTC_BF16)
+        f(Finish<TTC_BF16, true>{e, c});
+    else if (e.out_dtype == TTC_F16)
+        f(Finish<TTC_F16, true>{e, c});
+    else
+        f(Finish<TTC_F32, true>{e, c});
 }
 #endif  // __CUDACC__
 

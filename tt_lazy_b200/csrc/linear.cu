@@ -4,6 +4,7 @@
 // products themselves: linear_tc.cu).
 #include <algorithm>
 #include <cstring>
+#include <type_traits>
 
 #include "ffn.cuh"
 
@@ -118,15 +119,18 @@ int check_gated_backward(const ttc_gated_linear_backward_desc& d) {
 
 // ---------------------------------------- element-wise half of the backward
 // A block of 8 warps walks a band of rows of a 256-column stripe: a lane owns
-// 8 columns, a warp one row at a time. Memory bound: each value is read once
-// and written once, 16 bytes per lane and access.
+// 8 columns, a warp one row at a time, so that a column's sum for dbias stays
+// in a register. Memory bound: each value is read once and written once, 16
+// bytes per lane and access. 4096 x 8192 in bf16: 43 us with gelu (4.7 TB/s), 56
+// us for the gated pair with silu (6.0 TB/s). Two rows of loads in flight per
+// warp instead of one cost more in registers than they hid (72 and 88 us).
 constexpr int kStripe = 256, kBandWarps = 8;
 // Rows of a block: 64, more when that would make over 256 bands of partial sums.
 int band_rows(int M) { return std::max(64, (M + 255) / 256); }
 int bands(int M) { return (M + band_rows(M) - 1) / band_rows(M); }
 
 struct LinearGradParams {
-    int M, N, act, band_rows;
+    int M, N, band_rows;
     const void *dy, *pre;
     long long lddy, ldp;
     void* dz;  // or NULL: only the column sums
@@ -135,7 +139,8 @@ struct LinearGradParams {
     bool vec_dy, vec_pre, vec_dz;
 };
 
-template <class T>
+// ACT at compile time: as a switch in the loop it took 85 us instead of 49.
+template <class T, int ACT>
 __global__ void __launch_bounds__(32 * kBandWarps) linear_grad_kernel(const __grid_constant__ LinearGradParams p) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int col = blockIdx.y * kStripe + lane * 8, n = p.N - col;
@@ -145,13 +150,13 @@ __global__ void __launch_bounds__(32 * kBandWarps) linear_grad_kernel(const __gr
         for (long long r = (long long)blockIdx.x * p.band_rows + warp; r < r1; r += kBandWarps) {
             float g[8], z[8];
             load8(static_cast<const T*>(p.dy) + r * p.lddy + col, n, p.vec_dy, g);
-            if (p.act != TTC_ACT_NONE) {
+            if (ACT != TTC_ACT_NONE) {
                 load8(static_cast<const T*>(p.pre) + r * p.ldp + col, n, p.vec_pre, z);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    float a, da;
-                    activate_grad(p.act, z[i], a, da);
-                    g[i] *= da;
+                    float y, dy;
+                    activate_grad(ACT, z[i], y, dy);
+                    g[i] *= dy;
                 }
             }
             if (p.dz) store8(static_cast<T*>(p.dz) + r * p.lddz + col, n, p.vec_dz, g);
@@ -174,7 +179,7 @@ __global__ void __launch_bounds__(32 * kBandWarps) linear_grad_kernel(const __gr
 }
 
 struct GatedGradParams {
-    int M, N, act, band_rows;
+    int M, N, band_rows;
     const void *dy, *gate, *up;
     long long lddy, ldp;
     void *dg, *du;
@@ -182,7 +187,7 @@ struct GatedGradParams {
     bool vec_dy, vec_gate, vec_up;  // dg and du are always padded
 };
 
-template <class T>
+template <class T, int ACT>
 __global__ void __launch_bounds__(32 * kBandWarps) gated_grad_kernel(const __grid_constant__ GatedGradParams p) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int col = blockIdx.y * kStripe + lane * 8, n = p.N - col;
@@ -195,13 +200,25 @@ __global__ void __launch_bounds__(32 * kBandWarps) gated_grad_kernel(const __gri
         load8(static_cast<const T*>(p.up) + r * p.ldp + col, n, p.vec_up, u);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            float a, da;
-            activate_grad(p.act, g[i], a, da);
-            g[i] = d[i] * u[i] * da;
-            u[i] = d[i] * a;
+            float y, dy;
+            activate_grad(ACT, g[i], y, dy);
+            g[i] = d[i] * u[i] * dy;
+            u[i] = d[i] * y;
         }
         store8(static_cast<T*>(p.dg) + r * p.ldd + col, n, true, g);
         store8(static_cast<T*>(p.du) + r * p.ldd + col, n, true, u);
+    }
+}
+
+// f(the activation as a compile-time constant)
+template <class F>
+void with_activation(int act, F&& f) {
+    switch (act) {
+        case TTC_ACT_RELU: f(std::integral_constant<int, TTC_ACT_RELU>()); break;
+        case TTC_ACT_SILU: f(std::integral_constant<int, TTC_ACT_SILU>()); break;
+        case TTC_ACT_GELU: f(std::integral_constant<int, TTC_ACT_GELU>()); break;
+        case TTC_ACT_GELU_TANH: f(std::integral_constant<int, TTC_ACT_GELU_TANH>()); break;
+        default: f(std::integral_constant<int, TTC_ACT_NONE>());
     }
 }
 
@@ -219,7 +236,12 @@ struct Carver {
     }
 };
 
-unsigned vec_bit(unsigned bit, const void* p, int dtype, long long ld) { return vec8_ok(p, dtype, ld) ? bit : 0u; }
+bool all_vec(const ProductEpilogue& e) {
+    const int t = e.out_dtype;
+    return vec8_ok(e.out, t, e.ldo) && vec8_ok(e.out2, t, e.ldo) && vec8_ok(e.bias, t, 0) &&
+           vec8_ok(e.residual, t, e.ldr) && vec8_ok(e.pre, t, e.ldp) && vec8_ok(e.gate, t, e.ldp) &&
+           vec8_ok(e.up, t, e.ldp) && vec8_ok(e.col_scales[0], TTC_F32, 0) && vec8_ok(e.col_scales[1], TTC_F32, 0);
+}
 
 Product linear_product(const ttc_linear_desc& d) {
     Product p;
@@ -244,8 +266,7 @@ Product linear_product(const ttc_linear_desc& d) {
     e.ldp = d.ldp;
     e.row_scales = d.x_scales;
     e.col_scales[0] = d.w_scales;
-    e.vec = vec_bit(kVecOut, d.y, d.y_dtype, d.ldy) | vec_bit(kVecBias, d.bias, d.y_dtype, 0) |
-            vec_bit(kVecResidual, d.residual, d.y_dtype, d.ldr) | vec_bit(kVecPre, d.pre, d.y_dtype, d.ldp);
+    e.vec = all_vec(e);
     return p;
 }
 
@@ -273,8 +294,7 @@ Product gated_product(const ttc_gated_linear_desc& d) {
     e.row_scales = d.x_scales;
     e.col_scales[0] = d.wg_scales;
     e.col_scales[1] = d.wu_scales;
-    e.vec = vec_bit(kVecOut, d.y, d.y_dtype, d.ldy) | vec_bit(kVecGate, d.gate, d.y_dtype, d.ldp) |
-            vec_bit(kVecUp, d.up, d.y_dtype, d.ldp);
+    e.vec = all_vec(e);
     return p;
 }
 
@@ -295,7 +315,7 @@ Product grad_product(int M, int N, int K, int dtype, Operand a, bool a_mn, Opera
     p.epi.out = out;
     p.epi.ldo = ldo;
     p.epi.out_dtype = dtype;
-    p.epi.vec = vec_bit(kVecOut, out, dtype, ldo);
+    p.epi.vec = all_vec(p.epi);
     return p;
 }
 
@@ -337,7 +357,6 @@ int plan_linear_backward(const ttc_linear_backward_desc& d, void* ws, size_t* by
         g.M = d.M;
         g.N = d.N;
         g.band_rows = band_rows(d.M);
-        g.act = d.act;
         g.dy = d.dy;
         g.pre = d.pre;
         g.lddy = d.lddy;
@@ -347,10 +366,12 @@ int plan_linear_backward(const ttc_linear_backward_desc& d, void* ws, size_t* by
         g.vec_pre = vec8_ok(d.pre, d.dtype, d.ldp);
         g.vec_dz = true;
         const dim3 grid((unsigned)bands(d.M), (unsigned)((d.N + kStripe - 1) / kStripe));
-        if (d.dtype == TTC_BF16)
-            linear_grad_kernel<__nv_bfloat16><<<grid, 32 * kBandWarps, 0, rt().stream>>>(g);
-        else
-            linear_grad_kernel<__half><<<grid, 32 * kBandWarps, 0, rt().stream>>>(g);
+        with_activation(d.act, [&](auto act) {
+            if (d.dtype == TTC_BF16)
+                linear_grad_kernel<__nv_bfloat16, act()><<<grid, 32 * kBandWarps, 0, rt().stream>>>(g);
+            else
+                linear_grad_kernel<__half, act()><<<grid, 32 * kBandWarps, 0, rt().stream>>>(g);
+        });
         count_launch();
         if (int rc = check_cuda(cudaGetLastError(), "linear_backward launch")) return rc;
         if (d.dbias)
@@ -390,7 +411,7 @@ int plan_gated_backward(const ttc_gated_linear_backward_desc& d, void* ws, size_
     }
     pw.epi.split_skip = (int)(np - d.N);
     pw.epi.out2 = d.dwu;
-    pw.epi.vec |= vec_bit(kVecOut2, d.dwu, d.dtype, d.lddw);
+    pw.epi.vec = all_vec(pw.epi);
     size_t most = 0;
     if (d.dx) most = std::max(most, product_scratch(px));
     if (d.dwg) most = std::max(most, product_scratch(pw));
@@ -401,7 +422,6 @@ int plan_gated_backward(const ttc_gated_linear_backward_desc& d, void* ws, size_
     g.M = d.M;
     g.N = d.N;
     g.band_rows = band_rows(d.M);
-    g.act = d.act;
     g.dy = d.dy;
     g.gate = d.gate;
     g.up = d.up;
@@ -414,10 +434,12 @@ int plan_gated_backward(const ttc_gated_linear_backward_desc& d, void* ws, size_
     g.vec_gate = vec8_ok(d.gate, d.dtype, d.ldp);
     g.vec_up = vec8_ok(d.up, d.dtype, d.ldp);
     const dim3 grid((unsigned)bands(d.M), (unsigned)((d.N + kStripe - 1) / kStripe));
-    if (d.dtype == TTC_BF16)
-        gated_grad_kernel<__nv_bfloat16><<<grid, 32 * kBandWarps, 0, rt().stream>>>(g);
-    else
-        gated_grad_kernel<__half><<<grid, 32 * kBandWarps, 0, rt().stream>>>(g);
+    with_activation(d.act, [&](auto act) {
+        if (d.dtype == TTC_BF16)
+            gated_grad_kernel<__nv_bfloat16, act()><<<grid, 32 * kBandWarps, 0, rt().stream>>>(g);
+        else
+            gated_grad_kernel<__half, act()><<<grid, 32 * kBandWarps, 0, rt().stream>>>(g);
+    });
     count_launch();
     if (int rc = check_cuda(cudaGetLastError(), "gated_linear_backward launch")) return rc;
     if (d.dx)

@@ -5,7 +5,7 @@
 //
 // Two kernels:
 //   pair_kernel   large products: persistent CTA pairs (cta_group::2), one
-//                 256 x 256 tile a pair, operands in a ring of 6 stages.
+//                 256 x 256 tile a pair, operands in a ring of 5 stages.
 //   tile_kernel   few rows of x (single tokens, small batches): one 128-wide
 //                 tile of the weight's output columns against up to 256 rows,
 //                 the weight as the 128-row operand of the instruction, the
@@ -35,8 +35,11 @@
 namespace ttc {
 namespace {
 
-constexpr int kThreads = 192;      // warp 0: TMA, warp 1: MMA, warps 2-5: epilogue
-constexpr int kTileThreads = 320;  // tile kernel: warps 2-9 empty the accumulator, all of them finish the outputs
+// Warp 0: TMA, warp 1: MMA, warps 2-9: epilogue, two for each quarter of the
+// tensor-memory lanes (one each left its scheduler waiting on itself: the
+// epilogue of a 256 x 256 tile took 35 us).
+constexpr int kEpilogueWarps = 8;
+constexpr int kThreads = 32 * (2 + kEpilogueWarps);
 constexpr int kRow = 128;      // bytes of K a stage holds of each row
 constexpr int kBox = 64 * kRow;  // an MN-major box: 64 k-rows of 64 16-bit columns
 
@@ -103,11 +106,11 @@ __device__ __forceinline__ void load_rows(uint32_t dst, const CUtensorMap* map, 
 }
 
 // ---------------------------------------------------------------- pair kernel
-constexpr int kStages = 6;
 constexpr int kHalf = 128 * kRow;       // one CTA's rows of A, or of B: 16 KB
 constexpr int kStageBytes = 2 * kHalf;  // 32 KB
+constexpr int kStages = 5;
 constexpr int kStaging = 32 * 64 * 4;   // one epilogue warp's 32 rows x 64 fp32
-constexpr int kPairSmem = kStages * kStageBytes + 4 * kStaging + 1024 + 256;
+constexpr int kPairSmem = kStages * kStageBytes + kEpilogueWarps * kStaging + 1024 + 256;
 static_assert(kPairSmem <= 232448, "pair kernel: shared memory");
 constexpr int kGroupM = 8;  // pair tiles of M that are walked together, so that their operands stay in L2
 
@@ -132,7 +135,7 @@ __global__ void __launch_bounds__(kThreads, 1) pair_kernel(const __grid_constant
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint8_t* staging = smem + kStages * kStageBytes;
-    uint64_t* bars = (uint64_t*)(staging + 4 * kStaging);
+    uint64_t* bars = (uint64_t*)(staging + kEpilogueWarps * kStaging);
     uint32_t* tmem_slot = (uint32_t*)(bars + 2 * kStages + 4);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
@@ -150,7 +153,7 @@ __global__ void __launch_bounds__(kThreads, 1) pair_kernel(const __grid_constant
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(tfull_bar(b), 1);
-            mbar_init(tempty_bar(b), 8);
+            mbar_init(tempty_bar(b), 2 * kEpilogueWarps);
         }
         mbar_fence_init();
     }
@@ -262,8 +265,8 @@ __global__ void __launch_bounds__(kThreads, 1) pair_kernel(const __grid_constant
             }
         }
     } else {
-        const int quarter = warp & 3;  // this warp's quarter of the 128 tensor-memory lanes
-        float4* const mine = reinterpret_cast<float4*>(staging + quarter * kStaging);
+        const int quarter = warp & 3, which = (warp - 2) >> 2;  // which of the quarter's two warps
+        float4* const mine = reinterpret_cast<float4*>(staging + (warp - 2) * kStaging);
         auto chunk = [&](int row, int c) -> float4& { return mine[row * 16 + (c ^ (row & 7))]; };
         // two 16-byte chunks from c on, in the order that keeps 8 lanes on 8 different banks
         auto take8 = [&](int row, int c, int flip, float (&v)[8]) {
@@ -271,62 +274,84 @@ __global__ void __launch_bounds__(kThreads, 1) pair_kernel(const __grid_constant
             const float4 lo = flip ? y : x, hi = flip ? x : y;
             v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w, v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
         };
+        const bool early = p.epi.residual && p.epi.vec && p.epi.out_dtype != TTC_F32;
         int t = 0;
         for (int tile = cluster_id; tile < num_tiles; tile += nclusters, ++t) {
             int mt, nt;
             pair_coords(tile, q.m_tiles, q.n_tiles, mt, nt);
             const int b = t & 1;
+            const int row0 = mt * 256 + (int)rank * 128 + quarter * 32;
+            // The residual of a chunk's 8 rows a lane, asked for before the chunk is
+            // ready (the first one before the tile is): 16-bit, whole groups only.
+            uint4 res[8];
+            auto ahead = [&](int c) { return early && nt * 256 + c * 64 + 64 <= p.N; };
+            auto fetch = [&](int c) {
+                if (!ahead(c)) return;
+                const uint16_t* from = static_cast<const uint16_t*>(p.epi.residual) + nt * 256 + c * 64 + (lane & 7) * 8;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int row = row0 + i * 4 + (lane >> 3);
+                    if (row < p.M) res[i] = *reinterpret_cast<const uint4*>(from + row * p.epi.ldr);
+                }
+            };
+            fetch(which);
             if (!__all_sync(0xffffffffu, mbar_wait(tfull_bar(b), (t >> 1) & 1, q.wait_limit))) {
                 failed = true;
                 break;
             }
             tc_fence_after();
-            const int row0 = mt * 256 + (int)rank * 128 + quarter * 32;
-            const int col0 = nt * (p.gated ? 128 : 256);
             const uint32_t acc = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(b * 256);
-            for (int c = 0; c < 4; ++c) {
-                uint32_t r[2][32];
-                tc_ld_32x32b_x32(acc + (p.gated ? c * 32 : c * 64), r[0]);
-                tc_ld_32x32b_x32(acc + (p.gated ? 128 + c * 32 : c * 64 + 32), r[1]);
-                tc_wait_ld();
-                if (c == 3) {  // the accumulator is read: the MMA warp may start the tile after next
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive_cluster(cluster_addr(tempty_bar(b), 0));
+#pragma unroll 1
+            for (int c = which; c < 4; c += 2) {
+                // gated: 32 outputs, 4 lanes a row, 8 rows at a time; linear: 64, 8 lanes, 4 rows
+                const int width = p.gated ? 32 : 64, first = nt * (p.gated ? 128 : 256) + c * width;
+                const int j = p.gated ? lane & 3 : lane & 7, col = first + j * 8;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t r[32];
+                    tc_ld_32x32b_x32(acc + c * width + (h == 0 ? 0 : p.gated ? 128 : 32), r);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        chunk(lane, h * 8 + k) =
+                            make_float4(__uint_as_float(r[4 * k]), __uint_as_float(r[4 * k + 1]),
+                                        __uint_as_float(r[4 * k + 2]), __uint_as_float(r[4 * k + 3]));
                 }
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        chunk(lane, h * 8 + j) =
-                            make_float4(__uint_as_float(r[h][4 * j]), __uint_as_float(r[h][4 * j + 1]),
-                                        __uint_as_float(r[h][4 * j + 2]), __uint_as_float(r[h][4 * j + 3]));
+                tc_fence_before();
                 __syncwarp();
-                if (p.gated) {
-                    const int j = lane & 3, col = col0 + c * 32 + j * 8;
-#pragma unroll 1
-                    for (int i = 0; i < 4; ++i) {
-                        const int lr = i * 8 + (lane >> 2), row = row0 + lr;
-                        if (row < p.M && col < p.N) {
-                            float g[8], u[8];
-                            take8(lr, 2 * j, 0, g);
-                            take8(lr, 8 + 2 * j, 0, u);
-                            finish_gated(p.epi, row, col, p.N, g, u);
+                // read: the MMA warp may start the tile after next
+                if (c >= 2 && lane == 0) mbar_arrive_cluster(cluster_addr(tempty_bar(b), 0));
+                if (col < p.N) {
+                    const Columns cols = load_columns(p.epi, col, p.N);
+                    with_finish(p.epi, cols, p.epi.vec && first + width <= p.N, [&](const auto& finish) {
+                        if (p.gated) {
+#pragma unroll 2
+                            for (int i = 0; i < 4; ++i) {
+                                const int lr = i * 8 + (lane >> 2), row = row0 + lr;
+                                if (row >= p.M) break;
+                                float g[8], u[8];
+                                take8(lr, 2 * j, 0, g);
+                                take8(lr, 8 + 2 * j, 0, u);
+                                finish.gated(row, g, u);
+                            }
+                            return;
                         }
-                    }
-                } else {
-                    const int j = lane & 7, col = col0 + c * 64 + j * 8;
-#pragma unroll 1
-                    for (int i = 0; i < 8; ++i) {
-                        const int lr = i * 4 + (lane >> 3), row = row0 + lr;
-                        if (row < p.M && col < p.N) {
-                            float v[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const int lr = i * 4 + (lane >> 3), row = row0 + lr;
+                            if (row >= p.M) break;
+                            float v[8], t[8];
+                            if (ahead(c))
+                                finish.unpack(res[i], t);
+                            else
+                                finish.residual(row, t);
                             take8(lr, 2 * j, j >> 2, v);
-                            finish_linear(p.epi, row, col, p.N, v);
+                            finish.linear(row, v, t);
                         }
-                    }
+                    });
                 }
                 __syncwarp();
+                if (c < 2) fetch(c + 2);
             }
         }
     }
@@ -357,7 +382,7 @@ __device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
 }
 
 template <bool F8>
-__global__ void __launch_bounds__(kTileThreads) tile_kernel(const __grid_constant__ ProductParams q) {
+__global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ ProductParams q) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     const int stage_bytes = kHalf + q.tok * kRow, stages = q.stages;
@@ -511,17 +536,26 @@ __global__ void __launch_bounds__(kTileThreads) tile_kernel(const __grid_constan
             v[0] += lo.x, v[1] += lo.y, v[2] += lo.z, v[3] += lo.w, v[4] += hi.x, v[5] += hi.y, v[6] += hi.z, v[7] += hi.w;
         }
     };
-    for (int it = split * share + threadIdx.x; it < last; it += kTileThreads) {
-        const int row = it / groups, j = it % groups, col = n0 + j * 8;
-        if (col >= p.N) continue;
-        float v[8], u[8];
-        take8(row, j * 8, v);
-        if (p.gated) {
-            take8(row, 64 + j * 8, u);
-            finish_gated(p.epi, m0 + row, col, p.N, v, u);
-        } else {
-            finish_linear(p.epi, m0 + row, col, p.N, v);
-        }
+    // kThreads is a multiple of 16: a thread has the same columns in every item
+    const int j = (split * share + threadIdx.x) % groups, col = n0 + j * 8;
+    if (col < p.N) {
+        const Columns cols = load_columns(p.epi, col, p.N);
+        with_finish(p.epi, cols, p.epi.vec && n0 + (p.gated ? 64 : 128) <= p.N, [&](const auto& finish) {
+#pragma unroll 2
+            for (int it = split * share + threadIdx.x; it < last; it += kThreads) {
+                const int row = it / groups;
+                float v[8], u[8];
+                if (p.gated) {
+                    take8(row, j * 8, v);
+                    take8(row, 64 + j * 8, u);
+                    finish.gated(m0 + row, v, u);
+                } else {
+                    finish.residual(m0 + row, u);
+                    take8(row, j * 8, v);
+                    finish.linear(m0 + row, v, u);
+                }
+            }
+        });
     }
     if (splits > 1) {  // nobody leaves while its shared memory is still read
         __syncwarp();
@@ -624,7 +658,7 @@ int launch_tile(ProductParams& q) {
     cudaLaunchAttribute attr[2];
     cfg.attrs = attr;
     cfg.numAttrs = launch_attributes(attr, q.splits);
-    cfg.blockDim = dim3(kTileThreads, 1, 1);
+    cfg.blockDim = dim3(kThreads, 1, 1);
     cfg.dynamicSmemBytes = (size_t)ring + 1024 + 256;
     cfg.stream = rt().stream;
     cfg.gridDim = dim3((unsigned)((long long)q.m_tiles * q.n_tiles * q.splits), 1, 1);
@@ -678,7 +712,8 @@ int run_product(const Product& given, void* scratch) {
     q.wait_limit = q.stall ? kStallTestLimitCycles : kWaitLimitCycles;
     const int nb = p.gated ? 2 : p.segs;
 
-    const long long pair_m = ((long long)p.M + 255) / 256, pair_n = ((long long)p.N + (p.gated ? 127 : 255)) / (p.gated ? 128 : 256);
+    const int pair_width = p.gated ? 128 : 256;
+    const long long pair_m = ((long long)p.M + 255) / 256, pair_n = ((long long)p.N + pair_width - 1) / pair_width;
     if (pair_m * pair_n > INT32_MAX / 2) return set_error(TTC_ERR_UNSUPPORTED, "tt_cuda: too many output tiles");
     if (p.M > 256 && pair_m * pair_n >= sms / 2) {
         q.m_tiles = (int)pair_m;
