@@ -292,7 +292,7 @@ def test_rms_norm_gradient_against_differences(lib):
 # --------------------------------------------------------------------------------------------------- products
 SHAPES = [(1, 64, 64), (1, 1024, 512), (3, 8, 8), (2, 136, 1000), (16, 256, 320), (17, 200, 72), (33, 129, 257),
           (64, 512, 128), (77, 1000, 264), (130, 384, 520), (256, 1024, 512), (300, 1, 1), (1, 1, 4096), (513, 264, 136),
-          (1000, 776, 200), (1300, 4104, 136), (2304, 2080, 72)]
+          (1000, 776, 200), (1300, 4104, 136), (2304, 2080, 72), (2560, 2050, 64)]
 
 
 def product_inputs(g, M, N, K, dtype, trans_w, pad, shift, weights=("w",), scale=None):

@@ -286,10 +286,12 @@ __device__ __forceinline__ float activate(int act, float z) {
         default: return z;
     }
 }
-__device__ __forceinline__ void activate8(int act, float (&v)[8]) {
+// n values, with the choice of activation outside the loop.
+template <int N>
+__device__ __forceinline__ void activate_all(int act, float (&v)[N]) {
     auto all = [&](auto one) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = one(v[i]);
+        for (int i = 0; i < N; ++i) v[i] = one(v[i]);
     };
     switch (act) {
         case TTC_ACT_RELU: all([](float z) { return activate(TTC_ACT_RELU, z); }); break;
@@ -370,13 +372,6 @@ struct Finish {
     __device__ __forceinline__ void residual(int row, float (&t)[8]) const {
         if (e.residual) load(e.residual, row * e.ldr + c.col, t);
     }
-    // The same from registers, for 16-bit types.
-    __device__ __forceinline__ void unpack(const uint4& a, float (&t)[8]) const {
-        if (DT == TTC_BF16)
-            unpack8<__nv_bfloat16>(a, t);
-        else
-            unpack8<__half>(a, t);
-    }
     // v holds the product, res what residual() gave.
     __device__ __forceinline__ void linear(int row, float (&v)[8], const float (&res)[8]) const {
         int n = c.n;
@@ -390,7 +385,7 @@ struct Finish {
             for (int i = 0; i < 8; ++i) v[i] += c.bias[i];
         }
         if (e.pre) store(e.pre, row * e.ldp + c.col, n, v);
-        activate8(e.act, v);
+        activate_all<8>(e.act, v);
         if (e.residual) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] += res[i];
@@ -425,12 +420,60 @@ struct Finish {
             store(e.gate, row * e.ldp + c.col, c.n, g);
             store(e.up, row * e.ldp + c.col, c.n, u);
         }
-        activate8(e.act, g);
+        activate_all<8>(e.act, g);
 #pragma unroll
         for (int i = 0; i < 8; ++i) g[i] *= u[i];
         store(e.out, row * e.ldo + c.col, c.n, g);
     }
 };
+
+// The epilogue of single elements, for tensors that nothing wider can reach:
+// element (row, col) of a product, with its column's scales and bias.
+__device__ __forceinline__ float load1(int dtype, const void* base, long long i) {
+    return dtype == TTC_BF16  ? to_f32(static_cast<const __nv_bfloat16*>(base)[i])
+           : dtype == TTC_F16 ? to_f32(static_cast<const __half*>(base)[i])
+                              : static_cast<const float*>(base)[i];
+}
+__device__ __forceinline__ void store1(int dtype, void* base, long long i, float v) {
+    if (dtype == TTC_BF16)
+        static_cast<__nv_bfloat16*>(base)[i] = from_f32<__nv_bfloat16>(v);
+    else if (dtype == TTC_F16)
+        static_cast<__half*>(base)[i] = from_f32<__half>(v);
+    else
+        static_cast<float*>(base)[i] = v;
+}
+__device__ __forceinline__ void finish_one_linear(const ProductEpilogue& e, int row, int col, float v, float scale,
+                                                  float bias) {
+    if (e.row_scales) v = v * __ldg(e.row_scales + row) * scale;
+    v += bias;
+    if (e.pre) store1(e.out_dtype, e.pre, row * e.ldp + col, v);
+    v = activate(e.act, v);
+    if (e.residual) v += load1(e.out_dtype, e.residual, row * e.ldr + col);
+    void* out = e.out;
+    if (e.split_rows > 0 && row >= e.split_rows) {
+        row -= e.split_rows + e.split_skip;
+        if (row < 0) return;
+        out = e.out2;
+    } else if (e.split_cols > 0 && col >= e.split_cols) {
+        col -= e.split_cols + e.split_skip;
+        if (col < 0) return;
+        out = e.out2;
+    }
+    store1(e.out_dtype, out, row * e.ldo + col, v);
+}
+__device__ __forceinline__ void finish_one_gated(const ProductEpilogue& e, int row, int col, float g, float u,
+                                                 float gscale, float uscale) {
+    if (e.row_scales) {
+        const float rs = __ldg(e.row_scales + row);
+        g = g * rs * gscale;
+        u = u * rs * uscale;
+    }
+    if (e.gate) {
+        store1(e.out_dtype, e.gate, row * e.ldp + col, g);
+        store1(e.out_dtype, e.up, row * e.ldp + col, u);
+    }
+    store1(e.out_dtype, e.out, row * e.ldo + col, activate(e.act, g) * u);
+}
 
 // f(Finish) for the columns c; `full` is the same for the whole warp.
 template <class F>

@@ -45,6 +45,7 @@ constexpr int kBox = 64 * kRow;  // an MN-major box: 64 k-rows of 64 16-bit colu
 
 struct alignas(64) ProductParams {
     CUtensorMap a[2], b[2];
+    CUtensorMap out, out2, aside, residual;  // pair_kernel's tensors; out2: or up; aside: pre or gate
     Product p;
     int kb_seg, kb_total;  // k-blocks of one segment, of all segments
     int m_tiles, n_tiles;
@@ -106,11 +107,54 @@ __device__ __forceinline__ void load_rows(uint32_t dst, const CUtensorMap* map, 
 }
 
 // ---------------------------------------------------------------- pair kernel
+// TMA stores from a warp's own shared memory, tracked per issuing thread.
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int c0, int c1) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"((uint64_t)map),
+                 "r"(src), "r"(c0), "r"(c1)
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+template <int PENDING>
+__device__ __forceinline__ void tma_store_wait_read() {
+    asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(PENDING) : "memory");
+}
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Sixteen bytes of DT from floats, and back.
+template <int DT>
+constexpr int kPer16 = DT == TTC_F32 ? 4 : 8;
+template <int DT>
+__device__ __forceinline__ uint4 pack16(const float* v) {
+    if constexpr (DT == TTC_F32)
+        return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    else if constexpr (DT == TTC_BF16)
+        return make_uint4(pack2<__nv_bfloat16>(v[0], v[1]), pack2<__nv_bfloat16>(v[2], v[3]),
+                          pack2<__nv_bfloat16>(v[4], v[5]), pack2<__nv_bfloat16>(v[6], v[7]));
+    else
+        return make_uint4(pack2<__half>(v[0], v[1]), pack2<__half>(v[2], v[3]), pack2<__half>(v[4], v[5]),
+                          pack2<__half>(v[6], v[7]));
+}
+template <int DT>
+__device__ __forceinline__ void add16(const uint4& a, float* v) {
+    if constexpr (DT == TTC_F32) {
+        v[0] += __uint_as_float(a.x), v[1] += __uint_as_float(a.y), v[2] += __uint_as_float(a.z);
+        v[3] += __uint_as_float(a.w);
+    } else {
+        float t[8];
+        if constexpr (DT == TTC_BF16)
+            unpack8<__nv_bfloat16>(a, t);
+        else
+            unpack8<__half>(a, t);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += t[i];
+    }
+}
+
 constexpr int kHalf = 128 * kRow;       // one CTA's rows of A, or of B: 16 KB
 constexpr int kStageBytes = 2 * kHalf;  // 32 KB
 constexpr int kStages = 5;
-constexpr int kStaging = 32 * 64 * 4;   // one epilogue warp's 32 rows x 64 fp32
-constexpr int kPairSmem = kStages * kStageBytes + kEpilogueWarps * kStaging + 1024 + 256;
+constexpr int kBuffer = 32 * kRow;      // an epilogue warp's 32 rows of 128 bytes; it has two
+constexpr int kPairSmem = kStages * kStageBytes + kEpilogueWarps * 2 * kBuffer + 1024 + 512;
 static_assert(kPairSmem <= 232448, "pair kernel: shared memory");
 constexpr int kGroupM = 8;  // pair tiles of M that are walked together, so that their operands stay in L2
 
@@ -122,21 +166,264 @@ __device__ __forceinline__ void pair_coords(int tile, int m_tiles, int n_tiles, 
     nt = local / rows;
 }
 
+// The epilogue warps' part; true when a wait ran out.
+template <int DT>
+__device__ __forceinline__ bool pair_epilogue(const ProductParams& q, uint8_t* staging, uint32_t tmem_base,
+                                              uint32_t bar0, uint32_t rank) {
+    constexpr int W = kRow / (DT == TTC_F32 ? 4 : 2);  // columns of a chunk
+    constexpr int G = kPer16<DT>;                      // columns of 16 bytes
+    const Product& p = q.p;
+    const ProductEpilogue& e = p.epi;
+    const int lane = threadIdx.x & 31, w = (threadIdx.x >> 5) - 2;
+    const int quarter = (w + 2) & 3, which = w >> 2;  // quarter of the tensor-memory lanes; which of its two warps
+    uint8_t* const mine = staging + w * 2 * kBuffer;
+    const uint32_t mine_addr = smem_u32(mine), res_bar = bar0 + 8u * (2 * kStages + 4 + 2 * w);
+    const int tile_cols = p.gated ? 128 : 256, chunks = tile_cols / W;
+    const int num_tiles = q.m_tiles * q.n_tiles, nclusters = gridDim.x >> 1;
+    uint32_t res_phase = 0, res_pending = 0;  // a bit a buffer
+    int seq = 0;             // chunks sent so far: the next one goes through buffer seq & 1
+    auto slot = [&](int buffer, int i) -> uint4& {  // 16-byte group i of this lane's row
+        return *reinterpret_cast<uint4*>(mine + buffer * kBuffer + lane * kRow + ((i ^ (lane & 7)) << 4));
+    };
+    // TMA writes the chunk of columns from `first` on: aligned tensors, one output
+    // tensor, and per-column operands that do not end inside it.
+    auto by_tma = [&](int row0, int first) {
+        if (!e.vec || ((e.bias || e.row_scales) && first + W > p.N)) return false;
+        if (e.split_rows > 0) return row0 + 32 <= e.split_rows || row0 >= e.split_rows + e.split_skip;
+        if (e.split_cols > 0) return first + W <= e.split_cols || first >= e.split_cols + e.split_skip;
+        return true;
+    };
+    auto fetch_residual = [&](int buffer, int row0, int first) {
+        res_pending |= 1u << buffer;
+        if (lane == 0) {
+            mbar_arrive_expect_tx(res_bar + 8u * buffer, kBuffer);
+            tma_load_2d(mine_addr + buffer * kBuffer, &q.residual, res_bar + 8u * buffer, first, row0);
+        }
+    };
+    auto await_residual = [&](int buffer) {
+        const bool ok = __all_sync(0xffffffffu, mbar_wait(res_bar + 8u * buffer, res_phase >> buffer & 1, q.wait_limit));
+        res_phase ^= 1u << buffer;
+        res_pending &= ~(1u << buffer);
+        return ok;
+    };
+    // Never leave with copies in flight.
+    auto leave = [&](bool failed) {
+        for (int k = 0; k < 2; ++k)
+            if (res_pending >> k & 1) await_residual(k);
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        return failed;
+    };
+    const bool early = e.residual && !e.pre;  // two chunks' residuals before the tile is ready
+
+    int t = 0;
+    for (int tile = blockIdx.x >> 1; tile < num_tiles; tile += nclusters, ++t) {
+        int mt, nt;
+        pair_coords(tile, q.m_tiles, q.n_tiles, mt, nt);
+        const int b = t & 1;
+        const int row0 = mt * 256 + (int)rank * 128 + quarter * 32, row = row0 + lane;
+        const int col0 = nt * tile_cols;
+        if (early && row0 < p.M) {
+            if (lane == 0) tma_store_wait_read<0>();
+            __syncwarp();
+            for (int k = 0; k < 2; ++k) {
+                const int first = col0 + (which + 2 * k) * W;
+                if (first < p.N && by_tma(row0, first)) fetch_residual((seq + k) & 1, row0, first);
+            }
+        }
+        if (!__all_sync(0xffffffffu, mbar_wait(bar0 + 8u * (2 * kStages + b), (t >> 1) & 1, q.wait_limit)))
+            return leave(true);
+        tc_fence_after();
+        const uint32_t acc = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(b * 256);
+        const float row_scale = e.row_scales && row < p.M ? __ldg(e.row_scales + row) : 1.0f;
+        auto columns32 = [&](int c, float (&v)[32]) {
+            uint32_t r[32];
+            tc_ld_32x32b_x32(acc + c, r);
+            tc_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+        };
+        auto scale32 = [&](const float* scales, int col, float (&v)[32]) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+                const float4 s = __ldg(reinterpret_cast<const float4*>(scales + col + i));
+                v[i] = v[i] * row_scale * s.x;
+                v[i + 1] = v[i + 1] * row_scale * s.y;
+                v[i + 2] = v[i + 2] * row_scale * s.z;
+                v[i + 3] = v[i + 3] * row_scale * s.w;
+            }
+        };
+        // the value of 32 columns before the activation
+        auto linear32 = [&](int c, float (&v)[32]) {
+            columns32(c, v);
+            if (e.row_scales) scale32(e.col_scales[0], col0 + c, v);
+            if (e.bias) {
+                const uint4* bias = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(e.bias) +
+                                                                   (long long)(col0 + c) * (16 / G));
+#pragma unroll
+                for (int i = 0; i < 32 / G; ++i) add16<DT>(__ldg(bias + i), v + i * G);
+            }
+        };
+        auto put32 = [&](int buffer, int h, const float (&v)[32]) {
+#pragma unroll
+            for (int i = 0; i < 32 / G; ++i) slot(buffer, h * (32 / G) + i) = pack16<DT>(v + i * G);
+        };
+        auto free_buffer = [&] {  // the store before the last one has read its buffer, which is the next one's
+            if (lane == 0) tma_store_wait_read<1>();
+            __syncwarp();
+        };
+        auto send = [&](const CUtensorMap* map, int c, int r) {
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) tma_store_2d(map, mine_addr + (seq & 1) * kBuffer, c, r);
+            ++seq;
+        };
+        auto release = [&] {  // the accumulator is read: the MMA warp may start the tile after next
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(cluster_addr(bar0 + 8u * (2 * kStages + 2 + b), 0));
+        };
+        for (int c = which; c < chunks; c += 2) {
+            const int first = col0 + c * W;
+            const bool last = c + 2 >= chunks;
+            if (row0 >= p.M || first >= p.N) {
+                if (last) release();
+                continue;
+            }
+            if (by_tma(row0, first)) {
+                if (p.gated) {
+                    if (e.gate) {
+                        for (int k = 0; k < 2; ++k) {
+                            free_buffer();
+#pragma unroll
+                            for (int h = 0; h < W / 32; ++h) {
+                                float v[32];
+                                columns32(k * 128 + c * W + h * 32, v);
+                                if (e.row_scales) scale32(e.col_scales[k], first + h * 32, v);
+                                put32(seq & 1, h, v);
+                            }
+                            send(k == 0 ? &q.aside : &q.out2, first, row0);
+                        }
+                    }
+                    free_buffer();
+#pragma unroll
+                    for (int h = 0; h < W / 32; ++h) {
+                        float v[32], u[32];
+                        columns32(c * W + h * 32, v);
+                        columns32(128 + c * W + h * 32, u);
+                        if (last && h == W / 32 - 1) release();
+                        if (e.row_scales) {
+                            scale32(e.col_scales[0], first + h * 32, v);
+                            scale32(e.col_scales[1], first + h * 32, u);
+                        }
+                        activate_all<32>(e.act, v);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] *= u[i];
+                        put32(seq & 1, h, v);
+                    }
+                    send(&q.out, first, row0);
+                    continue;
+                }
+                if (e.pre) {
+                    free_buffer();
+#pragma unroll
+                    for (int h = 0; h < W / 32; ++h) {
+                        float v[32];
+                        linear32(c * W + h * 32, v);
+                        put32(seq & 1, h, v);
+                    }
+                    send(&q.aside, first, row0);
+                }
+                const int buffer = seq & 1;
+                if (e.residual) {
+                    if (!early || c >= 4) {  // not asked for above
+                        if (lane == 0) tma_store_wait_read<0>();
+                        __syncwarp();
+                        fetch_residual(buffer, row0, first);
+                    }
+                    if (!await_residual(buffer)) return leave(true);
+                } else {
+                    free_buffer();
+                }
+#pragma unroll
+                for (int h = 0; h < W / 32; ++h) {
+                    float v[32];
+                    linear32(c * W + h * 32, v);
+                    if (last && h == W / 32 - 1) release();
+                    activate_all<32>(e.act, v);
+                    if (e.residual) {
+#pragma unroll
+                        for (int i = 0; i < 32 / G; ++i) add16<DT>(slot(buffer, h * (32 / G) + i), v + i * G);
+                    }
+                    put32(buffer, h, v);
+                }
+                if (e.split_rows > 0 && row0 >= e.split_rows)
+                    send(&q.out2, first, row0 - e.split_rows - e.split_skip);
+                else if (e.split_cols > 0 && first >= e.split_cols)
+                    send(&q.out2, first - e.split_cols - e.split_skip, row0);
+                else
+                    send(&q.out, first, row0);
+                continue;
+            }
+            // Element by element: 32 columns at a time (gated: of both products), as
+            // fp32 rows of 128 bytes (the products side by side in the two buffers), read
+            // back a row at a time with a column a lane.
+            if (lane == 0) tma_store_wait_read<0>();
+            __syncwarp();
+            for (int h = 0; h < W / 32; ++h) {
+                const int col = first + h * 32 + lane;
+                for (int k = 0; k < (p.gated ? 2 : 1); ++k) {
+                    float v[32];
+                    columns32(k * 128 + c * W + h * 32, v);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) slot(k, i) = pack16<TTC_F32>(v + 4 * i);
+                }
+                if (last && h == W / 32 - 1) release();
+                __syncwarp();
+                auto at = [&](int k, int r) {
+                    return *reinterpret_cast<const float*>(mine + k * kBuffer + r * kRow +
+                                                           (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+                };
+                if (col < p.N) {
+                    const float s0 = e.row_scales ? __ldg(e.col_scales[0] + col) : 1.0f;
+                    const float s1 = e.row_scales && p.gated ? __ldg(e.col_scales[1] + col) : 1.0f;
+                    const float bias = e.bias ? load1(DT, e.bias, col) : 0.0f;
+                    const int rows = min(32, p.M - row0);
+#pragma unroll 4
+                    for (int r = 0; r < rows; ++r) {
+                        if (p.gated)
+                            finish_one_gated(e, row0 + r, col, at(0, r), at(1, r), s0, s1);
+                        else
+                            finish_one_linear(e, row0 + r, col, at(0, r), s0, bias);
+                    }
+                }
+                __syncwarp();
+            }
+        }
+    }
+    return leave(false);
+}
+
 // CTA r of a pair holds rows 128 r .. of the A tile and columns 128 r .. of the
 // B tile (gated: the gate columns for r = 0, the up columns for r = 1) and gets
 // its 128 rows x 256 columns of the result in its own tensor memory, two
 // accumulators deep, so that the epilogue of one tile runs under the next.
 //
-// Epilogue: tensor memory hands each lane one row; the rows go through shared
-// memory (16-byte chunks xored with the row, conflict-free both ways), so that
-// a warp reads the residual and writes the output in whole 128-byte lines.
+// Epilogue: tensor memory hands each lane one row. A warp takes chunks of 128
+// bytes of output (64 columns, 32 of fp32) through its two buffers in shared
+// memory, in the 128-byte swizzle, and TMA carries them: the residual into the
+// buffer before the tile is ready, the result out of it. Rows and columns past
+// the end are clipped there. (Writing the rows with the warps' own 16-byte
+// stores instead cost 15 of the 39 us of 1024 x 16384 x 512, and the address
+// arithmetic 7 more.) Chunks that TMA cannot write (unaligned tensors, the
+// seam of a split output, the last columns of a biased or scaled one) go
+// element by element, a column a lane.
 template <bool F8>
 __global__ void __launch_bounds__(kThreads, 1) pair_kernel(const __grid_constant__ ProductParams q) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint8_t* staging = smem + kStages * kStageBytes;
-    uint64_t* bars = (uint64_t*)(staging + kEpilogueWarps * kStaging);
-    uint32_t* tmem_slot = (uint32_t*)(bars + 2 * kStages + 4);
+    uint64_t* bars = (uint64_t*)(staging + kEpilogueWarps * 2 * kBuffer);
+    uint32_t* tmem_slot = (uint32_t*)(bars + 2 * kStages + 4 + 2 * kEpilogueWarps);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
     const uint32_t sbase = smem_u32(smem), bar0 = smem_u32(bars);
@@ -144,6 +431,7 @@ __global__ void __launch_bounds__(kThreads, 1) pair_kernel(const __grid_constant
     auto empty_bar = [&](int s) { return bar0 + 8u * (kStages + s); };
     auto tfull_bar = [&](int b) { return bar0 + 8u * (2 * kStages + b); };
     auto tempty_bar = [&](int b) { return bar0 + 8u * (2 * kStages + 2 + b); };
+    auto res_bar = [&](int w, int k) { return bar0 + 8u * (2 * kStages + 4 + 2 * w + k); };
     const Product& p = q.p;
 
     if (threadIdx.x == 0) {
@@ -155,6 +443,8 @@ __global__ void __launch_bounds__(kThreads, 1) pair_kernel(const __grid_constant
             mbar_init(tfull_bar(b), 1);
             mbar_init(tempty_bar(b), 2 * kEpilogueWarps);
         }
+        for (int w = 0; w < kEpilogueWarps; ++w)
+            for (int k = 0; k < 2; ++k) mbar_init(res_bar(w, k), 1);
         mbar_fence_init();
     }
     if (warp == 1) {
@@ -265,95 +555,12 @@ __global__ void __launch_bounds__(kThreads, 1) pair_kernel(const __grid_constant
             }
         }
     } else {
-        const int quarter = warp & 3, which = (warp - 2) >> 2;  // which of the quarter's two warps
-        float4* const mine = reinterpret_cast<float4*>(staging + (warp - 2) * kStaging);
-        auto chunk = [&](int row, int c) -> float4& { return mine[row * 16 + (c ^ (row & 7))]; };
-        // two 16-byte chunks from c on, in the order that keeps 8 lanes on 8 different banks
-        auto take8 = [&](int row, int c, int flip, float (&v)[8]) {
-            const float4 x = chunk(row, c + flip), y = chunk(row, c + (flip ^ 1));
-            const float4 lo = flip ? y : x, hi = flip ? x : y;
-            v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w, v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
-        };
-        const bool early = p.epi.residual && p.epi.vec && p.epi.out_dtype != TTC_F32;
-        int t = 0;
-        for (int tile = cluster_id; tile < num_tiles; tile += nclusters, ++t) {
-            int mt, nt;
-            pair_coords(tile, q.m_tiles, q.n_tiles, mt, nt);
-            const int b = t & 1;
-            const int row0 = mt * 256 + (int)rank * 128 + quarter * 32;
-            // The residual of a chunk's 8 rows a lane, asked for before the chunk is
-            // ready (the first one before the tile is): 16-bit, whole groups only.
-            uint4 res[8];
-            auto ahead = [&](int c) { return early && nt * 256 + c * 64 + 64 <= p.N; };
-            auto fetch = [&](int c) {
-                if (!ahead(c)) return;
-                const uint16_t* from = static_cast<const uint16_t*>(p.epi.residual) + nt * 256 + c * 64 + (lane & 7) * 8;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int row = row0 + i * 4 + (lane >> 3);
-                    if (row < p.M) res[i] = *reinterpret_cast<const uint4*>(from + row * p.epi.ldr);
-                }
-            };
-            fetch(which);
-            if (!__all_sync(0xffffffffu, mbar_wait(tfull_bar(b), (t >> 1) & 1, q.wait_limit))) {
-                failed = true;
-                break;
-            }
-            tc_fence_after();
-            const uint32_t acc = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(b * 256);
-#pragma unroll 1
-            for (int c = which; c < 4; c += 2) {
-                // gated: 32 outputs, 4 lanes a row, 8 rows at a time; linear: 64, 8 lanes, 4 rows
-                const int width = p.gated ? 32 : 64, first = nt * (p.gated ? 128 : 256) + c * width;
-                const int j = p.gated ? lane & 3 : lane & 7, col = first + j * 8;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t r[32];
-                    tc_ld_32x32b_x32(acc + c * width + (h == 0 ? 0 : p.gated ? 128 : 32), r);
-                    tc_wait_ld();
-#pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        chunk(lane, h * 8 + k) =
-                            make_float4(__uint_as_float(r[4 * k]), __uint_as_float(r[4 * k + 1]),
-                                        __uint_as_float(r[4 * k + 2]), __uint_as_float(r[4 * k + 3]));
-                }
-                tc_fence_before();
-                __syncwarp();
-                // read: the MMA warp may start the tile after next
-                if (c >= 2 && lane == 0) mbar_arrive_cluster(cluster_addr(tempty_bar(b), 0));
-                if (col < p.N) {
-                    const Columns cols = load_columns(p.epi, col, p.N);
-                    with_finish(p.epi, cols, p.epi.vec && first + width <= p.N, [&](const auto& finish) {
-                        if (p.gated) {
-#pragma unroll 2
-                            for (int i = 0; i < 4; ++i) {
-                                const int lr = i * 8 + (lane >> 2), row = row0 + lr;
-                                if (row >= p.M) break;
-                                float g[8], u[8];
-                                take8(lr, 2 * j, 0, g);
-                                take8(lr, 8 + 2 * j, 0, u);
-                                finish.gated(row, g, u);
-                            }
-                            return;
-                        }
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const int lr = i * 4 + (lane >> 3), row = row0 + lr;
-                            if (row >= p.M) break;
-                            float v[8], t[8];
-                            if (ahead(c))
-                                finish.unpack(res[i], t);
-                            else
-                                finish.residual(row, t);
-                            take8(lr, 2 * j, j >> 2, v);
-                            finish.linear(row, v, t);
-                        }
-                    });
-                }
-                __syncwarp();
-                if (c < 2) fetch(c + 2);
-            }
-        }
+        if (p.epi.out_dtype == TTC_BF16)
+            failed = pair_epilogue<TTC_BF16>(q, staging, tmem_base, bar0, rank);
+        else if (p.epi.out_dtype == TTC_F16)
+            failed = pair_epilogue<TTC_F16>(q, staging, tmem_base, bar0, rank);
+        else
+            failed = pair_epilogue<TTC_F32>(q, staging, tmem_base, bar0, rank);
     }
 
     if (failed) *(volatile int*)q.status = 1;
@@ -606,6 +813,31 @@ int make_map(CUtensorMap* map, const Product& p, const Operand& o, int width, bo
     return encode_tensor_map(map, type, es, o.ptr, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// The pair kernel's output side: boxes of 32 rows x 128 bytes.
+int make_output_maps(ProductParams& q) {
+    const Product& p = q.p;
+    const ProductEpilogue& e = p.epi;
+    const int es = dtype_size(e.out_dtype);
+    auto map = [&](CUtensorMap* m, const void* ptr, long long ld, int rows, int cols) -> int {
+        const unsigned long long dims[2] = {(unsigned long long)cols, (unsigned long long)rows};
+        const unsigned long long strides[1] = {(unsigned long long)ld};
+        const unsigned box[2] = {(unsigned)(kRow / es), 32};
+        return encode_tensor_map(m, es == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, es, ptr,
+                                 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    };
+    const int rows = e.split_rows ? e.split_rows : p.M, cols = e.split_cols ? e.split_cols : p.N;
+    if (int rc = map(&q.out, e.out, e.ldo, rows, cols)) return rc;
+    if (e.out2)
+        if (int rc = map(&q.out2, e.out2, e.ldo, rows, cols)) return rc;
+    if (e.gate) {
+        if (int rc = map(&q.aside, e.gate, e.ldp, p.M, p.N)) return rc;
+        if (int rc = map(&q.out2, e.up, e.ldp, p.M, p.N)) return rc;
+    }
+    if (e.pre)
+        if (int rc = map(&q.aside, e.pre, e.ldp, p.M, p.N)) return rc;
+    return e.residual ? map(&q.residual, e.residual, e.ldr, p.M, p.N) : TTC_OK;
+}
+
 unsigned instruction(const Product& p, bool a_mn, bool b_mn, int m, int n) {
     const unsigned fmt = p.dtype == TTC_BF16 ? 1u : 0u;  // kind::f16: f16 0, bf16 1; kind::f8f6f4: e4m3 0
     return (1u << 4) | (fmt << 7) | (fmt << 10) | ((unsigned)a_mn << 15) | ((unsigned)b_mn << 16) |
@@ -723,6 +955,8 @@ int run_product(const Product& given, void* scratch) {
             if (int rc = make_map(&q.a[i], p, p.a[i], p.M, p.a_mn, 128)) return rc;
         for (int i = 0; i < nb; ++i)
             if (int rc = make_map(&q.b[i], p, p.b[i], p.N, p.b_mn, 128)) return rc;
+        if (p.epi.vec)
+            if (int rc = make_output_maps(q)) return rc;
         return f8 ? launch_pair<true>(q) : launch_pair<false>(q);
     }
 
