@@ -526,6 +526,49 @@ def test_gated_linear_backward(lib, M, N, K, dtype, trans_w, form):
     assert dx.untouched_outside()
 
 
+@pytest.mark.parametrize("M,N,K", [(5, 132, 72), (40, 129, 200), (33, 1001, 136), (600, 132, 4104), (2048, 2052, 2056), (700, 2049, 3000)])
+@pytest.mark.parametrize("trans_w", [False, True])
+def test_widths_that_end_inside_an_aligned_row(lib, M, N, K, trans_w):
+    """Rows padded to 16 bytes around widths that are no multiple of 8: everything
+    is aligned, and still nothing past the last column may be written, nor
+    anything of one weight's gradient into the other's."""
+    g = gen(N)
+    pad = lambda n: -n % 8 + 8  # noqa: E731
+    x = Mat(M, K, "bf16", pad(K), 8, rand(g, M, K))
+    shape = (N, K) if trans_w else (K, N)
+    wg, wu = (Mat(*shape, "bf16", pad(shape[1]), 8, rand(g, *shape, K ** -0.5)) for _ in range(2))
+    gate, up, y, dy, bias, res = (Mat(M if i < 4 or i == 5 else 1, N, "bf16", pad(N), 8, rand(g, M if i < 4 or i == 5 else 1, N))
+                                  for i in range(6))
+    dx = Mat(M, K, "bf16", pad(K), 8)
+    dwg, dwu = (Mat(*shape, "bf16", pad(shape[1]), 8) for _ in range(2))
+    z = Mat(M, N, "bf16", pad(N), 8)
+    d = lib.linear_desc(M, N, K, x.ptr, x.ld, wg.ptr, wg.ld, z.ptr, z.ld, lib.BF16, trans_w=trans_w, bias=bias.ptr,
+                        residual=res.ptr, ldr=res.ld)
+    lib.linear(d, scratch(lib, d))
+    wgv, wuv = (w.f64().t() if trans_w else w.f64() for w in (wg, wu))
+    want, acc = product64(x.f64(), wgv)
+    want = want + bias.f64() + res.f64()
+    within(z.t, want, (U["bf16"] + 2.0 ** -22) * (want.abs() + bias.f64().abs() + res.f64().abs()) + acc, "linear")
+    d = lib.gated_linear_desc(M, N, K, x.ptr, x.ld, wg.ptr, wu.ptr, wg.ld, y.ptr, y.ld, lib.BF16, trans_w=trans_w,
+                              gate=gate.ptr, up=up.ptr, ldp=gate.ld)
+    lib.gated_linear(d, scratch(lib, d))
+    zg, ag = product64(x.f64(), wgv)
+    zu, au = product64(x.f64(), wuv)
+    within(gate.t, zg, U["bf16"] * zg.abs() + ag, "gate")
+    within(up.t, zu, U["bf16"] * zu.abs() + au, "up")
+    d = lib.gated_linear_backward_desc(M, N, K, dy.ptr, dy.ld, x.ptr, x.ld, wg.ptr, wu.ptr, wg.ld, gate.ptr, up.ptr,
+                                       gate.ld, lib.BF16, trans_w=trans_w, dx=dx.ptr, lddx=dx.ld, dwg=dwg.ptr,
+                                       dwu=dwu.ptr, lddw=dwg.ld)
+    lib.gated_linear_backward(d, scratch(lib, d))
+    a, s = act64("silu", gate.f64())
+    dg, du = dy.f64() * up.f64() * s, dy.f64() * a
+    normwise(dx.t, dg @ wgv.t() + du @ wuv.t(), "bf16", "dx", (dg, wgv.t()), (du, wuv.t()))
+    for got, v in ((dwg, dg), (dwu, du)):
+        normwise(got.t if trans_w else got.t.t(), v.t() @ x.f64(), "bf16", "dw", (v.t(), x.f64()))
+    for m in (z, y, gate, up, dx, dwg, dwu):
+        assert m.untouched_outside()
+
+
 def test_activation_slopes_at_far_values(lib):
     """dz = dy act'(pre) where exponentials overflow and z^2 exceeds fp32: with
     one output column and w = 1, dx is dz itself."""

@@ -218,31 +218,6 @@ __device__ __forceinline__ void store8(T* p, int n, bool vec, const float (&v)[8
     }
 }
 
-// The same for a type known to the compiler (DT >= 0) or chosen at run time, one
-// branch per 8 elements. FULL: all eight, vector accesses.
-template <int DT, bool FULL>
-__device__ __forceinline__ void load8_as(int dtype, const void* base, long long i, int n, bool vec, float (&v)[8]) {
-    const int d = DT >= 0 ? DT : dtype;
-    const int m = FULL ? 8 : n;
-    if (d == TTC_BF16)
-        load8(static_cast<const __nv_bfloat16*>(base) + i, m, FULL || vec, v);
-    else if (d == TTC_F16)
-        load8(static_cast<const __half*>(base) + i, m, FULL || vec, v);
-    else
-        load8(static_cast<const float*>(base) + i, m, FULL || vec, v);
-}
-template <int DT, bool FULL>
-__device__ __forceinline__ void store8_as(int dtype, void* base, long long i, int n, bool vec, const float (&v)[8]) {
-    const int d = DT >= 0 ? DT : dtype;
-    const int m = FULL ? 8 : n;
-    if (d == TTC_BF16)
-        store8(static_cast<__nv_bfloat16*>(base) + i, m, FULL || vec, v);
-    else if (d == TTC_F16)
-        store8(static_cast<__half*>(base) + i, m, FULL || vec, v);
-    else
-        store8(static_cast<float*>(base) + i, m, FULL || vec, v);
-}
-
 // Activations in fp32, with the hardware's approximate 2^x and 1 / x (good to
 // 2^-22; 2^x takes the rounding of its argument besides), far below the 2^-8
 // .. 2^-11 of the types the results are rounded to; an fp32 result of the
@@ -336,97 +311,6 @@ __device__ __forceinline__ void activate_grad(int act, float z, float& a, float&
     }
 }
 
-// What eight consecutive columns (from col < N on) have in common over all rows.
-struct Columns {
-    int col, n;  // n of the eight are inside
-    float scale[2][8];
-    float bias[8];
-};
-__device__ __forceinline__ Columns load_columns(const ProductEpilogue& e, int col, int N) {
-    Columns c;
-    c.col = col;
-    c.n = N - col < 8 ? N - col : 8;
-    if (e.row_scales) {
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-            if (e.col_scales[s]) load8(e.col_scales[s] + col, c.n, e.vec, c.scale[s]);
-    }
-    if (e.bias) load8_as<-1, false>(e.out_dtype, e.bias, col, c.n, e.vec, c.bias);
-    return c;
-}
-
-// The rest of the epilogue for one row of such columns. FULL (all eight inside,
-// e.vec) and the type DT are known to the compiler on the path that matters: the
-// general form, with its predicated single elements, ran 24 instructions a value.
-template <int DT, bool FULL>
-struct Finish {
-    const ProductEpilogue& e;
-    const Columns& c;
-    __device__ __forceinline__ void load(const void* base, long long i, float (&v)[8]) const {
-        load8_as<DT, FULL>(e.out_dtype, base, i, c.n, e.vec, v);
-    }
-    __device__ __forceinline__ void store(void* base, long long i, int n, const float (&v)[8]) const {
-        store8_as<DT, FULL>(e.out_dtype, base, i, n, e.vec, v);
-    }
-    // The residual of a row; issued ahead of the row's values.
-    __device__ __forceinline__ void residual(int row, float (&t)[8]) const {
-        if (e.residual) load(e.residual, row * e.ldr + c.col, t);
-    }
-    // v holds the product, res what residual() gave.
-    __device__ __forceinline__ void linear(int row, float (&v)[8], const float (&res)[8]) const {
-        int n = c.n;
-        if (e.row_scales) {
-            const float rs = __ldg(e.row_scales + row);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = v[i] * rs * c.scale[0][i];
-        }
-        if (e.bias) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] += c.bias[i];
-        }
-        if (e.pre) store(e.pre, row * e.ldp + c.col, n, v);
-        activate_all<8>(e.act, v);
-        if (e.residual) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] += res[i];
-        }
-        void* out = e.out;
-        int r = row, k = c.col;
-        if (e.split_rows > 0 && row >= e.split_rows) {
-            r -= e.split_rows + e.split_skip;
-            if (r < 0) return;
-            out = e.out2;
-        } else if (e.split_cols > 0) {  // split_cols + split_skip is a multiple of 8: no group straddles it
-            if (k >= e.split_cols + e.split_skip) {
-                out = e.out2;
-                k -= e.split_cols + e.split_skip;
-            } else if (!FULL && k + n > e.split_cols) {
-                n = e.split_cols - k;
-            }
-        }
-        store(out, r * e.ldo + k, n, v);
-    }
-    // The same columns of the two products of a gated pair.
-    __device__ __forceinline__ void gated(int row, float (&g)[8], float (&u)[8]) const {
-        if (e.row_scales) {
-            const float rs = __ldg(e.row_scales + row);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                g[i] = g[i] * rs * c.scale[0][i];
-                u[i] = u[i] * rs * c.scale[1][i];
-            }
-        }
-        if (e.gate) {
-            store(e.gate, row * e.ldp + c.col, c.n, g);
-            store(e.up, row * e.ldp + c.col, c.n, u);
-        }
-        activate_all<8>(e.act, g);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) g[i] *= u[i];
-        store(e.out, row * e.ldo + c.col, c.n, g);
-    }
-};
-
 // The epilogue of single elements, for tensors that nothing wider can reach:
 // element (row, col) of a product, with its column's scales and bias.
 __device__ __forceinline__ float load1(int dtype, const void* base, long long i) {
@@ -475,18 +359,6 @@ __device__ __forceinline__ void finish_one_gated(const ProductEpilogue& e, int r
     store1(e.out_dtype, e.out, row * e.ldo + col, activate(e.act, g) * u);
 }
 
-// f(Finish) for the columns c; `full` is the same for the whole warp.
-template <class F>
-__device__ __forceinline__ void with_finish(const ProductEpilogue& e, const Columns& c, bool full, F&& f) {
-    if (!full)
-        f(Finish<-1, false>{e, c});
-    else if (e.out_dtype == TTC_BF16)
-        f(Finish<TTC_BF16, true>{e, c});
-    else if (e.out_dtype == TTC_F16)
-        f(Finish<TTC_F16, true>{e, c});
-    else
-        f(Finish<TTC_F32, true>{e, c});
-}
 #endif  // __CUDACC__
 
 }  // namespace ttc

@@ -28,6 +28,7 @@
 // holds and returns. No TMA load is multicast.
 #include <algorithm>
 #include <cstring>
+#include <type_traits>
 
 #include "ffn.cuh"
 #include "tc_util.cuh"
@@ -186,9 +187,10 @@ __device__ __forceinline__ bool pair_epilogue(const ProductParams& q, uint8_t* s
         return *reinterpret_cast<uint4*>(mine + buffer * kBuffer + lane * kRow + ((i ^ (lane & 7)) << 4));
     };
     // TMA writes the chunk of columns from `first` on: aligned tensors, one output
-    // tensor, and per-column operands that do not end inside it.
+    // tensor, no per-column operand and no 16-byte group that ends inside it (a
+    // store that is clipped inside a group writes the whole group).
     auto by_tma = [&](int row0, int first) {
-        if (!e.vec || ((e.bias || e.row_scales) && first + W > p.N)) return false;
+        if (!e.vec || (first + W > p.N && (e.bias || e.row_scales || p.N % G))) return false;
         if (e.split_rows > 0) return row0 + 32 <= e.split_rows || row0 >= e.split_rows + e.split_skip;
         if (e.split_cols > 0) return first + W <= e.split_cols || first >= e.split_cols + e.split_skip;
         return true;
@@ -415,8 +417,8 @@ __device__ __forceinline__ bool pair_epilogue(const ProductParams& q, uint8_t* s
 // the end are clipped there. (Writing the rows with the warps' own 16-byte
 // stores instead cost 15 of the 39 us of 1024 x 16384 x 512, and the address
 // arithmetic 7 more.) Chunks that TMA cannot write (unaligned tensors, the
-// seam of a split output, the last columns of a biased or scaled one) go
-// element by element, a column a lane.
+// seam of a split output, the last columns of a biased or scaled one or of a
+// width that is no multiple of 16 bytes) go element by element, a column a lane.
 template <bool F8>
 __global__ void __launch_bounds__(kThreads, 1) pair_kernel(const __grid_constant__ ProductParams q) {
     extern __shared__ uint8_t smem_raw[];
@@ -577,8 +579,8 @@ __global__ void __launch_bounds__(kThreads, 1) pair_kernel(const __grid_constant
 // first half and their up columns in the second) against `tok` rows of x, over
 // its share of the k-blocks. The accumulator's lanes are output columns and its
 // columns rows of x; it goes to shared memory as [row of x][128] over the ring,
-// where the CTAs of the cluster add up each other's shares in rank order, a
-// contiguous share of the outputs each.
+// where the CTAs of the cluster add up each other's shares in rank order, some of
+// the rows each.
 __device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
     float4 v;
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
@@ -586,6 +588,158 @@ __device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
                  : "r"(addr)
                  : "memory");
     return v;
+}
+
+// Four values at float index i of the tile, added over the cluster's CTAs in rank order.
+__device__ __forceinline__ float4 tile_sum4(uint32_t sbase, int splits, int i) {
+    float4 t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const uint32_t at = sbase + 4u * (uint32_t)i;
+    if (splits == 1) {
+        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(t.x), "=f"(t.y), "=f"(t.z), "=f"(t.w)
+                     : "r"(at));
+        return t;
+    }
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) {
+        const float4 v = ld_cluster(cluster_addr(at, s));
+        t.x += v.x, t.y += v.y, t.z += v.z, t.w += v.w;
+    }
+    return t;
+}
+
+// Four consecutive elements of DT, 8 or 16 bytes.
+template <int DT>
+struct Four {
+    using Raw = typename std::conditional<DT == TTC_F32, uint4, uint2>::type;
+    static constexpr int kSize = DT == TTC_F32 ? 4 : 2;
+    static __device__ __forceinline__ Raw* at(const void* base, long long i) {
+        return reinterpret_cast<Raw*>(static_cast<char*>(const_cast<void*>(base)) + i * kSize);
+    }
+    static __device__ __forceinline__ float4 load(const void* base, long long i) {
+        const Raw r = *at(base, i);
+        if constexpr (DT == TTC_F32) {
+            return make_float4(__uint_as_float(r.x), __uint_as_float(r.y), __uint_as_float(r.z), __uint_as_float(r.w));
+        } else {
+            using T = typename std::conditional<DT == TTC_BF16, __nv_bfloat16, __half>::type;
+            const T *a = reinterpret_cast<const T*>(&r.x), *b = reinterpret_cast<const T*>(&r.y);
+            return make_float4(to_f32(a[0]), to_f32(a[1]), to_f32(b[0]), to_f32(b[1]));
+        }
+    }
+    static __device__ __forceinline__ void store(void* base, long long i, const float (&v)[4]) {
+        if constexpr (DT == TTC_F32) {
+            *at(base, i) = pack16<TTC_F32>(v);
+        } else {
+            using T = typename std::conditional<DT == TTC_BF16, __nv_bfloat16, __half>::type;
+            *at(base, i) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+        }
+    }
+};
+
+// Rows [r0, r1) of the tile's result, a lane four columns: a warp reads a row of
+// the tile (gated: two half rows) with one 512-byte access from each CTA of the
+// cluster and writes it with one, four rows on their way at a time. Eight columns
+// a thread with every choice made per row took 9 of the 22 us of 256 x 4096 x 4096.
+template <int DT, bool GATED>
+__device__ __forceinline__ void tile_finish(const ProductParams& q, uint32_t sbase, int m0, int n0, int r0, int r1) {
+    const ProductEpilogue& e = q.p.epi;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int j = GATED ? lane & 15 : lane, col = n0 + 4 * j;
+    constexpr int kStep = (GATED ? 2 : 1) * kThreads / 32;  // rows of all warps
+    constexpr int kAhead = 4;
+    float4 s0 = make_float4(1, 1, 1, 1), s1 = s0, bias = make_float4(0, 0, 0, 0);
+    if (e.row_scales) {
+        s0 = __ldg(reinterpret_cast<const float4*>(e.col_scales[0] + col));
+        if (GATED) s1 = __ldg(reinterpret_cast<const float4*>(e.col_scales[1] + col));
+    }
+    if (e.bias) bias = Four<DT>::load(e.bias, col);
+    for (int r = r0 + (GATED ? 2 * warp + (lane >> 4) : warp); r < r1; r += kAhead * kStep) {
+        float v[kAhead][4], u[kAhead][4];
+        auto each = [&](auto f) {
+#pragma unroll
+            for (int a = 0; a < kAhead; ++a)
+                if (r + a * kStep < r1) f(a, m0 + r + a * kStep);
+        };
+        auto get = [](float (&to)[4], const float4& x) { to[0] = x.x, to[1] = x.y, to[2] = x.z, to[3] = x.w; };
+        if (!GATED && e.residual)
+            each([&](int a, int row) { get(u[a], Four<DT>::load(e.residual, row * e.ldr + col)); });
+        each([&](int a, int row) { get(v[a], tile_sum4(sbase, q.splits, (row - m0) * 128 + 4 * j)); });
+        if (GATED) each([&](int a, int row) { get(u[a], tile_sum4(sbase, q.splits, (row - m0) * 128 + 64 + 4 * j)); });
+        if (e.row_scales)
+            each([&](int a, int row) {
+                const float rs = __ldg(e.row_scales + row);
+                v[a][0] *= rs * s0.x, v[a][1] *= rs * s0.y, v[a][2] *= rs * s0.z, v[a][3] *= rs * s0.w;
+                if (GATED) u[a][0] *= rs * s1.x, u[a][1] *= rs * s1.y, u[a][2] *= rs * s1.z, u[a][3] *= rs * s1.w;
+            });
+        if (GATED) {
+            if (e.gate)
+                each([&](int a, int row) {
+                    Four<DT>::store(e.gate, row * e.ldp + col, v[a]);
+                    Four<DT>::store(e.up, row * e.ldp + col, u[a]);
+                });
+        } else {
+            if (e.bias)
+                each([&](int a, int) { v[a][0] += bias.x, v[a][1] += bias.y, v[a][2] += bias.z, v[a][3] += bias.w; });
+            if (e.pre) each([&](int a, int row) { Four<DT>::store(e.pre, row * e.ldp + col, v[a]); });
+        }
+        if (e.act != TTC_ACT_NONE) {
+            float all[4 * kAhead];
+#pragma unroll
+            for (int i = 0; i < 4 * kAhead; ++i) all[i] = v[i / 4][i % 4];
+            activate_all<4 * kAhead>(e.act, all);
+#pragma unroll
+            for (int i = 0; i < 4 * kAhead; ++i) v[i / 4][i % 4] = all[i];
+        }
+        if (GATED)
+            each([&](int a, int) { v[a][0] *= u[a][0], v[a][1] *= u[a][1], v[a][2] *= u[a][2], v[a][3] *= u[a][3]; });
+        else if (e.residual)
+            each([&](int a, int) { v[a][0] += u[a][0], v[a][1] += u[a][1], v[a][2] += u[a][2], v[a][3] += u[a][3]; });
+        each([&](int a, int row) {
+            void* out = e.out;
+            int k = col;
+            if (!GATED && e.split_rows > 0 && row >= e.split_rows) {
+                row -= e.split_rows + e.split_skip;
+                if (row < 0) return;
+                out = e.out2;
+            } else if (!GATED && e.split_cols > 0 && col >= e.split_cols) {  // the seam is in no tile that comes here
+                k -= e.split_cols + e.split_skip;
+                out = e.out2;
+            }
+            Four<DT>::store(out, row * e.ldo + k, v[a]);
+        });
+    }
+}
+
+// The same for unaligned tensors and the last columns: a lane one column at a time.
+__device__ __noinline__ void tile_finish_scalar(const ProductParams& q, uint32_t sbase, int m0, int n0, int r0, int r1) {
+    const Product& p = q.p;
+    const ProductEpilogue& e = p.epi;
+    const int width = p.gated ? 64 : 128;
+    auto sum1 = [&](int i) {
+        float t = 0.0f;
+        for (int s = 0; s < q.splits; ++s) {
+            float v;
+            const uint32_t at = sbase + 4u * (uint32_t)i;
+            asm volatile("ld.shared::cluster.f32 %0, [%1];"
+                         : "=f"(v)
+                         : "r"(q.splits == 1 ? at : cluster_addr(at, s))
+                         : "memory");
+            t += v;
+        }
+        return t;
+    };
+    // kThreads is a multiple of neither width, so columns change from row to row
+#pragma unroll 2
+    for (int it = threadIdx.x; it < (r1 - r0) * width; it += kThreads) {
+        const int r = r0 + it / width, c = it % width, col = n0 + c, row = m0 + r;
+        if (col >= p.N) continue;
+        const float s0 = e.row_scales ? __ldg(e.col_scales[0] + col) : 1.0f;
+        if (p.gated)
+            finish_one_gated(e, row, col, sum1(r * 128 + c), sum1(r * 128 + 64 + c), s0,
+                             e.row_scales ? __ldg(e.col_scales[1] + col) : 1.0f);
+        else
+            finish_one_linear(e, row, col, sum1(r * 128 + c), s0, e.bias ? load1(e.out_dtype, e.bias, col) : 0.0f);
+    }
 }
 
 template <bool F8>
@@ -695,7 +849,7 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ 
         }
     }
     const int rows = min(q.tok, p.M - m0);
-    float* const part = reinterpret_cast<float*>(smem);
+    float* const part = reinterpret_cast<float*>(smem);  // [row of x][128] over the ring
     if (warp >= 2) {
         const int quarter = warp & 3;
         if (__all_sync(0xffffffffu, mbar_wait(done_bar, 0, q.wait_limit))) {
@@ -722,48 +876,20 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ 
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(tmem_cols)
                      : "memory");
 
-    const int groups = p.gated ? 8 : 16;  // of 8 columns
-    const int items = rows * groups, share = (items + splits - 1) / splits;
-    const int last = min(items, (split + 1) * share);
-    // 8 consecutive values of a row, added over the cluster's CTAs in rank order
-    auto take8 = [&](int row, int col, float (&v)[8]) {
-        if (splits == 1) {
-            const float4 lo = *reinterpret_cast<const float4*>(part + row * 128 + col);
-            const float4 hi = *reinterpret_cast<const float4*>(part + row * 128 + col + 4);
-            v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w, v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
-            return;
-        }
-        const uint32_t at = sbase + (uint32_t)(row * 128 + col) * 4u;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-#pragma unroll 4
-        for (int s = 0; s < splits; ++s) {
-            const uint32_t a = cluster_addr(at, s);
-            const float4 lo = ld_cluster(a), hi = ld_cluster(a + 16);
-            v[0] += lo.x, v[1] += lo.y, v[2] += lo.z, v[3] += lo.w, v[4] += hi.x, v[5] += hi.y, v[6] += hi.z, v[7] += hi.w;
-        }
-    };
-    // kThreads is a multiple of 16: a thread has the same columns in every item
-    const int j = (split * share + threadIdx.x) % groups, col = n0 + j * 8;
-    if (col < p.N) {
-        const Columns cols = load_columns(p.epi, col, p.N);
-        with_finish(p.epi, cols, p.epi.vec && n0 + (p.gated ? 64 : 128) <= p.N, [&](const auto& finish) {
-#pragma unroll 2
-            for (int it = split * share + threadIdx.x; it < last; it += kThreads) {
-                const int row = it / groups;
-                float v[8], u[8];
-                if (p.gated) {
-                    take8(row, j * 8, v);
-                    take8(row, 64 + j * 8, u);
-                    finish.gated(m0 + row, v, u);
-                } else {
-                    finish.residual(m0 + row, u);
-                    take8(row, j * 8, v);
-                    finish.linear(m0 + row, v, u);
-                }
-            }
-        });
-    }
+    const int share = (rows + splits - 1) / splits;  // rows that this CTA finishes
+    const int r0 = split * share, r1 = min(rows, r0 + share);
+    const bool seam = p.epi.split_cols > 0 && n0 < p.epi.split_cols + p.epi.split_skip && n0 + 128 > p.epi.split_cols;
+    if (!p.epi.vec || seam || n0 + (p.gated ? 64 : 128) > p.N)
+        tile_finish_scalar(q, sbase, m0, n0, r0, r1);
+    else if (p.epi.out_dtype == TTC_BF16)
+        p.gated ? tile_finish<TTC_BF16, true>(q, sbase, m0, n0, r0, r1)
+                : tile_finish<TTC_BF16, false>(q, sbase, m0, n0, r0, r1);
+    else if (p.epi.out_dtype == TTC_F16)
+        p.gated ? tile_finish<TTC_F16, true>(q, sbase, m0, n0, r0, r1)
+                : tile_finish<TTC_F16, false>(q, sbase, m0, n0, r0, r1);
+    else
+        p.gated ? tile_finish<TTC_F32, true>(q, sbase, m0, n0, r0, r1)
+                : tile_finish<TTC_F32, false>(q, sbase, m0, n0, r0, r1);
     if (splits > 1) {  // nobody leaves while its shared memory is still read
         __syncwarp();
         cluster_sync();
@@ -944,10 +1070,40 @@ int run_product(const Product& given, void* scratch) {
     q.wait_limit = q.stall ? kStallTestLimitCycles : kWaitLimitCycles;
     const int nb = p.gated ? 2 : p.segs;
 
+    // tile_kernel's shape. Rows a tile: all of x up to 256; fewer where even eight
+    // CTAs a tile would leave SMs idle (256 x 1024 x 512: 18.3 us with 8 tiles of
+    // 256 rows, 6.2 with 64 tiles of 32). CTAs a tile: until the SMs have one
+    // each, and two each for few rows, whose CTAs spend their time waiting for the
+    // weight (1 x 4096 x 16384: 24.2 us with 256 CTAs, 28.0 with 128; 64 x 4096 x
+    // 4096: 13.1 us with 128, 15.8 with 256), while every share has at least
+    // four k-blocks (two for a few rows, where joining the shares is quick).
+    const int unit = p.a_mn ? 64 : 16, width = p.gated ? 64 : 128;
+    const int least = p.M <= 16 ? 2 : 4;
+    q.n_tiles = (p.N + width - 1) / width;
+    int most_splits = 1;
+    while (most_splits < 8 && q.kb_total >= 2 * most_splits * least) most_splits *= 2;
+    q.tok = std::min(256, (p.M + unit - 1) / unit * unit);
+    auto tiles = [&] { return ((long long)p.M + q.tok - 1) / q.tok * q.n_tiles; };
+    while (q.tok > std::max(32, unit) && tiles() * most_splits < sms) q.tok = (q.tok / 2 + unit - 1) / unit * unit;
+    q.splits = 1;
+    while (q.splits < most_splits && tiles() * q.splits * 2 <= (q.tok <= 32 ? 2 * sms : sms)) q.splits *= 2;
+
+    // Which kernel: the shorter estimate, from k-blocks times their measured cost
+    // (0.35 us for a pair's 256 x 256, up to 0.42 us for a tile's 128 x 256, both
+    // 128 bytes deep) and what starting and ending takes (6 us, and 4 to 9 us with
+    // the rows of the tile). Measured,
+    // pair / tile, in bf16: 256 x 4096 x 4096 28.4 / 18.9 us, 512 rows 28.4 / 24.8,
+    // 768 rows 30.2 / 33.8, 1024 rows 29.5 / 34.4; 128 x 16384 x 4096 33.8 / 31.4,
+    // 256 rows 34.6 / 41.4; 512 x 2048 x 16384 89.7 / 37.0; 2048^3 18.8 / 22.6.
     const int pair_width = p.gated ? 128 : 256;
     const long long pair_m = ((long long)p.M + 255) / 256, pair_n = ((long long)p.N + pair_width - 1) / pair_width;
-    if (pair_m * pair_n > INT32_MAX / 2) return set_error(TTC_ERR_UNSUPPORTED, "tt_cuda: too many output tiles");
-    if (p.M > 256 && pair_m * pair_n >= sms / 2) {
+    if (pair_m * pair_n > INT32_MAX / 2 || tiles() * q.splits > INT32_MAX / 2)
+        return set_error(TTC_ERR_UNSUPPORTED, "tt_cuda: too many output tiles");
+    auto rounds = [](long long n, long long at_once) { return (double)((n + at_once - 1) / at_once); };
+    const double pair_us = 6.0 + 0.35 * q.kb_total * rounds(pair_m * pair_n, sms / 2);
+    const double tile_us = 3.5 + 5.5 * q.tok / 256 + 0.42 * (128 + q.tok) / 384 * rounds(q.kb_total, q.splits) *
+                                                         rounds(tiles() * q.splits, sms);
+    if (pair_us < tile_us) {
         q.m_tiles = (int)pair_m;
         q.n_tiles = (int)pair_n;
         q.idesc = instruction(p, p.a_mn, p.b_mn, 256, 256);
@@ -960,29 +1116,13 @@ int run_product(const Product& given, void* scratch) {
         return f8 ? launch_pair<true>(q) : launch_pair<false>(q);
     }
 
-    // Rows a tile: all of x up to 256; fewer where even eight CTAs a tile would
-    // leave SMs idle (256 x 1024 x 512: 18.3 us with 8 tiles of 256 rows, 6.2
-    // with 64 tiles of 32). CTAs a tile: until the SMs have one each, and two
-    // each for few rows, whose CTAs spend their time waiting for the weight
-    // (1 x 4096 x 16384: 24.2 us with 256 CTAs, 28.0 with 128; 64 x 4096 x
-    // 4096: 13.1 us with 128, 15.8 with 256), while every share has at least
-    // four k-blocks (two for a few rows, where joining the shares is quick).
-    const int unit = p.a_mn ? 64 : 16, width = p.gated ? 64 : 128;
-    const int least = p.M <= 16 ? 2 : 4;
-    q.n_tiles = (p.N + width - 1) / width;
-    int most_splits = 1;
-    while (most_splits < 8 && q.kb_total >= 2 * most_splits * least) most_splits *= 2;
-    q.tok = std::min(256, (p.M + unit - 1) / unit * unit);
-    auto tiles = [&] { return ((long long)p.M + q.tok - 1) / q.tok * q.n_tiles; };
-    while (q.tok > std::max(32, unit) && tiles() * most_splits < sms) q.tok = (q.tok / 2 + unit - 1) / unit * unit;
     q.m_tiles = (p.M + q.tok - 1) / q.tok;
-    q.splits = 1;
-    while (q.splits < most_splits && tiles() * q.splits * 2 <= (q.tok <= 32 ? 2 * sms : sms)) q.splits *= 2;
-    // The ring: half an SM's shared memory where that holds three stages, so
-    // that one CTA's loads run under the other's start and end (4 x 16384 x
-    // 4096 gated: 45 us, 51 with the whole of it).
+    // The ring: half an SM's shared memory where two CTAs meet on an SM and that
+    // holds three stages, so that one's loads run under the other's start and end
+    // (4 x 16384 x 4096 gated: 45 us, 51 with the whole of it); else most of it.
     const int stage_bytes = kHalf + q.tok * kRow;
-    q.stages = (3 * stage_bytes <= 104 * 1024 ? 104 * 1024 : 200 * 1024) / stage_bytes;
+    const bool two = tiles() * q.splits > sms && 3 * stage_bytes <= 104 * 1024;
+    q.stages = std::min(12, (two ? 104 * 1024 : 200 * 1024) / stage_bytes);
     q.idesc = instruction(p, p.b_mn, p.a_mn, 128, q.tok);
     for (int i = 0; i < p.segs; ++i)
         if (int rc = make_map(&q.a[i], p, p.a[i], p.M, p.a_mn, q.tok)) return rc;
