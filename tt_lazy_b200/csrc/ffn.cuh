@@ -60,7 +60,7 @@ inline bool vec8_ok(const void* p, int dtype, long long ld) {
 
 int check_workspace(const char* op, const void* ws, size_t have, size_t need);
 // out[c] = sum over b < n of partials[b][c], in a fixed order, stored as dtype.
-int launch_sum_partials(const float* partials, int n, int cols, void* out, int dtype, cudaStream_t st);
+int launch_sum_partials(const float* partials, int n, int cols, void* out, int dtype);
 
 // ------------------------------------------------------------------ products
 // One product C [M, N] = sum over `segs` segments of A_s [M, K] B_s [K, N], or
@@ -118,6 +118,19 @@ inline int launch_attributes(cudaLaunchAttribute (&attr)[2], int cluster) {
 }
 
 #ifdef __CUDACC__
+
+// Launches a kernel without clusters that way, on the library stream.
+template <class... Params, class... Args>
+int launch_overlapped(void (*kernel)(Params...), dim3 grid, int block, const Args&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)block);
+    cfg.stream = rt().stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = launch_attributes(attr, 1);
+    return check_cuda(cudaLaunchKernelEx(&cfg, kernel, args...), "kernel launch");
+}
 
 // Waits until the kernels before this one in the stream have finished and their
 // writes are visible; lets the kernel after this one start to be launched.

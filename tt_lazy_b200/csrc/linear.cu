@@ -145,6 +145,8 @@ __global__ void __launch_bounds__(32 * kBandWarps) linear_grad_kernel(const __gr
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int col = blockIdx.y * kStripe + lane * 8, n = p.N - col;
     float sum[8] = {};
+    grid_wait();
+    grid_trigger();
     if (n > 0) {
         const long long r1 = min((long long)p.M, (blockIdx.x + 1ll) * p.band_rows);
         for (long long r = (long long)blockIdx.x * p.band_rows + warp; r < r1; r += kBandWarps) {
@@ -191,6 +193,8 @@ template <class T, int ACT>
 __global__ void __launch_bounds__(32 * kBandWarps) gated_grad_kernel(const __grid_constant__ GatedGradParams p) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int col = blockIdx.y * kStripe + lane * 8, n = p.N - col;
+    grid_wait();
+    grid_trigger();
     if (n <= 0) return;
     const long long r1 = min((long long)p.M, (blockIdx.x + 1ll) * p.band_rows);
     for (long long r = (long long)blockIdx.x * p.band_rows + warp; r < r1; r += kBandWarps) {
@@ -212,13 +216,13 @@ __global__ void __launch_bounds__(32 * kBandWarps) gated_grad_kernel(const __gri
 
 // f(the activation as a compile-time constant)
 template <class F>
-void with_activation(int act, F&& f) {
+int with_activation(int act, F&& f) {
     switch (act) {
-        case TTC_ACT_RELU: f(std::integral_constant<int, TTC_ACT_RELU>()); break;
-        case TTC_ACT_SILU: f(std::integral_constant<int, TTC_ACT_SILU>()); break;
-        case TTC_ACT_GELU: f(std::integral_constant<int, TTC_ACT_GELU>()); break;
-        case TTC_ACT_GELU_TANH: f(std::integral_constant<int, TTC_ACT_GELU_TANH>()); break;
-        default: f(std::integral_constant<int, TTC_ACT_NONE>());
+        case TTC_ACT_RELU: return f(std::integral_constant<int, TTC_ACT_RELU>());
+        case TTC_ACT_SILU: return f(std::integral_constant<int, TTC_ACT_SILU>());
+        case TTC_ACT_GELU: return f(std::integral_constant<int, TTC_ACT_GELU>());
+        case TTC_ACT_GELU_TANH: return f(std::integral_constant<int, TTC_ACT_GELU_TANH>());
+        default: return f(std::integral_constant<int, TTC_ACT_NONE>());
     }
 }
 
@@ -366,16 +370,15 @@ int plan_linear_backward(const ttc_linear_backward_desc& d, void* ws, size_t* by
         g.vec_pre = vec8_ok(d.pre, d.dtype, d.ldp);
         g.vec_dz = true;
         const dim3 grid((unsigned)bands(d.M), (unsigned)((d.N + kStripe - 1) / kStripe));
-        with_activation(d.act, [&](auto act) {
-            if (d.dtype == TTC_BF16)
-                linear_grad_kernel<__nv_bfloat16, act()><<<grid, 32 * kBandWarps, 0, rt().stream>>>(g);
-            else
-                linear_grad_kernel<__half, act()><<<grid, 32 * kBandWarps, 0, rt().stream>>>(g);
-        });
         count_launch();
-        if (int rc = check_cuda(cudaGetLastError(), "linear_backward launch")) return rc;
+        if (int rc = with_activation(d.act, [&](auto act) {
+                return launch_overlapped(d.dtype == TTC_BF16 ? linear_grad_kernel<__nv_bfloat16, act()>
+                                                             : linear_grad_kernel<__half, act()>,
+                                         grid, 32 * kBandWarps, g);
+            }))
+            return rc;
         if (d.dbias)
-            if (int rc = launch_sum_partials(g.partials, bands(d.M), d.N, d.dbias, d.dtype, rt().stream)) return rc;
+            if (int rc = launch_sum_partials(g.partials, bands(d.M), d.N, d.dbias, d.dtype)) return rc;
     }
     if (d.dx)
         if (int rc = run_product(px, scratch)) return rc;
@@ -434,14 +437,13 @@ int plan_gated_backward(const ttc_gated_linear_backward_desc& d, void* ws, size_
     g.vec_gate = vec8_ok(d.gate, d.dtype, d.ldp);
     g.vec_up = vec8_ok(d.up, d.dtype, d.ldp);
     const dim3 grid((unsigned)bands(d.M), (unsigned)((d.N + kStripe - 1) / kStripe));
-    with_activation(d.act, [&](auto act) {
-        if (d.dtype == TTC_BF16)
-            gated_grad_kernel<__nv_bfloat16, act()><<<grid, 32 * kBandWarps, 0, rt().stream>>>(g);
-        else
-            gated_grad_kernel<__half, act()><<<grid, 32 * kBandWarps, 0, rt().stream>>>(g);
-    });
     count_launch();
-    if (int rc = check_cuda(cudaGetLastError(), "gated_linear_backward launch")) return rc;
+    if (int rc = with_activation(d.act, [&](auto act) {
+            return launch_overlapped(
+                d.dtype == TTC_BF16 ? gated_grad_kernel<__nv_bfloat16, act()> : gated_grad_kernel<__half, act()>, grid,
+                32 * kBandWarps, g);
+        }))
+        return rc;
     if (d.dx)
         if (int rc = run_product(px, scratch)) return rc;
     return d.dwg ? run_product(pw, scratch) : TTC_OK;

@@ -909,6 +909,8 @@ struct Copy {
 
 template <class T>
 __global__ void __launch_bounds__(256) pad_rows_kernel(const __grid_constant__ Copy c) {
+    grid_wait();
+    grid_trigger();
     for (long long r = blockIdx.x; r < c.rows; r += gridDim.x) {
         const T* s = static_cast<const T*>(c.src) + r * c.lds;
         T* d = static_cast<T*>(c.dst) + r * c.ldd;
@@ -1053,12 +1055,9 @@ int run_product(const Product& given, void* scratch) {
         Operand& o = const_cast<Operand&>(*s[i].o);
         const Copy c{o.ptr, room, s[i].rows, s[i].cols, o.ld, padded_ld(s[i].cols, es)};
         const unsigned grid = (unsigned)std::min<long long>(c.rows, 16ll * sms);
-        if (f8)
-            pad_rows_kernel<uint8_t><<<grid, 256, 0, rt().stream>>>(c);
-        else
-            pad_rows_kernel<uint16_t><<<grid, 256, 0, rt().stream>>>(c);
         count_launch();
-        if (int rc = check_cuda(cudaGetLastError(), "operand copy launch")) return rc;
+        if (int rc = launch_overlapped(f8 ? pad_rows_kernel<uint8_t> : pad_rows_kernel<uint16_t>, dim3(grid), 256, c))
+            return rc;
         o = {room, c.ldd};
         room += align256((size_t)c.rows * c.ldd * es);
     }

@@ -199,6 +199,10 @@ __global__ void __launch_bounds__(ONE ? 32 * kWarpRows : kMaxBlock) rms_norm_ker
     __shared__ float2 slots[2][kSlots];
     const RowPlace at = row_place<ONE>(p.cluster);
     const Lane l = at.lane;
+    // No grid_trigger(): blocks of the next kernel that came early would share
+    // the SMs unevenly with these, and this grid's size counts on an even share
+    // (43 -> 47 us for 8192 rows of 4096).
+    grid_wait();
     float w[C][kPer<T>];
     load_weight<T, VEC, C>(p.weight, p.weight_f32, p.cols, l, w);
     const T *x = static_cast<const T*>(p.x), *res = static_cast<const T*>(p.residual);
@@ -268,6 +272,7 @@ __global__ void __launch_bounds__(ONE ? 32 * kWarpRows : kMaxBlock, ONE ? (C == 
     __shared__ float2 slots[2][kSlots];
     const RowPlace at = row_place<ONE>(p.cluster);
     const Lane l = at.lane;
+    grid_wait();
     float w[C][kPer<T>], dw[C][kPer<T>] = {};
     load_weight<T, VEC, C>(p.weight, p.weight_f32, p.cols, l, w);
     const T *dy = static_cast<const T*>(p.dy), *hid = static_cast<const T*>(p.hidden);
@@ -355,6 +360,7 @@ constexpr int kWide = 1024;
 template <class T, class Y>
 __global__ void __launch_bounds__(kWide) rms_norm_wide_kernel(const __grid_constant__ NormParams p) {
     __shared__ float2 slots[2][kSlots];
+    grid_wait();
     auto weight = [&](int c) {
         return p.weight_f32 ? static_cast<const float*>(p.weight)[c] : to_f32<T>(static_cast<const T*>(p.weight)[c]);
     };
@@ -393,6 +399,7 @@ __global__ void __launch_bounds__(kWide) rms_norm_wide_kernel(const __grid_const
 template <class T>
 __global__ void __launch_bounds__(kWide) rms_norm_backward_wide_kernel(const __grid_constant__ NormBackwardParams p) {
     __shared__ float2 slots[2][kSlots];
+    grid_wait();
     float* part = p.partials ? p.partials + (long long)blockIdx.x * p.cols : nullptr;
     if (part)
         for (int c = threadIdx.x; c < p.cols; c += kWide) part[c] = 0.0f;  // a thread owns its columns throughout
@@ -433,6 +440,8 @@ __global__ void __launch_bounds__(1024) sum_partials_kernel(const float* partial
     __shared__ float part[32][33];
     const int lane = threadIdx.x & 31, g = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
     float s = 0.0f;
+    grid_wait();
+    grid_trigger();
     if (c < cols) {
 #pragma unroll 8
         for (int b = g; b < n; b += 32) s += partials[(long long)b * cols + c];
@@ -535,16 +544,12 @@ int launch_rows(void (*kernel)(const Params), const Params& p, const RowShape& s
     static int used = 0;
     cudaLaunchConfig_t cfg;
     std::memset(&cfg, 0, sizeof cfg);
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)s.cluster;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
     cfg.gridDim = dim3((unsigned)(clusters * s.cluster), 1, 1);
     cfg.blockDim = dim3((unsigned)s.block, 1, 1);
     cfg.stream = rt().stream;
     cfg.attrs = attr;
-    cfg.numAttrs = s.cluster > 1 ? 1 : 0;
+    cfg.numAttrs = launch_attributes(attr, s.cluster);
     int most = 0;
     for (int i = 0; i < used && !most; ++i)
         if (seen[i].kernel == (const void*)kernel && seen[i].device == rt().device && seen[i].block == s.block &&
@@ -572,8 +577,7 @@ template <class T, class Y, bool VEC>
 int launch_norm(const NormParams& p, const RowShape& s) {
     if (s.block == 0) {
         const long long n = std::min<long long>(p.rows, 2ll * rt().sm_count);
-        rms_norm_wide_kernel<T, Y><<<(unsigned)n, kWide, 0, rt().stream>>>(p);
-        return TTC_OK;
+        return launch_overlapped(rms_norm_wide_kernel<T, Y>, dim3((unsigned)n), kWide, p);
     }
     if (s.one) {
         const long long n = (p.rows + kWarpRows - 1) / kWarpRows;
@@ -597,8 +601,7 @@ int launch_norm_type(const NormParams& p, int y_dtype, const RowShape& s, bool v
 template <class T, bool VEC>
 int launch_norm_backward(const NormBackwardParams& p, const RowShape& s, int& clusters) {
     if (s.block == 0) {
-        rms_norm_backward_wide_kernel<T><<<clusters, kWide, 0, rt().stream>>>(p);
-        return TTC_OK;
+        return launch_overlapped(rms_norm_backward_wide_kernel<T>, dim3((unsigned)clusters), kWide, p);
     }
     return launch_rows(!s.one          ? rms_norm_backward_kernel<T, VEC, false, 2>
                        : s.chunks == 1 ? rms_norm_backward_kernel<T, VEC, true, 1>
@@ -624,10 +627,9 @@ int check_workspace(const char* op, const void* ws, size_t have, size_t need) {
     return TTC_OK;
 }
 
-int launch_sum_partials(const float* partials, int n, int cols, void* out, int dtype, cudaStream_t st) {
-    sum_partials_kernel<<<(cols + 31) / 32, 1024, 0, st>>>(partials, n, cols, out, dtype);
+int launch_sum_partials(const float* partials, int n, int cols, void* out, int dtype) {
     count_launch();
-    return check_cuda(cudaGetLastError(), "partial sums launch");
+    return launch_overlapped(sum_partials_kernel, dim3((unsigned)((cols + 31) / 32)), 1024, partials, n, cols, out, dtype);
 }
 
 }  // namespace ttc
@@ -696,7 +698,7 @@ int ttc_rms_norm_backward(const ttc_rms_norm_backward_desc* desc) {
         return rc;
     count_launch();
     if (int rc = check_cuda(cudaGetLastError(), "rms_norm_backward launch")) return rc;
-    return d.dweight ? launch_sum_partials(p.partials, clusters, d.cols, d.dweight, d.weight_dtype, st) : TTC_OK;
+    return d.dweight ? launch_sum_partials(p.partials, clusters, d.cols, d.dweight, d.weight_dtype) : TTC_OK;
 }
 
 }  // extern "C"
