@@ -103,18 +103,21 @@ struct Product {
 int run_product(const Product& p, void* scratch);
 size_t product_scratch(const Product& p);
 
-// Launch attributes of these operators' kernels: a cluster where there is one,
-// and leave to be launched while the kernel before it in the stream still runs
-// (each kernel calls grid_wait() before it touches memory). Returns their number.
+// The attribute of a launch in clusters; returns the number of attributes (0 or 1).
+inline int cluster_attribute(cudaLaunchAttribute& attr, int cluster) {
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)cluster;
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    return cluster > 1;
+}
+// The attributes of a launch that may begin while the kernel before it in the
+// stream still runs (the kernel calls grid_wait() before it touches memory), in
+// clusters where `cluster` > 1.
 inline int launch_attributes(cudaLaunchAttribute (&attr)[2], int cluster) {
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
-    if (cluster == 1) return 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = (unsigned)cluster;
-    attr[1].val.clusterDim.y = 1;
-    attr[1].val.clusterDim.z = 1;
-    return 2;
+    return 1 + cluster_attribute(attr[1], cluster);
 }
 
 #ifdef __CUDACC__

@@ -119,6 +119,7 @@ __device__ __forceinline__ void load_weight(const void* weight, bool f32, int co
 // use in turn, so that one barrier a row is enough; in a cluster of more than
 // one block every warp writes its pair into the buffer of each block.
 constexpr int kSlots = 64;  // 8 blocks of 8 warps
+constexpr int kMaxStages = 8;
 template <bool ONE, bool MAX>
 __device__ __forceinline__ void reduce_row(float& a, float& b, float2* slots, int blocks) {
     auto warp = [&] {
@@ -199,10 +200,6 @@ __global__ void __launch_bounds__(ONE ? 32 * kWarpRows : kMaxBlock) rms_norm_ker
     __shared__ float2 slots[2][kSlots];
     const RowPlace at = row_place<ONE>(p.cluster);
     const Lane l = at.lane;
-    // No grid_trigger(): blocks of the next kernel that came early would share
-    // the SMs unevenly with these, and this grid's size counts on an even share
-    // (43 -> 47 us for 8192 rows of 4096).
-    grid_wait();
     float w[C][kPer<T>];
     load_weight<T, VEC, C>(p.weight, p.weight_f32, p.cols, l, w);
     const T *x = static_cast<const T*>(p.x), *res = static_cast<const T*>(p.residual);
@@ -259,7 +256,7 @@ struct NormBackwardParams {
     void* dx;
     float* partials;  // [blocks or clusters, cols] sums of dy * hidden * rstd, or NULL
     long long lddy, ldh, lddh, lddx;
-    int weight_f32;
+    int weight_f32, weight_vec;  // weight_vec: of dtype, 16-byte aligned
     int cluster;
 };
 
@@ -272,7 +269,6 @@ __global__ void __launch_bounds__(ONE ? 32 * kWarpRows : kMaxBlock, ONE ? (C == 
     __shared__ float2 slots[2][kSlots];
     const RowPlace at = row_place<ONE>(p.cluster);
     const Lane l = at.lane;
-    grid_wait();
     float w[C][kPer<T>], dw[C][kPer<T>] = {};
     load_weight<T, VEC, C>(p.weight, p.weight_f32, p.cols, l, w);
     const T *dy = static_cast<const T*>(p.dy), *hid = static_cast<const T*>(p.hidden);
@@ -353,6 +349,153 @@ __global__ void __launch_bounds__(ONE ? 32 * kWarpRows : kMaxBlock, ONE ? (C == 
     }
 }
 
+// Longer aligned rows (more than 128 chunks, up to 2048): a ring in shared memory
+// that bulk copies keep full, so that several rows are on their way without
+// registers for them. Between two barriers a thread adds up its share of the next
+// row and finishes its share of this one, whose sums the last barrier completed:
+// two independent strands of work, one barrier a row.
+struct RingParams {
+    NormBackwardParams p;
+    int stages, row_bytes;
+    int* status;
+    long long wait_limit;
+};
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                 "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
+}
+
+template <class T, int C, int MAX>
+__global__ void __launch_bounds__(MAX, 512 / MAX) rms_norm_backward_ring_kernel(const __grid_constant__ RingParams q) {
+    extern __shared__ __align__(16) uint8_t ring[];
+    __shared__ float2 slots[2][MAX / 32];
+    __shared__ alignas(8) uint64_t bars[kMaxStages];
+    const NormBackwardParams& p = q.p;
+    const int t = threadIdx.x, threads = blockDim.x, n = p.cols / kPer<T>;  // chunks of a row
+    const int stage_bytes = (p.dhidden ? 3 : 2) * q.row_bytes;
+    const uint32_t base = smem_u32(ring);
+    const int mine = (int)((p.rows - blockIdx.x + gridDim.x - 1) / gridDim.x);  // rows of this block
+    auto issue = [&](int i, int s) {  // one thread
+        const long long r = blockIdx.x + (long long)i * gridDim.x;
+        const uint32_t bar = smem_u32(&bars[s]), dst = base + s * stage_bytes;
+        mbar_arrive_expect_tx(bar, stage_bytes);
+        bulk_load(dst, static_cast<const T*>(p.dy) + r * p.lddy, q.row_bytes, bar);
+        bulk_load(dst + q.row_bytes, static_cast<const T*>(p.hidden) + r * p.ldh, q.row_bytes, bar);
+        if (p.dhidden) bulk_load(dst + 2 * q.row_bytes, static_cast<const T*>(p.dhidden) + r * p.lddh, q.row_bytes, bar);
+    };
+    if (t == 0) {
+        for (int s = 0; s < q.stages; ++s) mbar_init(smem_u32(&bars[s]), 1);
+        mbar_fence_init();
+    }
+    __syncthreads();
+    if (t == 0)
+        for (int i = 0; i < q.stages && i < mine; ++i) issue(i, i);
+    uint4 w[C];
+    float dw[C][kPer<T>] = {};
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const int k = c * threads + t;
+        w[c] = p.weight_vec && k < n ? __ldg(static_cast<const uint4*>(p.weight) + k) : make_uint4(0, 0, 0, 0);
+    }
+    auto weight = [&](int c, float (&v)[kPer<T>]) {
+        if (p.weight_vec) {
+            unpack<T>(w[c], v);
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < kPer<T>; ++i) {
+            const int k = (c * threads + t) * kPer<T> + i;
+            v[i] = k >= p.cols    ? 0.0f
+                   : p.weight_f32 ? __ldg(static_cast<const float*>(p.weight) + k)
+                                  : to_f32<T>(static_cast<const T*>(p.weight)[k]);
+        }
+    };
+    auto chunk = [&](int s, int stream, int c, float (&v)[kPer<T>]) {
+        const int k = c * threads + t;
+        unpack<T>(k < n ? *reinterpret_cast<const uint4*>(ring + s * stage_bytes + stream * q.row_bytes + k * 16)
+                        : make_uint4(0, 0, 0, 0),
+                  v);
+    };
+    bool failed = false;
+    int next = 0;  // the stage of the next row to add up, and its parity
+    uint32_t parity = 0;
+    auto add_up = [&](int to) {
+        if (!failed) failed = !mbar_wait(smem_u32(&bars[next]), parity, q.wait_limit);
+        float sum = 0.0f, dot = 0.0f;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            float g[kPer<T>], h[kPer<T>], wv[kPer<T>];
+            chunk(next, 0, c, g);
+            chunk(next, 1, c, h);
+            weight(c, wv);
+#pragma unroll
+            for (int k = 0; k < kPer<T>; ++k) {
+                sum += h[k] * h[k];
+                dot += g[k] * wv[k] * h[k];
+            }
+        }
+        sum = warp_sum(sum);
+        dot = warp_sum(dot);
+        if ((t & 31) == 0) slots[to][t >> 5] = make_float2(sum, dot);
+        if (++next == q.stages) {
+            next = 0;
+            parity ^= 1;
+        }
+    };
+    add_up(0);
+    __syncthreads();
+    int s = 0;  // this row's stage
+    for (int i = 0; i < mine; ++i) {
+        const long long r = blockIdx.x + (long long)i * gridDim.x;
+        float2 total = slots[i & 1][0];
+        for (int k = 1; k < threads / 32; ++k) {
+            total.x += slots[i & 1][k].x;
+            total.y += slots[i & 1][k].y;
+        }
+        if (i + 1 < mine) add_up((i + 1) & 1);
+        const float rstd = rsqrtf(total.x / (float)p.cols + p.eps);
+        const float k2 = total.y * rstd * rstd / (float)p.cols;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            float g[kPer<T>], h[kPer<T>], wv[kPer<T>], out[1][kPer<T>];
+            chunk(s, 0, c, g);
+            chunk(s, 1, c, h);
+            weight(c, wv);
+#pragma unroll
+            for (int k = 0; k < kPer<T>; ++k) {
+                out[0][k] = rstd * (g[k] * wv[k] - h[k] * k2);
+                dw[c][k] += g[k] * h[k] * rstd;
+            }
+            if (p.dhidden) {
+                chunk(s, 2, c, g);
+#pragma unroll
+                for (int k = 0; k < kPer<T>; ++k) out[0][k] += g[k];
+            }
+            store_row<T, T, true, 1>(static_cast<T*>(p.dx) + r * p.lddx, p.cols, Lane{c * threads + t, 0}, out);
+        }
+        __syncthreads();
+        if (t == 0 && i + q.stages < mine) issue(i + q.stages, s);
+        if (++s == q.stages) s = 0;
+    }
+    if (failed) *(volatile int*)q.status = 1;
+    if (t == 0 && failed)  // never leave with copies in flight
+        for (int i = mine > q.stages ? mine - q.stages : 0; i < mine; ++i)
+            mbar_wait(smem_u32(&bars[i % q.stages]), (uint32_t)(i / q.stages) & 1, q.wait_limit);
+    if (!p.partials) return;
+    float* part = p.partials + (long long)blockIdx.x * p.cols;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const int k = (c * threads + t) * kPer<T>;
+        if (k < p.cols) {
+#pragma unroll
+            for (int i = 0; i < kPer<T>; i += 4)
+                *reinterpret_cast<float4*>(part + k + i) = make_float4(dw[c][i], dw[c][i + 1], dw[c][i + 2], dw[c][i + 3]);
+        }
+    }
+}
+
 // Rows that do not fit in registers: one block a row, two passes over it (the
 // second finds it in L2).
 constexpr int kWide = 1024;
@@ -360,7 +503,6 @@ constexpr int kWide = 1024;
 template <class T, class Y>
 __global__ void __launch_bounds__(kWide) rms_norm_wide_kernel(const __grid_constant__ NormParams p) {
     __shared__ float2 slots[2][kSlots];
-    grid_wait();
     auto weight = [&](int c) {
         return p.weight_f32 ? static_cast<const float*>(p.weight)[c] : to_f32<T>(static_cast<const T*>(p.weight)[c]);
     };
@@ -399,7 +541,6 @@ __global__ void __launch_bounds__(kWide) rms_norm_wide_kernel(const __grid_const
 template <class T>
 __global__ void __launch_bounds__(kWide) rms_norm_backward_wide_kernel(const __grid_constant__ NormBackwardParams p) {
     __shared__ float2 slots[2][kSlots];
-    grid_wait();
     float* part = p.partials ? p.partials + (long long)blockIdx.x * p.cols : nullptr;
     if (part)
         for (int c = threadIdx.x; c < p.cols; c += kWide) part[c] = 0.0f;  // a thread owns its columns throughout
@@ -506,6 +647,7 @@ int check_norm_backward(const ttc_rms_norm_backward_desc& d) {
 
 // How a row is divided: threads of a block, blocks of a cluster and chunks a
 // thread; one: a warp has the row; block 0: the row does not fit.
+constexpr int kRingBytes = 200 * 1024;
 struct RowShape {
     int block, cluster, chunks, one;
 };
@@ -523,7 +665,7 @@ RowShape row_shape(int cols, int dtype) {
 int backward_clusters(long long rows, const RowShape& s) {
     if (s.block == 0) return (int)std::min<long long>(rows, 148 * 2);
     if (s.one) return (int)std::min<long long>((rows + kWarpRows - 1) / kWarpRows, 148 * (s.chunks == 4 ? 2 : 4));
-    return (int)std::min<long long>(rows, std::max(1, 148 * 512 / (s.block * s.cluster)));
+    return (int)std::min<long long>(rows, 148 * std::max(6, 512 / (s.block * s.cluster)));  // 6: the ring kernel's
 }
 
 size_t backward_bytes(const ttc_rms_norm_backward_desc& d) {
@@ -532,7 +674,10 @@ size_t backward_bytes(const ttc_rms_norm_backward_desc& d) {
 }
 
 // Launches `clusters` clusters, or as many as the GPU holds at once: a few more
-// than that would take a second round as long as the first.
+// than that would take a second round as long as the first. Not under the tail of
+// the kernel before: blocks that came while that one still holds part of an SM
+// would end up unevenly spread, and these grids count on an even share (43 -> 47
+// us for 8192 rows of 4096).
 template <class Params>
 int launch_rows(void (*kernel)(const Params), const Params& p, const RowShape& s, long long clusters,
                 int* launched = nullptr) {
@@ -544,12 +689,12 @@ int launch_rows(void (*kernel)(const Params), const Params& p, const RowShape& s
     static int used = 0;
     cudaLaunchConfig_t cfg;
     std::memset(&cfg, 0, sizeof cfg);
-    cudaLaunchAttribute attr[2];
+    cudaLaunchAttribute attr[1];
     cfg.gridDim = dim3((unsigned)(clusters * s.cluster), 1, 1);
     cfg.blockDim = dim3((unsigned)s.block, 1, 1);
     cfg.stream = rt().stream;
     cfg.attrs = attr;
-    cfg.numAttrs = launch_attributes(attr, s.cluster);
+    cfg.numAttrs = cluster_attribute(attr[0], s.cluster);
     int most = 0;
     for (int i = 0; i < used && !most; ++i)
         if (seen[i].kernel == (const void*)kernel && seen[i].device == rt().device && seen[i].block == s.block &&
@@ -577,7 +722,8 @@ template <class T, class Y, bool VEC>
 int launch_norm(const NormParams& p, const RowShape& s) {
     if (s.block == 0) {
         const long long n = std::min<long long>(p.rows, 2ll * rt().sm_count);
-        return launch_overlapped(rms_norm_wide_kernel<T, Y>, dim3((unsigned)n), kWide, p);
+        rms_norm_wide_kernel<T, Y><<<(unsigned)n, kWide, 0, rt().stream>>>(p);
+        return check_cuda(cudaGetLastError(), "rms_norm launch");
     }
     if (s.one) {
         const long long n = (p.rows + kWarpRows - 1) / kWarpRows;
@@ -598,10 +744,57 @@ int launch_norm_type(const NormParams& p, int y_dtype, const RowShape& s, bool v
     return vec ? launch_norm<T, T, true>(p, s) : launch_norm<T, T, false>(p, s);
 }
 
+// The ring kernel's shape for the aligned rows that it is faster on; threads 0:
+// another kernel takes them. As many blocks an SM as have registers (96 a thread)
+// and a ring of three rows each. In us, register kernel / this one: 16384 x 4096
+// bf16 94 / 103, 8192 x 8192 bf16 133 / 108, 4096 x 16384 bf16 143 / 125, 16384 x
+// 2048 f32 92 / 84, 8192 x 8192 f32 231 / 187. 16-bit rows up to 512 chunks have
+// twice the arithmetic a byte and more rows on an SM with the register kernel.
+struct RingShape {
+    int threads, chunks, stages, per_sm;
+};
+RingShape ring_shape(int cols, int dtype, bool dhidden) {
+    const int es = dtype_size(dtype), n = cols / (16 / es);
+    const int stage = cols * es * (dhidden ? 3 : 2);
+    if (n <= (es == 4 ? 256 : 512) || n > 2048 || cols % (16 / es) || 2 * stage > kRingBytes) return {0, 0, 0, 0};
+    const int chunks = n <= 1024 ? 2 : 4, threads = (n + 32 * chunks - 1) / (32 * chunks) * 32;
+    int per_sm = std::max(1, std::min(6, 65536 / 96 / threads));
+    while (per_sm > 1 && 3 * stage > kRingBytes / per_sm) --per_sm;
+    return {threads, chunks, std::min(kMaxStages, kRingBytes / per_sm / stage), per_sm};
+}
+
+template <class T>
+int launch_ring(const NormBackwardParams& p, const RingShape& s, int& blocks) {
+    RingParams q;
+    q.p = p;
+    q.stages = s.stages;
+    q.row_bytes = p.cols * (int)sizeof(T);
+    q.wait_limit = kWaitLimitCycles;
+    if (int rc = device_status_ptr(&q.status)) return rc;
+    const int smem = s.stages * q.row_bytes * (p.dhidden ? 3 : 2);
+    auto kernel = s.threads <= 256 ? rms_norm_backward_ring_kernel<T, 2, 256>
+                  : s.chunks == 2  ? rms_norm_backward_ring_kernel<T, 2, 512>
+                                   : rms_norm_backward_ring_kernel<T, 4, 512>;
+    static bool seen[kMaxDevices][3] = {};
+    bool& ready = seen[rt().device][s.threads <= 256 ? 0 : s.chunks / 2];
+    if (!ready) {
+        TTC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes));
+        ready = true;
+    }
+    blocks = (int)std::min<long long>(p.rows, (long long)s.per_sm * std::min(rt().sm_count, 148));
+    kernel<<<(unsigned)blocks, s.threads, smem, rt().stream>>>(q);
+    return check_cuda(cudaGetLastError(), "rms_norm_backward launch");
+}
+
 template <class T, bool VEC>
 int launch_norm_backward(const NormBackwardParams& p, const RowShape& s, int& clusters) {
+    if (VEC) {
+        const RingShape ring = ring_shape(p.cols, sizeof(T) == 4 ? TTC_F32 : TTC_BF16, p.dhidden != nullptr);
+        if (ring.threads) return launch_ring<T>(p, ring, clusters);
+    }
     if (s.block == 0) {
-        return launch_overlapped(rms_norm_backward_wide_kernel<T>, dim3((unsigned)clusters), kWide, p);
+        rms_norm_backward_wide_kernel<T><<<clusters, kWide, 0, rt().stream>>>(p);
+        return check_cuda(cudaGetLastError(), "rms_norm_backward launch");
     }
     return launch_rows(!s.one          ? rms_norm_backward_kernel<T, VEC, false, 2>
                        : s.chunks == 1 ? rms_norm_backward_kernel<T, VEC, true, 1>
@@ -684,7 +877,8 @@ int ttc_rms_norm_backward(const ttc_rms_norm_backward_desc* desc) {
     int clusters = backward_clusters(d.rows, s);
     const NormBackwardParams p{d.rows, d.cols, d.eps, d.dy, d.hidden, d.weight, d.dhidden, d.dx,
                                d.dweight ? (float*)d.workspace : nullptr,
-                               d.lddy, d.ldh, d.lddh, d.lddx, d.weight_dtype == TTC_F32, s.cluster};
+                               d.lddy, d.ldh, d.lddh, d.lddx, d.weight_dtype == TTC_F32,
+                               d.weight_dtype == d.dtype && (uintptr_t)d.weight % 16 == 0, s.cluster};
     const int es = dtype_size(d.dtype), per = 16 / es;
     const bool vec = d.cols % per == 0 && rows_aligned(d.dy, es, per, d.lddy) && rows_aligned(d.hidden, es, per, d.ldh) &&
                      rows_aligned(d.dhidden, es, per, d.lddh) && rows_aligned(d.dx, es, per, d.lddx);
