@@ -327,19 +327,19 @@ def act_bound(act, z, dz):
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
 @pytest.mark.parametrize("dtype,trans_w", [("bf16", False), ("bf16", True), ("f16", False), ("f16", True), ("e4m3", True)])
-@pytest.mark.parametrize("form", ["plain", "all", "odd"])
+@pytest.mark.parametrize("form", ["plain", "all", "odd", "f32", "residual"])
 def test_linear(lib, M, N, K, dtype, trans_w, form):
     g = gen(M + 3 * N + 5 * K)
-    pad, shift = {"plain": (-K % 16 if trans_w else 0, 0), "all": (16, 16), "odd": (3, 1)}[form]
+    pad, shift = {"plain": (-K % 16 if trans_w else 0, 0), "odd": (3, 1)}.get(form, (16, 16))
     out = "bf16" if dtype == "e4m3" else dtype
-    if form == "odd":
+    if form in ("odd", "f32"):
         out = "f32"
-    act = {"plain": "none", "all": "gelu_tanh", "odd": "silu"}[form]
+    act = {"plain": "none", "all": "gelu_tanh", "odd": "silu", "f32": "gelu", "residual": "relu"}[form]
     x, (w,), xv, (wv,), xs, (ws,) = product_inputs(g, M, N, K, dtype, trans_w, pad, shift)
     y = Mat(M, N, out, pad, shift)
-    bias = Mat(1, N, out, 0, shift, rand(g, 1, N)) if form != "plain" else None
+    bias = Mat(1, N, out, 0, shift, rand(g, 1, N)) if form not in ("plain", "residual") else None
     res = Mat(M, N, out, pad, shift, rand(g, M, N)) if form != "plain" else None
-    pre = Mat(M, N, out, pad, shift) if form == "all" else None
+    pre = Mat(M, N, out, pad, shift) if form in ("all", "f32") else None
     d = lib.linear_desc(M, N, K, x.ptr, x.ld, w.ptr, w.ld, y.ptr, y.ld, lib.DTYPES[dtype], y_dtype=lib.DTYPES[out],
                         trans_w=trans_w, act=lib.ACTIVATIONS[act], bias=ptr(bias), residual=ptr(res), ldr=ld(res),
                         pre=ptr(pre), ldp=ld(pre), x_scales=ptr(xs), w_scales=ptr(ws))
@@ -404,17 +404,17 @@ def test_products_keep_infinities_and_nan_in_their_rows(lib, M):
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
 @pytest.mark.parametrize("dtype,trans_w", [("bf16", False), ("bf16", True), ("f16", True), ("e4m3", True)])
-@pytest.mark.parametrize("form", ["plain", "saved", "odd"])
+@pytest.mark.parametrize("form", ["plain", "saved", "odd", "f32"])
 def test_gated_linear(lib, M, N, K, dtype, trans_w, form):
     g = gen(M + 2 * N + 7 * K)
-    pad, shift = {"plain": (0, 0), "saved": (16, 16), "odd": (3, 1)}[form]
+    pad, shift = {"plain": (0, 0), "saved": (16, 16), "odd": (3, 1), "f32": (16, 16)}[form]
     out = "bf16" if dtype == "e4m3" else dtype
-    if form == "odd":
+    if form in ("odd", "f32"):
         out = "f32"
-    act = {"plain": "silu", "saved": "gelu", "odd": "gelu_tanh"}[form]
+    act = {"plain": "silu", "saved": "gelu", "odd": "gelu_tanh", "f32": "relu"}[form]
     x, (wg, wu), xv, (gv, uv), xs, (gs, us) = product_inputs(g, M, N, K, dtype, trans_w, pad, shift, ("wg", "wu"))
     y = Mat(M, N, out, pad, shift)
-    gate, up = (Mat(M, N, out, pad, shift) if form == "saved" else None for _ in range(2))
+    gate, up = (Mat(M, N, out, pad, shift) if form in ("saved", "f32") else None for _ in range(2))
     d = lib.gated_linear_desc(M, N, K, x.ptr, x.ld, wg.ptr, wu.ptr, wg.ld, y.ptr, y.ld, lib.DTYPES[dtype],
                               y_dtype=lib.DTYPES[out], trans_w=trans_w, act=lib.ACTIVATIONS[act], gate=ptr(gate),
                               up=ptr(up), ldp=ld(gate), x_scales=ptr(xs), wg_scales=ptr(gs), wu_scales=ptr(us))
@@ -773,6 +773,100 @@ def test_capture_and_replay_with_new_inputs(lib):
     torch.cuda.synchronize()
     for k, v in want.items():
         assert torch.equal(keep[k], v), k
+
+
+_FIRST_IN_A_CAPTURE = r"""
+import sys, torch
+sys.path.insert(0, %r)
+sys.path.insert(0, %r)
+import test_ffn_gpu as t
+from tt_lazy_b200 import capi as lib
+lib.init(0)
+M, D, H = 300, 256, 2560
+x = t.block_inputs(1, M, D, H)
+keep = {}
+side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+torch.cuda.synchronize()
+with torch.cuda.stream(side):
+    with torch.cuda.graph(graph, stream=side):
+        lib.set_stream(side.cuda_stream)
+        t.run_block(lib, x, M, D, H, keep)
+lib.set_stream(torch.cuda.default_stream().cuda_stream)
+graph.replay()
+torch.cuda.synchronize()
+got = {k: v.clone() for k, v in keep.items() if v is not None and not k.startswith("ws")}
+want = t.run_block(lib, x, M, D, H, {})
+lib.synchronize()
+assert all(torch.equal(v, want[k]) for k, v in got.items())
+print("equal", len(got))
+"""
+
+
+def test_first_calls_of_a_process_inside_a_capture():
+    """Nothing that a first call sets up is refused while a stream is being captured."""
+    import os
+    import subprocess
+    import sys
+
+    here = os.path.dirname(os.path.abspath(__file__))
+    r = subprocess.run([sys.executable, "-c", _FIRST_IN_A_CAPTURE % (os.path.dirname(here), here)], capture_output=True,
+                       text=True, timeout=300)
+    assert r.returncode == 0 and "equal" in r.stdout, r.stdout[-2000:] + r.stderr[-2000:]
+
+
+def test_offsets_past_32_bits(lib):
+    """Tensors of more than 2^31 elements: rows from their far end against the same
+    rows computed in a small call."""
+    torch.cuda.empty_cache()
+    rows, cols = 270_000, 8192
+    x = torch.randn(1000, cols, device="cuda").bfloat16().repeat(rows // 1000, 1)
+    y, hidden = torch.empty_like(x), torch.empty_like(x)
+    w = torch.randn(cols, device="cuda").bfloat16()
+    assert x.numel() > 2 ** 31
+
+    def norm(x, y, h):
+        lib.rms_norm(lib.rms_norm_desc(x.shape[0], cols, x.data_ptr(), cols, w.data_ptr(), y.data_ptr(), cols, lib.BF16,
+                                       residual=x.data_ptr(), ldr=cols, hidden=h.data_ptr(), ldh=cols))
+
+    norm(x, y, hidden)
+    small_y, small_h = torch.empty_like(x[:1000]), torch.empty_like(x[:1000])
+    norm(x[:1000], small_y, small_h)
+    for k in (0, rows // 1000 - 1):
+        assert torch.equal(y[k * 1000:(k + 1) * 1000], small_y) and torch.equal(hidden[k * 1000:(k + 1) * 1000], small_h)
+    dx, small_dx = y, small_y
+
+    def back(x, dx):
+        d = lib.rms_norm_backward_desc(x.shape[0], cols, x.data_ptr(), cols, x.data_ptr(), cols, w.data_ptr(),
+                                       dx.data_ptr(), cols, None, lib.BF16, dhidden=x.data_ptr(), lddh=cols)
+        lib.rms_norm_backward(d)
+
+    back(x, dx)
+    back(x[:1000], small_dx)
+    assert torch.equal(dx[-1000:], small_dx)
+    # a product with a far x, and one with a far y
+    N = 72
+    wn = (torch.randn(N, cols, device="cuda") / 90).bfloat16()
+    out = torch.empty(rows, N, device="cuda", dtype=torch.bfloat16)
+    lib.linear(lib.linear_desc(rows, N, cols, x.data_ptr(), cols, wn.data_ptr(), cols, out.data_ptr(), N, lib.BF16,
+                               trans_w=True))
+    want = x[:1000].double() @ wn.double().t()
+    bound = U["bf16"] * want.abs() + (cols / 16 + 16) * 2.0 ** -22 * (x[:1000].double().abs() @ wn.double().abs().t())
+    within(out[-1000:], want, bound, "far x")
+    del hidden, out
+    K = 64
+    a = torch.randn(1000, K, device="cuda").bfloat16().repeat(rows // 1000, 1)
+    wk = torch.randn(cols, K, device="cuda").bfloat16()
+    bias = torch.randn(cols, device="cuda").bfloat16()
+    for residual in (None, x):
+        lib.linear(lib.linear_desc(rows, cols, K, a.data_ptr(), K, wk.data_ptr(), K, y.data_ptr(), cols, lib.BF16,
+                                   trans_w=True, bias=bias.data_ptr(),
+                                   residual=None if residual is None else residual.data_ptr(), ldr=cols))
+        want = a[:1000].double() @ wk.double().t() + bias.double()
+        acc = (K / 16 + 16) * 2.0 ** -22 * (a[:1000].double().abs() @ wk.double().abs().t()) + 2.0 ** -22 * want.abs()
+        want = want + (0 if residual is None else x[:1000].double())
+        within(y[-1000:], want, (U["bf16"] + 2.0 ** -23) * want.abs() + acc, "far y")
+    del x, y, a, dx
+    torch.cuda.empty_cache()
 
 
 def test_two_streams_at_once(lib):

@@ -13,7 +13,7 @@ namespace {
 
 // ------------------------------------------------------------------- checks
 // Keeps every tile count and padded width inside 32 bits; offsets are 64-bit.
-constexpr int kMaxRows = 1 << 30, kMaxWidth = 1 << 24;
+constexpr int kMaxRows = 1 << 30, kMaxWidth = 1 << 23;
 
 int check_product(const char* op, int M, int N, int K, int dtype, int trans_w, int act, bool backward) {
     if (M < 0 || N < 1 || K < 1)

@@ -296,6 +296,10 @@ int ttc_init(int device) {
     TTC_CUDA(cudaDeviceGetDefaultMemPool(&pool, device));
     uint64_t threshold = UINT64_MAX;
     TTC_CUDA(cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &threshold));
+    // Now, not at the first kernel that wants it: that one may be recorded into a
+    // CUDA graph, where allocations are refused.
+    int* status = nullptr;
+    if (int rc = device_status_ptr(&status)) return rc;
     r.device = device;
     r.initialized = true;
     return TTC_OK;
