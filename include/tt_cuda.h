@@ -57,7 +57,9 @@ int ttc_device_count(int* count);
 int ttc_version(void); /* (major << 16) | minor */
 
 /* The library stream (a cudaStream_t). ttc_set_stream(NULL) restores the
- * library's own stream. All launches and async copies go to this stream. */
+ * library's own stream (CUDA's legacy default stream, whose handle is NULL too,
+ * is set by its other name cudaStreamLegacy, (cudaStream_t)0x1). All launches
+ * and async copies go to this stream. */
 void* ttc_get_stream(void);
 int ttc_set_stream(void* cuda_stream);
 int ttc_synchronize(void);

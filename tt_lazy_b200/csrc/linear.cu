@@ -121,9 +121,10 @@ int check_gated_backward(const ttc_gated_linear_backward_desc& d) {
 // A block of 8 warps walks a band of rows of a 256-column stripe: a lane owns
 // 8 columns, a warp one row at a time, so that a column's sum for dbias stays
 // in a register. Memory bound: each value is read once and written once, 16
-// bytes per lane and access. 4096 x 8192 in bf16: 43 us with gelu (4.7 TB/s), 56
-// us for the gated pair with silu (6.0 TB/s). Two rows of loads in flight per
-// warp instead of one cost more in registers than they hid (72 and 88 us).
+// bytes per lane and access, a row's loads ahead of its arithmetic (as packed
+// registers: as floats, 72 and 88 us). 4096 x 8192 in bf16: 39 us with gelu (5.2
+// TB/s), 51 us for the gated pair with silu (6.6 TB/s); without the row ahead 47
+// and 73.
 constexpr int kStripe = 256, kBandWarps = 8;
 // Rows of a block: 64, more when that would make over 256 bands of partial sums.
 int band_rows(int M) { return std::max(64, (M + 255) / 256); }
@@ -139,9 +140,9 @@ struct LinearGradParams {
     bool vec_dy, vec_pre, vec_dz;
 };
 
-// ACT at compile time: as a switch in the loop it took 85 us instead of 49.
+// ACT at compile time: as a switch in the loop it took half as long again.
 template <class T, int ACT>
-__global__ void __launch_bounds__(32 * kBandWarps) linear_grad_kernel(const __grid_constant__ LinearGradParams p) {
+__global__ void __launch_bounds__(32 * kBandWarps, 4) linear_grad_kernel(const __grid_constant__ LinearGradParams p) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int col = blockIdx.y * kStripe + lane * 8, n = p.N - col;
     float sum[8] = {};
@@ -149,11 +150,27 @@ __global__ void __launch_bounds__(32 * kBandWarps) linear_grad_kernel(const __gr
     grid_trigger();
     if (n > 0) {
         const long long r1 = min((long long)p.M, (blockIdx.x + 1ll) * p.band_rows);
-        for (long long r = (long long)blockIdx.x * p.band_rows + warp; r < r1; r += kBandWarps) {
+        // whole aligned groups: the next row is on its way while this one is computed
+        const bool ahead = p.vec_dy && n >= 8 && (ACT == TTC_ACT_NONE || p.vec_pre);
+        uint4 gn = {}, zn = {};
+        auto fetch = [&](long long r) {
+            gn = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.dy) + r * p.lddy + col);
+            if (ACT != TTC_ACT_NONE)
+                zn = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.pre) + r * p.ldp + col);
+        };
+        long long r = (long long)blockIdx.x * p.band_rows + warp;
+        if (ahead && r < r1) fetch(r);
+        for (; r < r1; r += kBandWarps) {
             float g[8], z[8];
-            load8(static_cast<const T*>(p.dy) + r * p.lddy + col, n, p.vec_dy, g);
+            if (ahead) {
+                unpack8<T>(gn, g);
+                if (ACT != TTC_ACT_NONE) unpack8<T>(zn, z);
+                if (r + kBandWarps < r1) fetch(r + kBandWarps);
+            } else {
+                load8(static_cast<const T*>(p.dy) + r * p.lddy + col, n, p.vec_dy, g);
+                if (ACT != TTC_ACT_NONE) load8(static_cast<const T*>(p.pre) + r * p.ldp + col, n, p.vec_pre, z);
+            }
             if (ACT != TTC_ACT_NONE) {
-                load8(static_cast<const T*>(p.pre) + r * p.ldp + col, n, p.vec_pre, z);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     float y, dy;
@@ -190,18 +207,34 @@ struct GatedGradParams {
 };
 
 template <class T, int ACT>
-__global__ void __launch_bounds__(32 * kBandWarps) gated_grad_kernel(const __grid_constant__ GatedGradParams p) {
+__global__ void __launch_bounds__(32 * kBandWarps, 4) gated_grad_kernel(const __grid_constant__ GatedGradParams p) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int col = blockIdx.y * kStripe + lane * 8, n = p.N - col;
     grid_wait();
     grid_trigger();
     if (n <= 0) return;
     const long long r1 = min((long long)p.M, (blockIdx.x + 1ll) * p.band_rows);
-    for (long long r = (long long)blockIdx.x * p.band_rows + warp; r < r1; r += kBandWarps) {
+    const bool ahead = n >= 8 && p.vec_dy && p.vec_gate && p.vec_up;
+    uint4 dn = {}, gn = {}, un = {};
+    auto fetch = [&](long long r) {
+        dn = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.dy) + r * p.lddy + col);
+        gn = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.gate) + r * p.ldp + col);
+        un = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.up) + r * p.ldp + col);
+    };
+    long long r = (long long)blockIdx.x * p.band_rows + warp;
+    if (ahead && r < r1) fetch(r);
+    for (; r < r1; r += kBandWarps) {
         float d[8], g[8], u[8];
-        load8(static_cast<const T*>(p.dy) + r * p.lddy + col, n, p.vec_dy, d);
-        load8(static_cast<const T*>(p.gate) + r * p.ldp + col, n, p.vec_gate, g);
-        load8(static_cast<const T*>(p.up) + r * p.ldp + col, n, p.vec_up, u);
+        if (ahead) {
+            unpack8<T>(dn, d);
+            unpack8<T>(gn, g);
+            unpack8<T>(un, u);
+            if (r + kBandWarps < r1) fetch(r + kBandWarps);
+        } else {
+            load8(static_cast<const T*>(p.dy) + r * p.lddy + col, n, p.vec_dy, d);
+            load8(static_cast<const T*>(p.gate) + r * p.ldp + col, n, p.vec_gate, g);
+            load8(static_cast<const T*>(p.up) + r * p.ldp + col, n, p.vec_up, u);
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             float y, dy;

@@ -597,7 +597,8 @@ __device__ __forceinline__ float4 tile_sum4(uint32_t sbase, int splits, int i) {
     if (splits == 1) {
         asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
                      : "=f"(t.x), "=f"(t.y), "=f"(t.z), "=f"(t.w)
-                     : "r"(at));
+                     : "r"(at)
+                     : "memory");
         return t;
     }
 #pragma unroll 4
@@ -1090,10 +1091,10 @@ int run_product(const Product& given, void* scratch) {
     // Which kernel: the shorter estimate, from k-blocks times their measured cost
     // (0.35 us for a pair's 256 x 256, up to 0.42 us for a tile's 128 x 256, both
     // 128 bytes deep) and what starting and ending takes (6 us, and 4 to 9 us with
-    // the rows of the tile). Measured,
-    // pair / tile, in bf16: 256 x 4096 x 4096 28.4 / 18.9 us, 512 rows 28.4 / 24.8,
-    // 768 rows 30.2 / 33.8, 1024 rows 29.5 / 34.4; 128 x 16384 x 4096 33.8 / 31.4,
-    // 256 rows 34.6 / 41.4; 512 x 2048 x 16384 89.7 / 37.0; 2048^3 18.8 / 22.6.
+    // the rows of the tile). Measured, pair / tile, in bf16: 256 x 4096 x 4096 28.4
+    // / 18.9 us, 512 rows 28.4 / 24.8, 768 rows 30.2 / 33.8, 1024 rows 29.5 / 34.4;
+    // 128 x 16384 x 4096 33.8 / 31.4, 256 rows 34.6 / 41.4; 512 x 2048 x 16384 89.7
+    // / 37.0; 2048^3 18.8 / 22.6.
     const int pair_width = p.gated ? 128 : 256;
     const long long pair_m = ((long long)p.M + 255) / 256, pair_n = ((long long)p.N + pair_width - 1) / pair_width;
     if (pair_m * pair_n > INT32_MAX / 2 || tiles() * q.splits > INT32_MAX / 2)
