@@ -8,6 +8,8 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "ttc_internal.cuh"
 
 namespace ttc {
@@ -327,54 +329,82 @@ __device__ __forceinline__ void activate_grad(int act, float z, float& a, float&
     }
 }
 
-// The epilogue of single elements, for tensors that nothing wider can reach:
-// element (row, col) of a product, with its column's scales and bias.
-__device__ __forceinline__ float load1(int dtype, const void* base, long long i) {
-    return dtype == TTC_BF16  ? to_f32(static_cast<const __nv_bfloat16*>(base)[i])
-           : dtype == TTC_F16 ? to_f32(static_cast<const __half*>(base)[i])
-                              : static_cast<const float*>(base)[i];
-}
-__device__ __forceinline__ void store1(int dtype, void* base, long long i, float v) {
-    if (dtype == TTC_BF16)
-        static_cast<__nv_bfloat16*>(base)[i] = from_f32<__nv_bfloat16>(v);
-    else if (dtype == TTC_F16)
-        static_cast<__half*>(base)[i] = from_f32<__half>(v);
-    else
-        static_cast<float*>(base)[i] = v;
-}
-__device__ __forceinline__ void finish_one_linear(const ProductEpilogue& e, int row, int col, float v, float scale,
-                                                  float bias) {
-    if (e.row_scales) v = v * __ldg(e.row_scales + row) * scale;
-    v += bias;
-    if (e.pre) store1(e.out_dtype, e.pre, row * e.ldp + col, v);
-    v = activate(e.act, v);
-    if (e.residual) v += load1(e.out_dtype, e.residual, row * e.ldr + col);
+// The epilogue for tensors that nothing wider than an element can reach: eight
+// rows (row, row + step, ...; the first `count` exist) of one column, whose scales
+// and bias are given, a lane of a warp each of 32 neighbouring columns. Eight at a
+// time so that the residual's loads are on their way together: one row after the
+// other, 5000 x 4097 results took 460 us.
+template <int DT>
+struct Element {
+    using T = typename std::conditional<DT == TTC_F32, float,
+                                        typename std::conditional<DT == TTC_BF16, __nv_bfloat16, __half>::type>::type;
+    static __device__ __forceinline__ float load(const void* base, long long i) {
+        return to_f32<T>(static_cast<const T*>(base)[i]);
+    }
+    static __device__ __forceinline__ void store(void* base, long long i, float v) {
+        static_cast<T*>(base)[i] = from_f32<T>(v);
+    }
+};
+template <int DT, bool GATED>
+__device__ __forceinline__ void finish_column(const ProductEpilogue& e, int row, int step, int count, int col,
+                                              float (&v)[8], float (&u)[8], float s0, float s1, float bias) {
+    using E = Element<DT>;
+    auto each = [&](auto f) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < count) f(i, row + i * step);
+    };
+    float res[8];
+    if (!GATED && e.residual) each([&](int i, int r) { res[i] = E::load(e.residual, r * e.ldr + col); });
+    if (e.row_scales)
+        each([&](int i, int r) {
+            const float rs = __ldg(e.row_scales + r);
+            v[i] = v[i] * rs * s0;
+            if (GATED) u[i] = u[i] * rs * s1;
+        });
+    if (GATED) {
+        if (e.gate)
+            each([&](int i, int r) {
+                E::store(e.gate, r * e.ldp + col, v[i]);
+                E::store(e.up, r * e.ldp + col, u[i]);
+            });
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += bias;
+        if (e.pre) each([&](int i, int r) { E::store(e.pre, r * e.ldp + col, v[i]); });
+    }
+    activate_all<8>(e.act, v);
+    if (GATED) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= u[i];
+    } else if (e.residual) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += res[i];
+    }
+    if (e.split_rows > 0) {
+        each([&](int i, int r) {
+            const int second = r - e.split_rows - e.split_skip;
+            if (r < e.split_rows)
+                E::store(e.out, r * e.ldo + col, v[i]);
+            else if (second >= 0)
+                E::store(e.out2, second * e.ldo + col, v[i]);
+        });
+        return;
+    }
     void* out = e.out;
-    if (e.split_rows > 0 && row >= e.split_rows) {
-        row -= e.split_rows + e.split_skip;
-        if (row < 0) return;
-        out = e.out2;
-    } else if (e.split_cols > 0 && col >= e.split_cols) {
+    if (e.split_cols > 0 && col >= e.split_cols) {
         col -= e.split_cols + e.split_skip;
         if (col < 0) return;
         out = e.out2;
     }
-    store1(e.out_dtype, out, row * e.ldo + col, v);
+    each([&](int i, int r) { E::store(out, r * e.ldo + col, v[i]); });
 }
-__device__ __forceinline__ void finish_one_gated(const ProductEpilogue& e, int row, int col, float g, float u,
-                                                 float gscale, float uscale) {
-    if (e.row_scales) {
-        const float rs = __ldg(e.row_scales + row);
-        g = g * rs * gscale;
-        u = u * rs * uscale;
-    }
-    if (e.gate) {
-        store1(e.out_dtype, e.gate, row * e.ldp + col, g);
-        store1(e.out_dtype, e.up, row * e.ldp + col, u);
-    }
-    store1(e.out_dtype, e.out, row * e.ldo + col, activate(e.act, g) * u);
+__device__ __forceinline__ float bias_at(const ProductEpilogue& e, int col) {
+    if (!e.bias) return 0.0f;
+    return e.out_dtype == TTC_BF16  ? Element<TTC_BF16>::load(e.bias, col)
+           : e.out_dtype == TTC_F16 ? Element<TTC_F16>::load(e.bias, col)
+                                    : Element<TTC_F32>::load(e.bias, col);
 }
-
 #endif  // __CUDACC__
 
 }  // namespace ttc

@@ -388,14 +388,20 @@ __device__ __forceinline__ bool pair_epilogue(const ProductParams& q, uint8_t* s
                 if (col < p.N) {
                     const float s0 = e.row_scales ? __ldg(e.col_scales[0] + col) : 1.0f;
                     const float s1 = e.row_scales && p.gated ? __ldg(e.col_scales[1] + col) : 1.0f;
-                    const float bias = e.bias ? load1(DT, e.bias, col) : 0.0f;
+                    const float bias = bias_at(e, col);
                     const int rows = min(32, p.M - row0);
-#pragma unroll 4
-                    for (int r = 0; r < rows; ++r) {
+#pragma unroll 1
+                    for (int r = 0; r < rows; r += 8) {
+                        float v[8], u[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            v[i] = at(0, r + i);
+                            if (p.gated) u[i] = at(1, r + i);
+                        }
                         if (p.gated)
-                            finish_one_gated(e, row0 + r, col, at(0, r), at(1, r), s0, s1);
+                            finish_column<DT, true>(e, row0 + r, 1, rows - r, col, v, u, s0, s1, 0.0f);
                         else
-                            finish_one_linear(e, row0 + r, col, at(0, r), s0, bias);
+                            finish_column<DT, false>(e, row0 + r, 1, rows - r, col, v, u, s0, 1.0f, bias);
                     }
                 }
                 __syncwarp();
@@ -590,6 +596,12 @@ __device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
     return v;
 }
 
+__device__ __forceinline__ float ld_cluster1(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+
 // Four values at float index i of the tile, added over the cluster's CTAs in rank order.
 __device__ __forceinline__ float4 tile_sum4(uint32_t sbase, int splits, int i) {
     float4 t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -711,35 +723,32 @@ __device__ __forceinline__ void tile_finish(const ProductParams& q, uint32_t sba
     }
 }
 
-// The same for unaligned tensors and the last columns: a lane one column at a time.
-__device__ __noinline__ void tile_finish_scalar(const ProductParams& q, uint32_t sbase, int m0, int n0, int r0, int r1) {
-    const Product& p = q.p;
-    const ProductEpilogue& e = p.epi;
-    const int width = p.gated ? 64 : 128;
-    auto sum1 = [&](int i) {
-        float t = 0.0f;
-        for (int s = 0; s < q.splits; ++s) {
-            float v;
-            const uint32_t at = sbase + 4u * (uint32_t)i;
-            asm volatile("ld.shared::cluster.f32 %0, [%1];"
-                         : "=f"(v)
-                         : "r"(q.splits == 1 ? at : cluster_addr(at, s))
-                         : "memory");
-            t += v;
+// The same for unaligned tensors and the last columns: a lane a column, eight
+// rows at a time. Eight of the warps share the tile: four (gated: two) side by
+// side, the others on the rows between.
+template <int DT, bool GATED>
+__device__ __noinline__ void tile_finish_columns(const ProductParams& q, uint32_t sbase, int m0, int n0, int r0, int r1) {
+    constexpr int kAcross = GATED ? 2 : 4, kStep = 8 / kAcross;
+    const ProductEpilogue& e = q.p.epi;
+    const int warp = threadIdx.x >> 5, c = (warp % kAcross) * 32 + (threadIdx.x & 31), col = n0 + c;
+    if (warp >= 8 || col >= q.p.N) return;
+    const float s0 = e.row_scales ? __ldg(e.col_scales[0] + col) : 1.0f;
+    const float s1 = GATED && e.row_scales ? __ldg(e.col_scales[1] + col) : 1.0f;
+    const float bias = bias_at(e, col);
+#pragma unroll 1
+    for (int r = r0 + warp / kAcross; r < r1; r += 8 * kStep) {
+        const int count = min(8, (r1 - r + kStep - 1) / kStep);
+        float v[8] = {}, u[8] = {};
+        for (int s = 0; s < q.splits; ++s) {  // the cluster's shares in rank order
+            const uint32_t from = (q.splits == 1 ? sbase : cluster_addr(sbase, s)) + 4u * (uint32_t)(r * 128 + c);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < count) {
+                    v[i] += ld_cluster1(from + 4u * (uint32_t)(i * kStep * 128));
+                    if (GATED) u[i] += ld_cluster1(from + 4u * (uint32_t)(i * kStep * 128 + 64));
+                }
         }
-        return t;
-    };
-    // kThreads is a multiple of neither width, so columns change from row to row
-#pragma unroll 2
-    for (int it = threadIdx.x; it < (r1 - r0) * width; it += kThreads) {
-        const int r = r0 + it / width, c = it % width, col = n0 + c, row = m0 + r;
-        if (col >= p.N) continue;
-        const float s0 = e.row_scales ? __ldg(e.col_scales[0] + col) : 1.0f;
-        if (p.gated)
-            finish_one_gated(e, row, col, sum1(r * 128 + c), sum1(r * 128 + 64 + c), s0,
-                             e.row_scales ? __ldg(e.col_scales[1] + col) : 1.0f);
-        else
-            finish_one_linear(e, row, col, sum1(r * 128 + c), s0, e.bias ? load1(e.out_dtype, e.bias, col) : 0.0f);
+        finish_column<DT, GATED>(e, m0 + r, kStep, count, col, v, u, s0, s1, bias);
     }
 }
 
@@ -880,17 +889,25 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ 
     const int share = (rows + splits - 1) / splits;  // rows that this CTA finishes
     const int r0 = split * share, r1 = min(rows, r0 + share);
     const bool seam = p.epi.split_cols > 0 && n0 < p.epi.split_cols + p.epi.split_skip && n0 + 128 > p.epi.split_cols;
-    if (!p.epi.vec || seam || n0 + (p.gated ? 64 : 128) > p.N)
-        tile_finish_scalar(q, sbase, m0, n0, r0, r1);
-    else if (p.epi.out_dtype == TTC_BF16)
-        p.gated ? tile_finish<TTC_BF16, true>(q, sbase, m0, n0, r0, r1)
-                : tile_finish<TTC_BF16, false>(q, sbase, m0, n0, r0, r1);
+    const bool columns = !p.epi.vec || seam || n0 + (p.gated ? 64 : 128) > p.N;
+    auto finish = [&](auto dt, auto gated) {
+        if (columns)
+            tile_finish_columns<dt(), gated()>(q, sbase, m0, n0, r0, r1);
+        else
+            tile_finish<dt(), gated()>(q, sbase, m0, n0, r0, r1);
+    };
+    auto typed = [&](auto dt) {
+        if (p.gated)
+            finish(dt, std::true_type());
+        else
+            finish(dt, std::false_type());
+    };
+    if (p.epi.out_dtype == TTC_BF16)
+        typed(std::integral_constant<int, TTC_BF16>());
     else if (p.epi.out_dtype == TTC_F16)
-        p.gated ? tile_finish<TTC_F16, true>(q, sbase, m0, n0, r0, r1)
-                : tile_finish<TTC_F16, false>(q, sbase, m0, n0, r0, r1);
+        typed(std::integral_constant<int, TTC_F16>());
     else
-        p.gated ? tile_finish<TTC_F32, true>(q, sbase, m0, n0, r0, r1)
-                : tile_finish<TTC_F32, false>(q, sbase, m0, n0, r0, r1);
+        typed(std::integral_constant<int, TTC_F32>());
     if (splits > 1) {  // nobody leaves while its shared memory is still read
         __syncwarp();
         cluster_sync();
@@ -903,19 +920,52 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ 
 bool aligned16(const Operand& o, int es) { return (uintptr_t)o.ptr % 16 == 0 && (o.ld * es) % 16 == 0; }
 
 struct Copy {
-    const void* src;
-    void* dst;
-    long long rows, cols, lds, ldd;
+    const uint8_t* src;
+    uint8_t* dst;
+    long long src_pitch, dst_pitch;  // bytes
+    unsigned rows, segments;         // segments of kSegment bytes a row
+    int bytes;                       // of a row
 };
+struct Copies {
+    Copy c[4];
+    int n;
+    unsigned blocks;  // segments of all rows of all copies
+};
+constexpr int kSegment = 4096;  // 256 threads, four words each
 
-template <class T>
-__global__ void __launch_bounds__(256) pad_rows_kernel(const __grid_constant__ Copy c) {
+// A block a segment of a row, in 32-bit words: a word that starts inside a source
+// word is put together from two, so that a row is read and written in whole lines
+// wherever it starts. The first and last words of a row go byte by byte: nothing
+// outside the row is read.
+__global__ void __launch_bounds__(256) pad_rows_kernel(const __grid_constant__ Copies all) {
     grid_wait();
     grid_trigger();
-    for (long long r = blockIdx.x; r < c.rows; r += gridDim.x) {
-        const T* s = static_cast<const T*>(c.src) + r * c.lds;
-        T* d = static_cast<T*>(c.dst) + r * c.ldd;
-        for (long long i = threadIdx.x; i < c.cols; i += 256) d[i] = s[i];
+    for (unsigned b = blockIdx.x; b < all.blocks; b += gridDim.x) {
+        unsigned k = b;
+        int which = 0;
+        while (k >= all.c[which].rows * all.c[which].segments) k -= all.c[which].rows * all.c[which].segments, ++which;
+        const Copy& c = all.c[which];
+        const unsigned row = k / c.segments;
+        const uint8_t* src = c.src + row * c.src_pitch;
+        uint8_t* dst = c.dst + row * c.dst_pitch;
+        const int first = (int)(k - row * c.segments) * kSegment + threadIdx.x * 4;
+        const int off = (int)((uintptr_t)src & 3);
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int at = first + i * 1024;
+            w[i] = 0;
+            if (at >= c.bytes) continue;
+            if (at > 0 && at + 8 <= c.bytes) {
+                const uint32_t* p = reinterpret_cast<const uint32_t*>(src + at - off);
+                w[i] = off ? __funnelshift_r(p[0], p[1], 8 * off) : p[0];
+            } else {
+                for (int j = 0; j < 4 && at + j < c.bytes; ++j) w[i] |= (uint32_t)src[at + j] << (8 * j);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (first + i * 1024 < c.bytes) *reinterpret_cast<uint32_t*>(dst + first + i * 1024) = w[i];
     }
 }
 
@@ -1051,16 +1101,26 @@ int run_product(const Product& given, void* scratch) {
     Stored s[4];
     const int n = stored_operands(p, s);
     char* room = (char*)scratch;
+    Copies copies = {};
+    long long segments = 0;
     for (int i = 0; i < n; ++i) {
         if (aligned16(*s[i].o, es)) continue;
         Operand& o = const_cast<Operand&>(*s[i].o);
-        const Copy c{o.ptr, room, s[i].rows, s[i].cols, o.ld, padded_ld(s[i].cols, es)};
-        const unsigned grid = (unsigned)std::min<long long>(c.rows, 16ll * sms);
+        const long long ldd = padded_ld(s[i].cols, es);
+        Copy& c = copies.c[copies.n++];
+        const int bytes = (int)s[i].cols * es;
+        c = {(const uint8_t*)o.ptr, (uint8_t*)room, o.ld * es, ldd * es, (unsigned)s[i].rows,
+             (unsigned)((bytes + kSegment - 1) / kSegment), bytes};
+        segments += (long long)c.rows * c.segments;
+        o = {room, ldd};
+        room += align256((size_t)s[i].rows * ldd * es);
+    }
+    if (copies.n) {
         count_launch();
-        if (int rc = launch_overlapped(f8 ? pad_rows_kernel<uint8_t> : pad_rows_kernel<uint16_t>, dim3(grid), 256, c))
-            return rc;
-        o = {room, c.ldd};
-        room += align256((size_t)c.rows * c.ldd * es);
+        if (segments > INT32_MAX) return set_error(TTC_ERR_UNSUPPORTED, "tt_cuda: unaligned operands are too large");
+        copies.blocks = (unsigned)segments;
+        const dim3 grid((unsigned)std::min<long long>(segments, 64ll * sms));
+        if (int rc = launch_overlapped(pad_rows_kernel, grid, 256, copies)) return rc;
     }
     const int bk = kRow / es;
     q.kb_seg = (p.K + bk - 1) / bk;
