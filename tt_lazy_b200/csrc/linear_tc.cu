@@ -170,7 +170,7 @@ __device__ __forceinline__ void pair_coords(int tile, int m_tiles, int n_tiles, 
 }
 
 // The epilogue warps' part; true when a wait ran out.
-template <int DT>
+template <int DT, bool GATED>
 __device__ __forceinline__ bool pair_epilogue(const ProductParams& q, uint8_t* staging, uint32_t tmem_base,
                                               uint32_t bar0, uint32_t rank) {
     constexpr int W = kRow / (DT == TTC_F32 ? 4 : 2);  // columns of a chunk
@@ -181,7 +181,7 @@ __device__ __forceinline__ bool pair_epilogue(const ProductParams& q, uint8_t* s
     const int quarter = (w + 2) & 3, which = w >> 2;  // quarter of the tensor-memory lanes; which of its two warps
     uint8_t* const mine = staging + w * 2 * kBuffer;
     const uint32_t mine_addr = smem_u32(mine), res_bar = bar0 + 8u * (2 * kStages + 4 + 2 * w);
-    const int tile_cols = p.gated ? 128 : 256, chunks = tile_cols / W;
+    const int tile_cols = GATED ? 128 : 256, chunks = tile_cols / W;
     const int num_tiles = q.m_tiles * q.n_tiles, nclusters = gridDim.x >> 1;
     uint32_t res_phase = 0, res_pending = 0;  // a bit a buffer
     int seq = 0;             // chunks sent so far: the next one goes through buffer seq & 1
@@ -294,7 +294,7 @@ __device__ __forceinline__ bool pair_epilogue(const ProductParams& q, uint8_t* s
                 continue;
             }
             if (by_tma(row0, first)) {
-                if (p.gated) {
+                if constexpr (GATED) {
                     if (e.gate) {
                         for (int k = 0; k < 2; ++k) {
                             free_buffer();
@@ -375,7 +375,7 @@ __device__ __forceinline__ bool pair_epilogue(const ProductParams& q, uint8_t* s
             __syncwarp();
             for (int h = 0; h < W / 32; ++h) {
                 const int col = first + h * 32 + lane;
-                for (int k = 0; k < (p.gated ? 2 : 1); ++k) {
+                for (int k = 0; k < (GATED ? 2 : 1); ++k) {
                     float v[32];
                     columns32(k * 128 + c * W + h * 32, v);
 #pragma unroll
@@ -389,7 +389,7 @@ __device__ __forceinline__ bool pair_epilogue(const ProductParams& q, uint8_t* s
                 };
                 if (col < p.N) {
                     const float s0 = e.row_scales ? __ldg(e.col_scales[0] + col) : 1.0f;
-                    const float s1 = e.row_scales && p.gated ? __ldg(e.col_scales[1] + col) : 1.0f;
+                    const float s1 = e.row_scales && GATED ? __ldg(e.col_scales[1] + col) : 1.0f;
                     const float bias = bias_at(e, col);
                     const int rows = min(32, p.M - row0);
 #pragma unroll 1
@@ -398,9 +398,9 @@ __device__ __forceinline__ bool pair_epilogue(const ProductParams& q, uint8_t* s
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
                             v[i] = at(0, r + i);
-                            if (p.gated) u[i] = at(1, r + i);
+                            if (GATED) u[i] = at(1, r + i);
                         }
-                        if (p.gated)
+                        if (GATED)
                             finish_column<DT, true>(e, row0 + r, 1, rows - r, col, v, u, s0, s1, 0.0f);
                         else
                             finish_column<DT, false>(e, row0 + r, 1, rows - r, col, v, u, s0, 1.0f, bias);
@@ -427,7 +427,7 @@ __device__ __forceinline__ bool pair_epilogue(const ProductParams& q, uint8_t* s
 // arithmetic 7 more.) Chunks that TMA cannot write (unaligned tensors, the
 // seam of a split output, the last columns of a biased or scaled one or of a
 // width that is no multiple of 16 bytes) go element by element, a column a lane.
-template <bool F8>
+template <bool F8, bool GATED, int DT>
 __global__ void __launch_bounds__(kThreads, 1) pair_kernel(const __grid_constant__ ProductParams q) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -484,7 +484,7 @@ __global__ void __launch_bounds__(kThreads, 1) pair_kernel(const __grid_constant
                 int mt, nt;
                 pair_coords(tile, q.m_tiles, q.n_tiles, mt, nt);
                 const int row0 = mt * 256 + (int)rank * 128;
-                const int col0 = p.gated ? nt * 128 : nt * 256 + (int)rank * 128;
+                const int col0 = GATED ? nt * 128 : nt * 256 + (int)rank * 128;
                 for (int kb = 0; kb < q.kb_total; ++kb) {
                     if (!mbar_wait(empty_bar(stage), phase ^ 1, q.wait_limit)) {
                         failed = true;
@@ -494,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, 1) pair_kernel(const __grid_constant
                     mbar_arrive_expect_tx(full_bar(stage), kStageBytes);
                     const uint32_t a_dst = sbase + stage * kStageBytes;
                     load_rows(a_dst, &q.a[seg], full_bar(stage), p.a_mn, k, bk, row0, 128);
-                    load_rows(a_dst + kHalf, &q.b[p.gated ? rank : seg], full_bar(stage), p.b_mn, k, bk, col0, 128);
+                    load_rows(a_dst + kHalf, &q.b[GATED ? rank : seg], full_bar(stage), p.b_mn, k, bk, col0, 128);
                     ++issued;
                     if (++stage == kStages) {
                         stage = 0;
@@ -565,12 +565,7 @@ __global__ void __launch_bounds__(kThreads, 1) pair_kernel(const __grid_constant
             }
         }
     } else {
-        if (p.epi.out_dtype == TTC_BF16)
-            failed = pair_epilogue<TTC_BF16>(q, staging, tmem_base, bar0, rank);
-        else if (p.epi.out_dtype == TTC_F16)
-            failed = pair_epilogue<TTC_F16>(q, staging, tmem_base, bar0, rank);
-        else
-            failed = pair_epilogue<TTC_F32>(q, staging, tmem_base, bar0, rank);
+        failed = pair_epilogue<DT, GATED>(q, staging, tmem_base, bar0, rank);
     }
 
     if (failed) *(volatile int*)q.status = 1;
@@ -1032,8 +1027,9 @@ bool first_on_device(bool (&seen)[kMaxDevices]) {
     return first;
 }
 
-template <bool F8>
-int launch_pair(ProductParams& q) {
+template <bool F8, bool GATED, int DT>
+int launch_pair_as(ProductParams& q) {
+    auto kernel = pair_kernel<F8, GATED, DT>;
     static bool seen[kMaxDevices] = {};
     static int most[kMaxDevices] = {};
     cudaLaunchConfig_t cfg;
@@ -1046,18 +1042,32 @@ int launch_pair(ProductParams& q) {
     cfg.stream = rt().stream;
     int& clusters = most[rt().device];
     if (first_on_device(seen)) {
-        TTC_CUDA(cudaFuncSetAttribute(pair_kernel<F8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
+        TTC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
         cfg.gridDim = dim3(2 * (rt().sm_count / 2), 1, 1);
-        if (cudaOccupancyMaxActiveClusters(&clusters, pair_kernel<F8>, &cfg) != cudaSuccess || clusters < 1) {
+        if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess || clusters < 1) {
             cudaGetLastError();
             clusters = rt().sm_count / 2;
         }
     }
     const long long tiles = (long long)q.m_tiles * q.n_tiles;
     cfg.gridDim = dim3(2u * (unsigned)std::min<long long>(tiles, clusters), 1, 1);
-    TTC_CUDA(cudaLaunchKernelEx(&cfg, pair_kernel<F8>, q));
+    TTC_CUDA(cudaLaunchKernelEx(&cfg, kernel, q));
     count_launch();
     return TTC_OK;
+}
+
+// An instantiation for each kind of epilogue: the kernel's speed at small K is that
+// of fetching the epilogue's instructions.
+template <bool F8>
+int launch_pair(ProductParams& q) {
+    auto typed = [&](auto gated) {
+        switch (q.p.epi.out_dtype) {
+            case TTC_BF16: return launch_pair_as<F8, gated(), TTC_BF16>(q);
+            case TTC_F16: return launch_pair_as<F8, gated(), TTC_F16>(q);
+            default: return launch_pair_as<F8, gated(), TTC_F32>(q);
+        }
+    };
+    return q.p.gated ? typed(std::true_type()) : typed(std::false_type());
 }
 
 template <bool F8>
