@@ -337,8 +337,9 @@ int ttc_gemm_select_path(const ttc_gemm_desc* desc);
  *
  * Layout. Matrices are row-major with a leading dimension in elements. With
  * trans_w = 0 a weight is stored [K, N] as for ttc_gemm, with trans_w = 1
- * [N, K]; E4M3 weights have trans_w = 1. Any size, leading dimension and
- * element-aligned address is accepted. A matrix operand of a product whose
+ * [N, K]; E4M3 weights have trans_w = 1. Any leading dimension and element-
+ * aligned address is accepted, and any size up to 2^30 rows and a width (N, K) of
+ * 2^23. A matrix operand of a product whose
  * address or row pitch is not a multiple of 16 bytes is first copied into the
  * workspace with padded rows.
  *
@@ -377,8 +378,8 @@ typedef enum {
  * `hidden` and `y` may be `x` or `residual` themselves (same address and
  * leading dimension, same type); no other overlap is allowed. */
 typedef struct {
-    int64_t rows;
-    int32_t cols; /* >= 1 */
+    int64_t rows; /* below 2^31 */
+    int32_t cols; /* 1 to 2^30 */
     int32_t dtype, weight_dtype, y_dtype; /* weight_dtype: dtype or F32 */
     float eps;                            /* >= 0 */
     const void* x; int64_t ldx;
@@ -396,7 +397,7 @@ int ttc_rms_norm(const ttc_rms_norm_desc* desc);
  *   dweight[c] = sum_r dy(r, c) hidden(r, c) rstd(r)
  * dhidden, optional, is the gradient that reaches `hidden` by another way (the
  * residual stream); dx is then the gradient of both x and residual. dx may be
- * dy or dhidden themselves. */
+ * dy or dhidden themselves (same address and leading dimension). */
 typedef struct {
     int64_t rows;
     int32_t cols;
@@ -416,7 +417,8 @@ int ttc_rms_norm_backward_workspace(const ttc_rms_norm_backward_desc* desc, size
 /* y [M, N] = act(x [M, K] W + bias) + residual. With dtype E4M3 the product is
  * scaled before the bias: x_scales[m] * w_scales[n] * (x W)(m, n).
  * y, bias, residual and pre have y_dtype: dtype or F32 for 16-bit operands;
- * F16, BF16 or F32 for E4M3. y may be `residual` itself. */
+ * F16, BF16 or F32 for E4M3. y may be `residual` itself (same address and leading
+ * dimension); no other overlap is allowed. */
 typedef struct {
     int32_t M, N, K; /* M >= 0, N >= 1, K >= 1 */
     int32_t dtype, y_dtype, trans_w, act;

@@ -133,6 +133,18 @@ def test_workspace_that_is_missing_short_or_misaligned_is_refused(desc):
         assert b"workspace" in L.ttc_last_error()
 
 
+def test_norm_rows_whose_column_index_could_pass_32_bits_are_refused():
+    L, n, widest = capi.lib(), C.c_size_t(), 1 << 30
+    for cols in (widest + 1, (1 << 31) - 1):
+        desc = norm(cols=cols, ldx=cols, ldy=cols)
+        assert L.ttc_rms_norm(C.byref(desc)) == UNSUPPORTED
+        assert b"columns" in L.ttc_last_error()
+        desc = norm_backward(cols=cols, lddy=cols, ldh=cols, lddx=cols)
+        for rc in (L.ttc_rms_norm_backward(C.byref(desc)), L.ttc_rms_norm_backward_workspace(C.byref(desc), C.byref(n))):
+            assert rc == UNSUPPORTED and b"columns" in L.ttc_last_error()
+    assert capi.workspace_size(norm_backward(cols=widest, lddy=widest, ldh=widest, lddx=widest)) >= 4 * widest
+
+
 def test_null_descriptors_are_refused():
     L = capi.lib()
     n = C.c_size_t()

@@ -139,6 +139,9 @@ int launch_overlapped(void (*kernel)(Params...), dim3 grid, int block, const Arg
 
 // Waits until the kernels before this one in the stream have finished and their
 // writes are visible; lets the kernel after this one start to be launched.
+// Kernels that begin with it read what those wrote with plain loads: the
+// read-only path (__ldg) is for memory that nobody writes while a kernel runs, and
+// the compiler may move its loads above the wait.
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
@@ -358,7 +361,7 @@ __device__ __forceinline__ void finish_column(const ProductEpilogue& e, int row,
     if (!GATED && e.residual) each([&](int i, int r) { res[i] = E::load(e.residual, r * e.ldr + col); });
     if (e.row_scales)
         each([&](int i, int r) {
-            const float rs = __ldg(e.row_scales + r);
+            const float rs = e.row_scales[r];
             v[i] = v[i] * rs * s0;
             if (GATED) u[i] = u[i] * rs * s1;
         });

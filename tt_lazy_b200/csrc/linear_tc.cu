@@ -238,7 +238,7 @@ __device__ __forceinline__ bool pair_epilogue(const ProductParams& q, uint8_t* s
             return leave(true);
         tc_fence_after();
         const uint32_t acc = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(b * 256);
-        const float row_scale = e.row_scales && row < p.M ? __ldg(e.row_scales + row) : 1.0f;
+        const float row_scale = e.row_scales && row < p.M ? e.row_scales[row] : 1.0f;
         auto columns32 = [&](int c, float (&v)[32]) {
             uint32_t r[32];
             tc_ld_32x32b_x32(acc + c, r);
@@ -249,7 +249,7 @@ __device__ __forceinline__ bool pair_epilogue(const ProductParams& q, uint8_t* s
         auto scale32 = [&](const float* scales, int col, float (&v)[32]) {
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
-                const float4 s = __ldg(reinterpret_cast<const float4*>(scales + col + i));
+                const float4 s = *reinterpret_cast<const float4*>(scales + col + i);
                 v[i] = v[i] * row_scale * s.x;
                 v[i + 1] = v[i + 1] * row_scale * s.y;
                 v[i + 2] = v[i + 2] * row_scale * s.z;
@@ -264,7 +264,7 @@ __device__ __forceinline__ bool pair_epilogue(const ProductParams& q, uint8_t* s
                 const uint4* bias = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(e.bias) +
                                                                    (long long)(col0 + c) * (16 / G));
 #pragma unroll
-                for (int i = 0; i < 32 / G; ++i) add16<DT>(__ldg(bias + i), v + i * G);
+                for (int i = 0; i < 32 / G; ++i) add16<DT>(bias[i], v + i * G);
             }
         };
         auto put32 = [&](int buffer, int h, const float (&v)[32]) {
@@ -388,8 +388,8 @@ __device__ __forceinline__ bool pair_epilogue(const ProductParams& q, uint8_t* s
                                                            (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
                 };
                 if (col < p.N) {
-                    const float s0 = e.row_scales ? __ldg(e.col_scales[0] + col) : 1.0f;
-                    const float s1 = e.row_scales && GATED ? __ldg(e.col_scales[1] + col) : 1.0f;
+                    const float s0 = e.row_scales ? e.col_scales[0][col] : 1.0f;
+                    const float s1 = e.row_scales && GATED ? e.col_scales[1][col] : 1.0f;
                     const float bias = bias_at(e, col);
                     const int rows = min(32, p.M - row0);
 #pragma unroll 1
@@ -406,6 +406,7 @@ __device__ __forceinline__ bool pair_epilogue(const ProductParams& q, uint8_t* s
                             finish_column<DT, false>(e, row0 + r, 1, rows - r, col, v, u, s0, 1.0f, bias);
                     }
                 }
+                fence_async_smem();  // TMA may write the buffers next
                 __syncwarp();
             }
         }
@@ -659,8 +660,8 @@ __device__ __forceinline__ void tile_finish(const ProductParams& q, uint32_t sba
     constexpr int kAhead = 4;
     float4 s0 = make_float4(1, 1, 1, 1), s1 = s0, bias = make_float4(0, 0, 0, 0);
     if (e.row_scales) {
-        s0 = __ldg(reinterpret_cast<const float4*>(e.col_scales[0] + col));
-        if (GATED) s1 = __ldg(reinterpret_cast<const float4*>(e.col_scales[1] + col));
+        s0 = *reinterpret_cast<const float4*>(e.col_scales[0] + col);
+        if (GATED) s1 = *reinterpret_cast<const float4*>(e.col_scales[1] + col);
     }
     if (e.bias) bias = Four<DT>::load(e.bias, col);
     for (int r = r0 + (GATED ? 2 * warp + (lane >> 4) : warp); r < r1; r += kAhead * kStep) {
@@ -677,7 +678,7 @@ __device__ __forceinline__ void tile_finish(const ProductParams& q, uint32_t sba
         if (GATED) each([&](int a, int row) { get(u[a], tile_sum4(sbase, q.splits, (row - m0) * 128 + 64 + 4 * j)); });
         if (e.row_scales)
             each([&](int a, int row) {
-                const float rs = __ldg(e.row_scales + row);
+                const float rs = e.row_scales[row];
                 v[a][0] *= rs * s0.x, v[a][1] *= rs * s0.y, v[a][2] *= rs * s0.z, v[a][3] *= rs * s0.w;
                 if (GATED) u[a][0] *= rs * s1.x, u[a][1] *= rs * s1.y, u[a][2] *= rs * s1.z, u[a][3] *= rs * s1.w;
             });
@@ -729,8 +730,8 @@ __device__ __noinline__ void tile_finish_columns(const ProductParams& q, uint32_
     const ProductEpilogue& e = q.p.epi;
     const int warp = threadIdx.x >> 5, c = (warp % kAcross) * 32 + (threadIdx.x & 31), col = n0 + c;
     if (warp >= 8 || col >= q.p.N) return;
-    const float s0 = e.row_scales ? __ldg(e.col_scales[0] + col) : 1.0f;
-    const float s1 = GATED && e.row_scales ? __ldg(e.col_scales[1] + col) : 1.0f;
+    const float s0 = e.row_scales ? e.col_scales[0][col] : 1.0f;
+    const float s1 = GATED && e.row_scales ? e.col_scales[1][col] : 1.0f;
     const float bias = bias_at(e, col);
 #pragma unroll 1
     for (int r = r0 + warp / kAcross; r < r1; r += 8 * kStep) {

@@ -601,11 +601,15 @@ __global__ void __launch_bounds__(1024) sum_partials_kernel(const float* partial
         static_cast<float*>(out)[c] = s;
 }
 
+constexpr int kMaxCols = 1 << 30;
+
 int check_norm_types(const char* op, int dtype, int weight_dtype, long long rows, int cols, float eps) {
     if (rows < 0 || cols < 1)
         return set_error(TTC_ERR_INVALID_ARGUMENT, "tt_cuda: %s: shape %lld x %d", op, rows, cols);
     if (rows > INT32_MAX)
         return set_error(TTC_ERR_UNSUPPORTED, "tt_cuda: %s: %lld rows exceed %d", op, rows, INT32_MAX);
+    if (cols > kMaxCols)  // column indices that step past the end of a row stay inside 32 bits
+        return set_error(TTC_ERR_UNSUPPORTED, "tt_cuda: %s: %d columns exceed %d", op, cols, kMaxCols);
     if (dtype != TTC_F32 && dtype != TTC_F16 && dtype != TTC_BF16)
         return set_error(TTC_ERR_INVALID_ARGUMENT, "tt_cuda: %s: dtype %d is not F32, F16 or BF16", op, dtype);
     if (weight_dtype != dtype && weight_dtype != TTC_F32)
