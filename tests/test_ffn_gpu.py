@@ -489,6 +489,56 @@ def test_linear_backward_parts(lib, wanted):
         assert torch.equal(part[k].t, whole[k].t if k == wanted else torch.full_like(part[k].t, 9.0)), k
 
 
+@pytest.mark.parametrize("M,N,K,trans_w", [(512, 1024, 128, True), (300, 1032, 200, False), (33, 4096, 520, True),
+                                           (700, 129, 1001, False), (16, 72, 2056, True)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_gradients_alone_equal_those_of_the_whole_call(lib, M, N, K, trans_w, gated):
+    """Whichever products share a launch, a gradient's sums are the same."""
+    g = gen(M + N + K)
+    x, ws, _, _, _, _ = product_inputs(g, M, N, K, "bf16", trans_w, 0, 0, ("wg", "wu") if gated else ("w",))
+    dy, gate, up = (Mat(M, N, "bf16", fill=rand(g, M, N)) for _ in range(3))
+    shape = (N, K) if trans_w else (K, N)
+
+    def call(want_dx, want_dw):
+        dx = Mat(M, K, "bf16") if want_dx else None
+        dws = [Mat(*shape, "bf16") for _ in ws] if want_dw else [None for _ in ws]
+        kw = dict(dx=ptr(dx), lddx=K, lddw=shape[1])
+        if gated:
+            d = lib.gated_linear_backward_desc(M, N, K, dy.ptr, N, x.ptr, K, ws[0].ptr, ws[1].ptr, shape[1], gate.ptr,
+                                               up.ptr, N, lib.BF16, trans_w=trans_w, act=lib.ACT_SILU,
+                                               dwg=ptr(dws[0]), dwu=ptr(dws[1]), **kw)
+            lib.gated_linear_backward(d, scratch(lib, d))
+        else:
+            d = lib.linear_backward_desc(M, N, K, dy.ptr, N, x.ptr, K, ws[0].ptr, shape[1], lib.BF16, trans_w=trans_w,
+                                         act=lib.ACT_NONE, dw=ptr(dws[0]), **kw)
+            lib.linear_backward(d, scratch(lib, d))
+        return dx, dws
+
+    dx, dws = call(True, True)
+    alone, _ = call(True, False)
+    assert torch.equal(dx.t, alone.t)
+    _, alone = call(False, True)
+    for a, b in zip(dws, alone):
+        assert torch.equal(a.t, b.t)
+
+
+@pytest.mark.parametrize("M", [1, 7, 64, 65, 130, 449, 512, 513, 1000, 16385])
+@pytest.mark.parametrize("N,act", [(1, "none"), (259, "gelu"), (2048, "relu")])
+def test_bias_gradient_over_bands_of_rows(lib, M, N, act):
+    """Row counts around those where the column sums change hands: whole numbers, so exact in any order."""
+    g = gen(M + N)
+    vals = torch.randint(-3, 4, (M, N), generator=g, device=g.device).to(torch.float32)
+    dy = Mat(M, N, "f16", fill=vals)
+    pre = Mat(M, N, "f16", fill=torch.where(torch.rand(M, N, generator=g, device=g.device) < 0.5, 100.0, -100.0))
+    db = Mat(1, N, "f16")
+    d = lib.linear_backward_desc(M, N, 8, dy.ptr, N, None, 8, None, 8, lib.F16, trans_w=True,
+                                 act=lib.ACTIVATIONS[act], pre=pre.ptr if act != "none" else None, ldp=N, dbias=db.ptr)
+    lib.linear_backward(d, scratch(lib, d))
+    on = torch.ones_like(vals) if act == "none" else (pre.t > 0).float()  # the slope at +-100 is 1 or 0
+    assert torch.equal(db.t[0], (vals * on).sum(0).to(torch.float16))
+    assert db.untouched_outside()
+
+
 @pytest.mark.parametrize("M,N,K", SHAPES)
 @pytest.mark.parametrize("dtype,trans_w", [("bf16", False), ("bf16", True), ("f16", False)])
 @pytest.mark.parametrize("form", ["plain", "odd"])

@@ -100,10 +100,11 @@ struct Product {
     Operand a[2], b[2];
     ProductEpilogue epi;
 };
-// Runs it on the library stream. `scratch` (256-byte aligned) holds the padded
-// copies of operands that cannot be read in place, of product_scratch() bytes.
-int run_product(const Product& p, void* scratch);
-size_t product_scratch(const Product& p);
+// Runs one product, or two of one 16-bit type that do not depend on one another, on
+// the library stream. `scratch` (256-byte aligned) holds the padded copies of
+// operands that cannot be read in place, of product_scratch() bytes.
+int run_products(const Product* products, int count, void* scratch);
+size_t product_scratch(const Product* products, int count);
 
 // The attribute of a launch in clusters; returns the number of attributes (0 or 1).
 inline int cluster_attribute(cudaLaunchAttribute& attr, int cluster) {
@@ -124,16 +125,16 @@ inline int launch_attributes(cudaLaunchAttribute (&attr)[2], int cluster) {
 
 #ifdef __CUDACC__
 
-// Launches a kernel without clusters that way, on the library stream.
+// Launches a kernel that way, on the library stream.
 template <class... Params, class... Args>
-int launch_overlapped(void (*kernel)(Params...), dim3 grid, int block, const Args&... args) {
+int launch_overlapped(void (*kernel)(Params...), dim3 grid, int block, int cluster, const Args&... args) {
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
     cfg.gridDim = grid;
     cfg.blockDim = dim3((unsigned)block);
     cfg.stream = rt().stream;
     cfg.attrs = attr;
-    cfg.numAttrs = launch_attributes(attr, 1);
+    cfg.numAttrs = launch_attributes(attr, cluster);
     return check_cuda(cudaLaunchKernelEx(&cfg, kernel, args...), "kernel launch");
 }
 

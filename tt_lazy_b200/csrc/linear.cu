@@ -7,6 +7,7 @@
 #include <type_traits>
 
 #include "ffn.cuh"
+#include "tc_util.cuh"
 
 namespace ttc {
 namespace {
@@ -129,6 +130,7 @@ constexpr int kStripe = 256, kBandWarps = 8;
 // Rows of a block: 64, more when that would make over 256 bands of partial sums.
 int band_rows(int M) { return std::max(64, (M + 255) / 256); }
 int bands(int M) { return (M + band_rows(M) - 1) / band_rows(M); }
+constexpr int kClusterBands = 8;  // up to so many bands are a cluster: dbias needs no second launch
 
 struct LinearGradParams {
     int M, N, band_rows;
@@ -137,6 +139,7 @@ struct LinearGradParams {
     void* dz;  // or NULL: only the column sums
     long long lddz;
     float* partials;  // [bands, N] column sums of dz, or NULL
+    void* dbias;      // [N], or NULL: the bands of a stripe are one cluster, which adds them up itself
     bool vec_dy, vec_pre, vec_dz;
 };
 
@@ -183,18 +186,33 @@ __global__ void __launch_bounds__(32 * kBandWarps, 4) linear_grad_kernel(const _
             for (int i = 0; i < 8; ++i) sum[i] += g[i];
         }
     }
-    if (!p.partials) return;
+    if (!p.partials && !p.dbias) return;
     __shared__ float part[kBandWarps][kStripe];
 #pragma unroll
     for (int i = 0; i < 8; ++i) part[warp][lane * 8 + i] = sum[i];
     __syncthreads();
     const int c = blockIdx.y * kStripe + threadIdx.x;
-    if (c < p.N) {
-        float s = 0.0f;
+    float s = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kBandWarps; ++w) s += part[w][threadIdx.x];
-        p.partials[(long long)blockIdx.x * p.N + c] = s;
+    for (int w = 0; w < kBandWarps; ++w) s += part[w][threadIdx.x];
+    if (!p.dbias) {
+        if (c < p.N) p.partials[(long long)blockIdx.x * p.N + c] = s;
+        return;
     }
+    if (gridDim.x > 1) {
+        part[0][threadIdx.x] = s;  // this thread's own column
+        cluster_sync();
+        if (blockIdx.x == 0) {
+            const uint32_t at = smem_u32(&part[0][threadIdx.x]);
+            for (int b = 1; b < (int)gridDim.x; ++b) {
+                float v;
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr(at, b)) : "memory");
+                s += v;
+            }
+        }
+        cluster_sync();  // nobody leaves while its shared memory is still read
+    }
+    if (blockIdx.x == 0 && c < p.N) static_cast<T*>(p.dbias)[c] = from_f32<T>(s);
 }
 
 struct GatedGradParams {
@@ -381,14 +399,16 @@ int plan_linear_backward(const ttc_linear_backward_desc& d, void* ws, size_t* by
     void* scratch = c.base ? c.base + c.used : nullptr;
     // dx [M, K] = dz [M, N] W^T: the sum runs over N, which is contiguous in a
     // weight stored [K, N] and strided in one stored [N, K].
-    Product px = grad_product(d.M, d.K, d.N, d.dtype, dz, false, {d.w, d.ldw}, d.trans_w, d.dx, d.lddx);
+    Product products[2];
+    int count = 0;
+    if (d.dx)
+        products[count++] = grad_product(d.M, d.K, d.N, d.dtype, dz, false, {d.w, d.ldw}, d.trans_w, d.dx, d.lddx);
     // dw [K, N] = x^T dz, or [N, K] = dz^T x; the sum runs over the rows.
-    Product pw = d.trans_w ? grad_product(d.N, d.K, d.M, d.dtype, dz, true, {d.x, d.ldx}, true, d.dw, d.lddw)
-                           : grad_product(d.K, d.N, d.M, d.dtype, {d.x, d.ldx}, true, dz, true, d.dw, d.lddw);
-    size_t most = 0;
-    if (d.dx) most = std::max(most, product_scratch(px));
-    if (d.dw) most = std::max(most, product_scratch(pw));
-    if (bytes) *bytes = c.used + most;
+    if (d.dw)
+        products[count++] = d.trans_w
+                                ? grad_product(d.N, d.K, d.M, d.dtype, dz, true, {d.x, d.ldx}, true, d.dw, d.lddw)
+                                : grad_product(d.K, d.N, d.M, d.dtype, {d.x, d.ldx}, true, dz, true, d.dw, d.lddw);
+    if (bytes) *bytes = c.used + product_scratch(products, count);
     if (!run) return TTC_OK;
     if (dz_needed || d.dbias) {
         g.M = d.M;
@@ -402,20 +422,24 @@ int plan_linear_backward(const ttc_linear_backward_desc& d, void* ws, size_t* by
         g.vec_dy = vec8_ok(d.dy, d.dtype, d.lddy);
         g.vec_pre = vec8_ok(d.pre, d.dtype, d.ldp);
         g.vec_dz = true;
-        const dim3 grid((unsigned)bands(d.M), (unsigned)((d.N + kStripe - 1) / kStripe));
+        const int n = bands(d.M);
+        const bool joined = d.dbias && n <= kClusterBands;
+        if (joined) {
+            g.dbias = d.dbias;
+            g.partials = nullptr;
+        }
+        const dim3 grid((unsigned)n, (unsigned)((d.N + kStripe - 1) / kStripe));
         count_launch();
         if (int rc = with_activation(d.act, [&](auto act) {
                 return launch_overlapped(d.dtype == TTC_BF16 ? linear_grad_kernel<__nv_bfloat16, act()>
                                                              : linear_grad_kernel<__half, act()>,
-                                         grid, 32 * kBandWarps, g);
+                                         grid, 32 * kBandWarps, joined ? n : 1, g);
             }))
             return rc;
-        if (d.dbias)
-            if (int rc = launch_sum_partials(g.partials, bands(d.M), d.N, d.dbias, d.dtype)) return rc;
+        if (d.dbias && !joined)
+            if (int rc = launch_sum_partials(g.partials, n, d.N, d.dbias, d.dtype)) return rc;
     }
-    if (d.dx)
-        if (int rc = run_product(px, scratch)) return rc;
-    return d.dw ? run_product(pw, scratch) : TTC_OK;
+    return run_products(products, count, scratch);
 }
 
 int plan_gated_backward(const ttc_gated_linear_backward_desc& d, void* ws, size_t* bytes, bool run) {
@@ -432,10 +456,15 @@ int plan_gated_backward(const ttc_gated_linear_backward_desc& d, void* ws, size_
     void* scratch = c.base ? c.base + c.used : nullptr;
     const Operand dg{dgu, ldd}, du{dgu ? dgu + np * es : nullptr, ldd};
     // dx [M, K] = dg Wg^T + du Wu^T: one accumulation over both weights.
-    Product px = grad_product(d.M, d.K, d.N, d.dtype, dg, false, {d.wg, d.ldw}, d.trans_w, d.dx, d.lddx);
-    px.segs = 2;
-    px.a[1] = du;
-    px.b[1] = {d.wu, d.ldw};
+    Product products[2];
+    int count = 0;
+    if (d.dx) {
+        Product& px = products[count++];
+        px = grad_product(d.M, d.K, d.N, d.dtype, dg, false, {d.wg, d.ldw}, d.trans_w, d.dx, d.lddx);
+        px.segs = 2;
+        px.a[1] = du;
+        px.b[1] = {d.wu, d.ldw};
+    }
     const int both = (int)(np + d.N);
     Product pw;
     if (d.trans_w) {  // [dwg; dwu] = [dg | du]^T x, one block of rows for each
@@ -448,10 +477,8 @@ int plan_gated_backward(const ttc_gated_linear_backward_desc& d, void* ws, size_
     pw.epi.split_skip = (int)(np - d.N);
     pw.epi.out2 = d.dwu;
     pw.epi.vec = all_vec(pw.epi);
-    size_t most = 0;
-    if (d.dx) most = std::max(most, product_scratch(px));
-    if (d.dwg) most = std::max(most, product_scratch(pw));
-    if (bytes) *bytes = c.used + most;
+    if (d.dwg) products[count++] = pw;
+    if (bytes) *bytes = c.used + product_scratch(products, count);
     if (!run) return TTC_OK;
     GatedGradParams g;
     std::memset(&g, 0, sizeof g);
@@ -474,12 +501,10 @@ int plan_gated_backward(const ttc_gated_linear_backward_desc& d, void* ws, size_
     if (int rc = with_activation(d.act, [&](auto act) {
             return launch_overlapped(
                 d.dtype == TTC_BF16 ? gated_grad_kernel<__nv_bfloat16, act()> : gated_grad_kernel<__half, act()>, grid,
-                32 * kBandWarps, g);
+                32 * kBandWarps, 1, g);
         }))
         return rc;
-    if (d.dx)
-        if (int rc = run_product(px, scratch)) return rc;
-    return d.dwg ? run_product(pw, scratch) : TTC_OK;
+    return run_products(products, count, scratch);
 }
 
 }  // namespace
@@ -493,7 +518,8 @@ int ttc_linear_workspace(const ttc_linear_desc* desc, size_t* bytes) {
     if (!desc || !bytes) return set_error(TTC_ERR_INVALID_ARGUMENT, "tt_cuda: linear_workspace: NULL argument");
     *bytes = 0;
     if (int rc = check_linear(*desc)) return rc;
-    *bytes = product_scratch(linear_product(*desc));
+    const Product p = linear_product(*desc);
+    *bytes = product_scratch(&p, 1);
     return TTC_OK;
 }
 
@@ -501,18 +527,19 @@ int ttc_linear(const ttc_linear_desc* desc) {
     if (!desc) return set_error(TTC_ERR_INVALID_ARGUMENT, "tt_cuda: linear: desc is NULL");
     if (int rc = check_linear(*desc)) return rc;
     const Product p = linear_product(*desc);
-    if (int rc = check_workspace("linear", desc->workspace, desc->workspace_bytes, product_scratch(p))) return rc;
+    if (int rc = check_workspace("linear", desc->workspace, desc->workspace_bytes, product_scratch(&p, 1))) return rc;
     TTC_REQUIRE_INIT();
     if (desc->M == 0) return TTC_OK;
     DeviceGuard guard;
-    return run_product(p, desc->workspace);
+    return run_products(&p, 1, desc->workspace);
 }
 
 int ttc_gated_linear_workspace(const ttc_gated_linear_desc* desc, size_t* bytes) {
     if (!desc || !bytes) return set_error(TTC_ERR_INVALID_ARGUMENT, "tt_cuda: gated_linear_workspace: NULL argument");
     *bytes = 0;
     if (int rc = check_gated(*desc)) return rc;
-    *bytes = product_scratch(gated_product(*desc));
+    const Product p = gated_product(*desc);
+    *bytes = product_scratch(&p, 1);
     return TTC_OK;
 }
 
@@ -520,11 +547,11 @@ int ttc_gated_linear(const ttc_gated_linear_desc* desc) {
     if (!desc) return set_error(TTC_ERR_INVALID_ARGUMENT, "tt_cuda: gated_linear: desc is NULL");
     if (int rc = check_gated(*desc)) return rc;
     const Product p = gated_product(*desc);
-    if (int rc = check_workspace("gated_linear", desc->workspace, desc->workspace_bytes, product_scratch(p))) return rc;
+    if (int rc = check_workspace("gated_linear", desc->workspace, desc->workspace_bytes, product_scratch(&p, 1))) return rc;
     TTC_REQUIRE_INIT();
     if (desc->M == 0) return TTC_OK;
     DeviceGuard guard;
-    return run_product(p, desc->workspace);
+    return run_products(&p, 1, desc->workspace);
 }
 
 int ttc_linear_backward_workspace(const ttc_linear_backward_desc* desc, size_t* bytes) {

@@ -59,6 +59,14 @@ struct alignas(64) ProductParams {
     int stall;
 };
 
+// The products of one tile_kernel launch. Of two, the second's blocks start at
+// `second`; each has blocks in whole clusters, the last of which may have no tile.
+template <int N>
+struct ProductSet {
+    ProductParams q[N];
+    unsigned second;
+};
+
 template <int GROUP, bool F8>
 __device__ __forceinline__ void mma(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                     uint32_t accumulate) {
@@ -750,8 +758,15 @@ __device__ __noinline__ void tile_finish_columns(const ProductParams& q, uint32_
     }
 }
 
-template <bool F8>
-__global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ ProductParams q) {
+// N = 2: both products of a backward pass, which do not wait for one another. One
+// launch and dbias without a second one: 79 x 976 x 512 with silu and bias 20.5 ->
+// 13.6 us a call, 104 x 440 x 1240 21.2 -> 13.7.
+template <bool F8, int N>
+__global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ ProductSet<N> set) {
+    const int which = N == 2 && blockIdx.x >= set.second;
+    const ProductParams& q = set.q[which];
+    const int block = (int)(blockIdx.x - (which ? set.second : 0));
+    if (N == 2 && block >= q.m_tiles * q.n_tiles * q.splits) return;  // (splits is 1 here)
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     const int stage_bytes = kHalf + q.tok * kRow, stages = q.stages;
@@ -764,7 +779,7 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ 
     const uint32_t done_bar = bar0 + 8u * (2 * stages);
     const Product& p = q.p;
     const int splits = q.splits, split = splits > 1 ? (int)cluster_rank() : 0;
-    const int tile = blockIdx.x / splits;
+    const int tile = block / splits;
     const int m0 = tile % q.m_tiles * q.tok, n0 = tile / q.m_tiles * (p.gated ? 64 : 128);
     const int kb0 = (int)((long long)q.kb_total * split / splits);
     const int kb1 = (int)((long long)q.kb_total * (split + 1) / splits);
@@ -924,8 +939,9 @@ struct Copy {
     unsigned rows, segments;         // segments of kSegment bytes a row
     int bytes;                       // of a row
 };
+constexpr int kMaxOperands = 8;  // of two products
 struct Copies {
-    Copy c[4];
+    Copy c[kMaxOperands];
     int n;
     unsigned blocks;  // segments of all rows of all copies
 };
@@ -1071,77 +1087,97 @@ int launch_pair(ProductParams& q) {
     return q.p.gated ? typed(std::true_type()) : typed(std::false_type());
 }
 
-template <bool F8>
-int launch_tile(ProductParams& q) {
+template <bool F8, int N>
+int launch_tile(const ProductSet<N>& set, unsigned blocks, int cluster) {
     static bool seen[kMaxDevices] = {};
-    const int ring = q.stages * (kHalf + q.tok * kRow);
+    int ring = 0;
+    for (const ProductParams& q : set.q) ring = std::max(ring, q.stages * (kHalf + q.tok * kRow));
     if (first_on_device(seen))
-        TTC_CUDA(cudaFuncSetAttribute(tile_kernel<F8>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448));
+        TTC_CUDA(cudaFuncSetAttribute(tile_kernel<F8, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448));
     cudaLaunchConfig_t cfg;
     std::memset(&cfg, 0, sizeof cfg);
     cudaLaunchAttribute attr[2];
     cfg.attrs = attr;
-    cfg.numAttrs = launch_attributes(attr, q.splits);
+    cfg.numAttrs = launch_attributes(attr, cluster);
     cfg.blockDim = dim3(kThreads, 1, 1);
     cfg.dynamicSmemBytes = (size_t)ring + 1024 + 256;
     cfg.stream = rt().stream;
-    cfg.gridDim = dim3((unsigned)((long long)q.m_tiles * q.n_tiles * q.splits), 1, 1);
-    TTC_CUDA(cudaLaunchKernelEx(&cfg, tile_kernel<F8>, q));
+    cfg.gridDim = dim3(blocks, 1, 1);
+    TTC_CUDA(cudaLaunchKernelEx(&cfg, tile_kernel<F8, N>, set));
     count_launch();
     return TTC_OK;
 }
 
-}  // namespace
-
-size_t product_scratch(const Product& p) {
-    Stored s[4];
-    const int n = stored_operands(p, s), es = dtype_size(p.dtype);
+// The operands that must be copied and where each goes; one that several products
+// read is copied once.
+struct Padding {
+    struct Entry {
+        Operand o;
+        long long rows, cols;
+        size_t at;
+    } e[kMaxOperands];
+    int n = 0;
     size_t bytes = 0;
-    for (int i = 0; i < n; ++i)
-        if (!aligned16(*s[i].o, es)) bytes += align256((size_t)s[i].rows * padded_ld(s[i].cols, es) * es);
-    return bytes;
+    int find(const Stored& s) const {
+        int j = 0;
+        while (j < n && !(e[j].o.ptr == s.o->ptr && e[j].o.ld == s.o->ld && e[j].rows == s.rows && e[j].cols == s.cols)) ++j;
+        return j;
+    }
+};
+Padding padding_of(const Product* products, int count) {
+    Padding pad;
+    for (int k = 0; k < count; ++k) {
+        Stored s[4];
+        const int n = stored_operands(products[k], s), es = dtype_size(products[k].dtype);
+        for (int i = 0; i < n; ++i) {
+            if (aligned16(*s[i].o, es) || pad.find(s[i]) < pad.n) continue;
+            pad.e[pad.n++] = {*s[i].o, s[i].rows, s[i].cols, pad.bytes};
+            pad.bytes += align256((size_t)s[i].rows * padded_ld(s[i].cols, es) * es);
+        }
+    }
+    return pad;
 }
 
-int run_product(const Product& given, void* scratch) {
-    if (rt().device < 0 || rt().device >= kMaxDevices)
-        return set_error(TTC_ERR_UNSUPPORTED, "tt_cuda: device %d", rt().device);
-    ProductParams q;
-    std::memset(&q, 0, sizeof q);
-    Product& p = q.p;
-    p = given;
-    const int es = dtype_size(p.dtype), sms = rt().sm_count;
-    const bool f8 = p.dtype == TTC_E4M3;
-    Stored s[4];
-    const int n = stored_operands(p, s);
-    char* room = (char*)scratch;
+// Copies what must be copied and has the products read the copies.
+int pad_operands(Product* products, int count, void* scratch) {
+    const Padding pad = padding_of(products, count);
+    if (!pad.n) return TTC_OK;
+    const int es = dtype_size(products[0].dtype);
     Copies copies = {};
     long long segments = 0;
-    for (int i = 0; i < n; ++i) {
-        if (aligned16(*s[i].o, es)) continue;
-        Operand& o = const_cast<Operand&>(*s[i].o);
-        const long long ldd = padded_ld(s[i].cols, es);
-        Copy& c = copies.c[copies.n++];
-        const int bytes = (int)s[i].cols * es;
-        c = {(const uint8_t*)o.ptr, (uint8_t*)room, o.ld * es, ldd * es, (unsigned)s[i].rows,
-             (unsigned)((bytes + kSegment - 1) / kSegment), bytes};
+    for (int j = 0; j < pad.n; ++j) {
+        const Padding::Entry& e = pad.e[j];
+        const int bytes = (int)e.cols * es;
+        const Copy c = {(const uint8_t*)e.o.ptr, (uint8_t*)scratch + e.at, e.o.ld * es, padded_ld(e.cols, es) * es,
+                        (unsigned)e.rows, (unsigned)((bytes + kSegment - 1) / kSegment), bytes};
+        copies.c[copies.n++] = c;
         segments += (long long)c.rows * c.segments;
-        o = {room, ldd};
-        room += align256((size_t)s[i].rows * ldd * es);
     }
-    if (copies.n) {
-        count_launch();
-        if (segments > INT32_MAX) return set_error(TTC_ERR_UNSUPPORTED, "tt_cuda: unaligned operands are too large");
-        copies.blocks = (unsigned)segments;
-        const dim3 grid((unsigned)std::min<long long>(segments, 64ll * sms));
-        if (int rc = launch_overlapped(pad_rows_kernel, grid, 256, copies)) return rc;
+    if (segments > INT32_MAX) return set_error(TTC_ERR_UNSUPPORTED, "tt_cuda: unaligned operands are too large");
+    for (int k = 0; k < count; ++k) {
+        Stored s[4];
+        const int n = stored_operands(products[k], s);
+        for (int i = 0; i < n; ++i) {
+            if (aligned16(*s[i].o, es)) continue;
+            const Padding::Entry& e = pad.e[pad.find(s[i])];
+            *const_cast<Operand*>(s[i].o) = {(char*)scratch + e.at, padded_ld(e.cols, es)};
+        }
     }
-    const int bk = kRow / es;
+    copies.blocks = (unsigned)segments;
+    count_launch();
+    const dim3 grid((unsigned)std::min<long long>(segments, 64ll * rt().sm_count));
+    return launch_overlapped(pad_rows_kernel, grid, 256, 1, copies);
+}
+
+// tile_kernel's shape for q.p, and whether pair_kernel is expected to be faster.
+int plan_product(ProductParams& q, bool* pair) {
+    const Product& p = q.p;
+    const int sms = rt().sm_count, bk = kRow / dtype_size(p.dtype);
     q.kb_seg = (p.K + bk - 1) / bk;
     q.kb_total = q.kb_seg * p.segs;
     if (int rc = device_status_ptr(&q.status)) return rc;
     q.stall = stall_test("linear") ? 1 : 0;
     q.wait_limit = q.stall ? kStallTestLimitCycles : kWaitLimitCycles;
-    const int nb = p.gated ? 2 : p.segs;
 
     // tile_kernel's shape. Rows a tile: all of x up to 256; fewer where even eight
     // CTAs a tile would leave SMs idle (256 x 1024 x 512: 18.3 us with 8 tiles of
@@ -1176,32 +1212,85 @@ int run_product(const Product& given, void* scratch) {
     const double pair_us = 6.0 + 0.35 * q.kb_total * rounds(pair_m * pair_n, sms / 2);
     const double tile_us = 3.5 + 5.5 * q.tok / 256 + 0.42 * (128 + q.tok) / 384 * rounds(q.kb_total, q.splits) *
                                                          rounds(tiles() * q.splits, sms);
-    if (pair_us < tile_us) {
-        q.m_tiles = (int)pair_m;
-        q.n_tiles = (int)pair_n;
-        q.idesc = instruction(p, p.a_mn, p.b_mn, 256, 256);
-        for (int i = 0; i < p.segs; ++i)
-            if (int rc = make_map(&q.a[i], p, p.a[i], p.M, p.a_mn, 128)) return rc;
-        for (int i = 0; i < nb; ++i)
-            if (int rc = make_map(&q.b[i], p, p.b[i], p.N, p.b_mn, 128)) return rc;
-        if (p.epi.vec)
-            if (int rc = make_output_maps(q)) return rc;
-        return f8 ? launch_pair<true>(q) : launch_pair<false>(q);
-    }
+    *pair = pair_us < tile_us;
+    if (!*pair) q.m_tiles = (p.M + q.tok - 1) / q.tok;
+    return TTC_OK;
+}
 
-    q.m_tiles = (p.M + q.tok - 1) / q.tok;
+int run_pair(ProductParams& q) {
+    const Product& p = q.p;
+    q.m_tiles = (p.M + 255) / 256;
+    q.n_tiles = p.gated ? (p.N + 127) / 128 : (p.N + 255) / 256;
+    q.idesc = instruction(p, p.a_mn, p.b_mn, 256, 256);
+    for (int i = 0; i < p.segs; ++i)
+        if (int rc = make_map(&q.a[i], p, p.a[i], p.M, p.a_mn, 128)) return rc;
+    for (int i = 0; i < (p.gated ? 2 : p.segs); ++i)
+        if (int rc = make_map(&q.b[i], p, p.b[i], p.N, p.b_mn, 128)) return rc;
+    if (p.epi.vec)
+        if (int rc = make_output_maps(q)) return rc;
+    return p.dtype == TTC_E4M3 ? launch_pair<true>(q) : launch_pair<false>(q);
+}
+
+template <bool F8, int N>
+int run_tiles(ProductSet<N>& set) {
+    const int sms = rt().sm_count;
+    int cluster = 1;
+    for (const ProductParams& q : set.q) cluster = std::max(cluster, q.splits);
+    unsigned blocks = 0;
+    bool small = true;  // rings of three stages in half an SM's shared memory
+    for (ProductParams& q : set.q) {
+        if (&q != set.q) set.second = blocks;
+        const unsigned tiles = (unsigned)q.m_tiles * q.n_tiles * q.splits;
+        blocks += (tiles + cluster - 1) / cluster * cluster;
+        small = small && 3 * (kHalf + q.tok * kRow) <= 104 * 1024;
+    }
     // The ring: half an SM's shared memory where two CTAs meet on an SM and that
     // holds three stages, so that one's loads run under the other's start and end
     // (4 x 16384 x 4096 gated: 45 us, 51 with the whole of it); else most of it.
-    const int stage_bytes = kHalf + q.tok * kRow;
-    const bool two = tiles() * q.splits > sms && 3 * stage_bytes <= 104 * 1024;
-    q.stages = std::min(12, (two ? 104 * 1024 : 200 * 1024) / stage_bytes);
-    q.idesc = instruction(p, p.b_mn, p.a_mn, 128, q.tok);
-    for (int i = 0; i < p.segs; ++i)
-        if (int rc = make_map(&q.a[i], p, p.a[i], p.M, p.a_mn, q.tok)) return rc;
-    for (int i = 0; i < nb; ++i)
-        if (int rc = make_map(&q.b[i], p, p.b[i], p.N, p.b_mn, p.gated ? 64 : 128)) return rc;
-    return f8 ? launch_tile<true>(q) : launch_tile<false>(q);
+    const int room = small && blocks > (unsigned)sms ? 104 * 1024 : 200 * 1024;
+    for (ProductParams& q : set.q) {
+        const Product& p = q.p;
+        q.stages = std::min(12, room / (kHalf + q.tok * kRow));
+        q.idesc = instruction(p, p.b_mn, p.a_mn, 128, q.tok);
+        for (int i = 0; i < p.segs; ++i)
+            if (int rc = make_map(&q.a[i], p, p.a[i], p.M, p.a_mn, q.tok)) return rc;
+        for (int i = 0; i < (p.gated ? 2 : p.segs); ++i)
+            if (int rc = make_map(&q.b[i], p, p.b[i], p.N, p.b_mn, p.gated ? 64 : 128)) return rc;
+    }
+    return launch_tile<F8, N>(set, blocks, cluster);
+}
+
+}  // namespace
+
+size_t product_scratch(const Product* products, int count) { return padding_of(products, count).bytes; }
+
+int run_products(const Product* given, int count, void* scratch) {
+    if (rt().device < 0 || rt().device >= kMaxDevices)
+        return set_error(TTC_ERR_UNSUPPORTED, "tt_cuda: device %d", rt().device);
+    Product products[2];
+    for (int k = 0; k < count; ++k) products[k] = given[k];
+    if (int rc = pad_operands(products, count, scratch)) return rc;
+    ProductSet<2> both;
+    std::memset(&both, 0, sizeof both);
+    bool pair[2] = {};
+    for (int k = 0; k < count; ++k) {
+        both.q[k].p = products[k];
+        if (int rc = plan_product(both.q[k], &pair[k])) return rc;
+    }
+    // Together only where neither product's sums are split differently than alone.
+    const int s0 = both.q[0].splits, s1 = both.q[1].splits;
+    if (count == 2 && !pair[0] && !pair[1] && (s0 == s1 || s0 == 1 || s1 == 1)) return run_tiles<false, 2>(both);
+    for (int k = 0; k < count; ++k) {
+        if (pair[k]) {
+            if (int rc = run_pair(both.q[k])) return rc;
+            continue;
+        }
+        ProductSet<1> one;
+        one.second = 0;
+        one.q[0] = both.q[k];
+        if (int rc = products[k].dtype == TTC_E4M3 ? run_tiles<true, 1>(one) : run_tiles<false, 1>(one)) return rc;
+    }
+    return TTC_OK;
 }
 
 }  // namespace ttc

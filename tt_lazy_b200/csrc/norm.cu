@@ -826,7 +826,8 @@ int check_workspace(const char* op, const void* ws, size_t have, size_t need) {
 
 int launch_sum_partials(const float* partials, int n, int cols, void* out, int dtype) {
     count_launch();
-    return launch_overlapped(sum_partials_kernel, dim3((unsigned)((cols + 31) / 32)), 1024, partials, n, cols, out, dtype);
+    const dim3 grid((unsigned)((cols + 31) / 32));
+    return launch_overlapped(sum_partials_kernel, grid, 1024, 1, partials, n, cols, out, dtype);
 }
 
 }  // namespace ttc
