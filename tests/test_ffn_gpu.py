@@ -522,7 +522,7 @@ def test_gradients_alone_equal_those_of_the_whole_call(lib, M, N, K, trans_w, ga
         assert torch.equal(a.t, b.t)
 
 
-@pytest.mark.parametrize("M", [1, 7, 64, 65, 130, 449, 512, 513, 1000, 16385])
+@pytest.mark.parametrize("M", [1, 7, 8, 9, 64, 65, 130, 255, 256, 257, 449, 512, 513, 1000, 16385])
 @pytest.mark.parametrize("N,act", [(1, "none"), (259, "gelu"), (2048, "relu")])
 def test_bias_gradient_over_bands_of_rows(lib, M, N, act):
     """Row counts around those where the column sums change hands: whole numbers, so exact in any order."""

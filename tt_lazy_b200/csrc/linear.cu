@@ -127,10 +127,29 @@ int check_gated_backward(const ttc_gated_linear_backward_desc& d) {
 // TB/s), 51 us for the gated pair with silu (6.6 TB/s); without the row ahead 47
 // and 73.
 constexpr int kStripe = 256, kBandWarps = 8;
-// Rows of a block: 64, more when that would make over 256 bands of partial sums.
-int band_rows(int M) { return std::max(64, (M + 255) / 256); }
-int bands(int M) { return (M + band_rows(M) - 1) / band_rows(M); }
-constexpr int kClusterBands = 8;  // up to so many bands are a cluster: dbias needs no second launch
+// Rows of a block: 64, more when that would make over 256 bands of partial sums,
+// and fewer, down to one a warp, while that leaves SMs without two blocks: a
+// warp's rows come one after the other (what this kernel adds to a call with silu,
+// 64 rows and then fewer: 128 x 4096 8.4 -> 3.7 us, 2461 x 663 12.3 -> 4.3).
+// Bands of up to 32 rows that are at most a cluster are `joined`: the cluster adds
+// up dbias itself. (With 64 rows that costs more than a second launch: 512 x 1024
+// 10.3 us, 1000 x 1000 in bands of 8 rows 5.0.)
+constexpr int kClusterBands = 8, kJoinedRows = 32;
+struct Bands {
+    int rows, n, stripes;
+    bool joined;
+};
+Bands bands_of(int M, int N, bool dbias) {
+    Bands b;
+    b.stripes = (N + kStripe - 1) / kStripe;
+    auto count = [&](int rows) { return (M + rows - 1) / rows; };
+    b.joined = dbias && count(kJoinedRows) <= kClusterBands;
+    b.rows = b.joined ? kJoinedRows : std::max(64, count(256));
+    const int most = b.joined ? kClusterBands : 256;
+    while (b.rows > kBandWarps && (long long)count(b.rows) * b.stripes < 2 * 148 && count(b.rows / 2) <= most) b.rows /= 2;
+    b.n = count(b.rows);
+    return b;
+}
 
 struct LinearGradParams {
     int M, N, band_rows;
@@ -395,7 +414,8 @@ int plan_linear_backward(const ttc_linear_backward_desc& d, void* ws, size_t* by
         g.dz = c.take((size_t)d.M * lddz * es);
         dz = {g.dz, lddz};
     }
-    if (d.dbias) g.partials = (float*)c.take((size_t)bands(d.M) * d.N * sizeof(float));
+    const Bands b = bands_of(d.M, d.N, d.dbias != nullptr);
+    if (d.dbias) g.partials = (float*)c.take((size_t)b.n * d.N * sizeof(float));
     void* scratch = c.base ? c.base + c.used : nullptr;
     // dx [M, K] = dz [M, N] W^T: the sum runs over N, which is contiguous in a
     // weight stored [K, N] and strided in one stored [N, K].
@@ -413,7 +433,7 @@ int plan_linear_backward(const ttc_linear_backward_desc& d, void* ws, size_t* by
     if (dz_needed || d.dbias) {
         g.M = d.M;
         g.N = d.N;
-        g.band_rows = band_rows(d.M);
+        g.band_rows = b.rows;
         g.dy = d.dy;
         g.pre = d.pre;
         g.lddy = d.lddy;
@@ -422,22 +442,20 @@ int plan_linear_backward(const ttc_linear_backward_desc& d, void* ws, size_t* by
         g.vec_dy = vec8_ok(d.dy, d.dtype, d.lddy);
         g.vec_pre = vec8_ok(d.pre, d.dtype, d.ldp);
         g.vec_dz = true;
-        const int n = bands(d.M);
-        const bool joined = d.dbias && n <= kClusterBands;
-        if (joined) {
+        if (b.joined) {
             g.dbias = d.dbias;
             g.partials = nullptr;
         }
-        const dim3 grid((unsigned)n, (unsigned)((d.N + kStripe - 1) / kStripe));
+        const dim3 grid((unsigned)b.n, (unsigned)b.stripes);
         count_launch();
         if (int rc = with_activation(d.act, [&](auto act) {
                 return launch_overlapped(d.dtype == TTC_BF16 ? linear_grad_kernel<__nv_bfloat16, act()>
                                                              : linear_grad_kernel<__half, act()>,
-                                         grid, 32 * kBandWarps, joined ? n : 1, g);
+                                         grid, 32 * kBandWarps, b.joined ? b.n : 1, g);
             }))
             return rc;
-        if (d.dbias && !joined)
-            if (int rc = launch_sum_partials(g.partials, n, d.N, d.dbias, d.dtype)) return rc;
+        if (d.dbias && !b.joined)
+            if (int rc = launch_sum_partials(g.partials, b.n, d.N, d.dbias, d.dtype)) return rc;
     }
     return run_products(products, count, scratch);
 }
@@ -484,7 +502,8 @@ int plan_gated_backward(const ttc_gated_linear_backward_desc& d, void* ws, size_
     std::memset(&g, 0, sizeof g);
     g.M = d.M;
     g.N = d.N;
-    g.band_rows = band_rows(d.M);
+    const Bands b = bands_of(d.M, d.N, false);
+    g.band_rows = b.rows;
     g.dy = d.dy;
     g.gate = d.gate;
     g.up = d.up;
@@ -496,7 +515,7 @@ int plan_gated_backward(const ttc_gated_linear_backward_desc& d, void* ws, size_
     g.vec_dy = vec8_ok(d.dy, d.dtype, d.lddy);
     g.vec_gate = vec8_ok(d.gate, d.dtype, d.ldp);
     g.vec_up = vec8_ok(d.up, d.dtype, d.ldp);
-    const dim3 grid((unsigned)bands(d.M), (unsigned)((d.N + kStripe - 1) / kStripe));
+    const dim3 grid((unsigned)b.n, (unsigned)b.stripes);
     count_launch();
     if (int rc = with_activation(d.act, [&](auto act) {
             return launch_overlapped(
