@@ -1087,24 +1087,46 @@ int launch_pair(ProductParams& q) {
     return q.p.gated ? typed(std::true_type()) : typed(std::false_type());
 }
 
-template <bool F8, int N>
-int launch_tile(const ProductSet<N>& set, unsigned blocks, int cluster) {
-    static bool seen[kMaxDevices] = {};
-    int ring = 0;
-    for (const ProductParams& q : set.q) ring = std::max(ring, q.stages * (kHalf + q.tok * kRow));
-    if (first_on_device(seen))
-        TTC_CUDA(cudaFuncSetAttribute(tile_kernel<F8, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448));
+constexpr int kTileExtra = 1024 + 256;  // shared memory beside the ring: alignment, barriers
+
+// A launch of tile_kernel but for its arguments.
+struct TileLaunch {
     cudaLaunchConfig_t cfg;
-    std::memset(&cfg, 0, sizeof cfg);
     cudaLaunchAttribute attr[2];
-    cfg.attrs = attr;
-    cfg.numAttrs = launch_attributes(attr, cluster);
-    cfg.blockDim = dim3(kThreads, 1, 1);
-    cfg.dynamicSmemBytes = (size_t)ring + 1024 + 256;
-    cfg.stream = rt().stream;
-    cfg.gridDim = dim3(blocks, 1, 1);
-    TTC_CUDA(cudaLaunchKernelEx(&cfg, tile_kernel<F8, N>, set));
-    count_launch();
+    TileLaunch(unsigned blocks, int cluster, int ring) {
+        std::memset(&cfg, 0, sizeof cfg);
+        cfg.attrs = attr;
+        cfg.numAttrs = launch_attributes(attr, cluster);
+        cfg.blockDim = dim3(kThreads, 1, 1);
+        cfg.dynamicSmemBytes = (size_t)ring + kTileExtra;
+        cfg.stream = rt().stream;
+        cfg.gridDim = dim3(blocks, 1, 1);
+    }
+};
+
+// Blocks that run at once, in clusters (a power of two up to 8), with a ring of
+// kFullRing bytes: fewer than the SMs where a cluster has to fit into what an
+// earlier one leaves of a group of SMs.
+constexpr int kFullRing = 200 * 1024, kHalfRing = 104 * 1024;
+bool half_ring_holds(int tok) { return 3 * (kHalf + tok * kRow) <= kHalfRing; }  // three stages
+template <bool F8, int N>
+int tile_blocks_at_once(int cluster, int* blocks) {
+    static bool seen[kMaxDevices] = {};
+    static int most[kMaxDevices][4] = {};
+    auto kernel = tile_kernel<F8, N>;
+    if (first_on_device(seen)) {
+        TTC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448));
+        for (int i = 0; i < 4; ++i) {
+            const TileLaunch l(rt().sm_count / (1 << i) << i, 1 << i, kFullRing);
+            int n = 0;
+            if (cudaOccupancyMaxActiveClusters(&n, kernel, &l.cfg) != cudaSuccess || n < 1) {
+                cudaGetLastError();
+                n = rt().sm_count >> i;
+            }
+            most[rt().device][i] = n << i;
+        }
+    }
+    *blocks = most[rt().device][cluster >= 8 ? 3 : cluster >> 1];
     return TTC_OK;
 }
 
@@ -1195,7 +1217,16 @@ int plan_product(ProductParams& q, bool* pair) {
     auto tiles = [&] { return ((long long)p.M + q.tok - 1) / q.tok * q.n_tiles; };
     while (q.tok > std::max(32, unit) && tiles() * most_splits < sms) q.tok = (q.tok / 2 + unit - 1) / unit * unit;
     q.splits = 1;
-    while (q.splits < most_splits && tiles() * q.splits * 2 <= (q.tok <= 32 ? 2 * sms : sms)) q.splits *= 2;
+    auto room_for = [&](int splits, long long* blocks) {  // CTAs that run at once
+        int at_once = 0;
+        const int rc = tile_blocks_at_once<false, 1>(splits, &at_once);
+        *blocks = q.tok <= 32 ? 2 * sms : half_ring_holds(q.tok) ? sms : at_once;
+        return rc;
+    };
+    for (long long blocks; q.splits < most_splits; q.splits *= 2) {
+        if (int rc = room_for(2 * q.splits, &blocks)) return rc;
+        if (tiles() * q.splits * 2 > blocks) break;
+    }
 
     // Which kernel: the shorter estimate, from k-blocks times their measured cost
     // (0.35 us for a pair's 256 x 256, up to 0.42 us for a tile's 128 x 256, both
@@ -1233,31 +1264,39 @@ int run_pair(ProductParams& q) {
 
 template <bool F8, int N>
 int run_tiles(ProductSet<N>& set) {
-    const int sms = rt().sm_count;
     int cluster = 1;
     for (const ProductParams& q : set.q) cluster = std::max(cluster, q.splits);
     unsigned blocks = 0;
-    bool small = true;  // rings of three stages in half an SM's shared memory
+    bool small = true;
     for (ProductParams& q : set.q) {
         if (&q != set.q) set.second = blocks;
         const unsigned tiles = (unsigned)q.m_tiles * q.n_tiles * q.splits;
         blocks += (tiles + cluster - 1) / cluster * cluster;
-        small = small && 3 * (kHalf + q.tok * kRow) <= 104 * 1024;
+        small = small && half_ring_holds(q.tok);
     }
-    // The ring: half an SM's shared memory where two CTAs meet on an SM and that
-    // holds three stages, so that one's loads run under the other's start and end
-    // (4 x 16384 x 4096 gated: 45 us, 51 with the whole of it); else most of it.
-    const int room = small && blocks > (unsigned)sms ? 104 * 1024 : 200 * 1024;
+    // The ring: half an SM's shared memory where not all CTAs run at once otherwise
+    // and that holds three stages, so that two meet on an SM and one's loads run
+    // under the other's start and end (4 x 16384 x 4096 gated: 45 us, 51 with the
+    // whole of it; 32 x 2048 x 8192 in 16 clusters of 8, of which 15 fit: 11.4 and
+    // 22.4); else most of it.
+    int at_once = 0;
+    if (int rc = tile_blocks_at_once<F8, N>(cluster, &at_once)) return rc;
+    const int room = small && blocks > (unsigned)at_once ? kHalfRing : kFullRing;
+    int ring = 0;
     for (ProductParams& q : set.q) {
         const Product& p = q.p;
         q.stages = std::min(12, room / (kHalf + q.tok * kRow));
+        ring = std::max(ring, q.stages * (kHalf + q.tok * kRow));
         q.idesc = instruction(p, p.b_mn, p.a_mn, 128, q.tok);
         for (int i = 0; i < p.segs; ++i)
             if (int rc = make_map(&q.a[i], p, p.a[i], p.M, p.a_mn, q.tok)) return rc;
         for (int i = 0; i < (p.gated ? 2 : p.segs); ++i)
             if (int rc = make_map(&q.b[i], p, p.b[i], p.N, p.b_mn, p.gated ? 64 : 128)) return rc;
     }
-    return launch_tile<F8, N>(set, blocks, cluster);
+    const TileLaunch l(blocks, cluster, ring);
+    TTC_CUDA(cudaLaunchKernelEx(&l.cfg, tile_kernel<F8, N>, set));
+    count_launch();
+    return TTC_OK;
 }
 
 }  // namespace
