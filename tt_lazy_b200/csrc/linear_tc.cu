@@ -1104,29 +1104,29 @@ struct TileLaunch {
     }
 };
 
-// Blocks that run at once, in clusters (a power of two up to 8), with a ring of
-// kFullRing bytes: fewer than the SMs where a cluster has to fit into what an
-// earlier one leaves of a group of SMs.
+// Blocks that run at once, in clusters, with a ring of kFullRing bytes: fewer than
+// the SMs where a cluster has to fit into what earlier ones leave of a group of SMs.
+constexpr int kMaxSplits = 8;
 constexpr int kFullRing = 200 * 1024, kHalfRing = 104 * 1024;
 bool half_ring_holds(int tok) { return 3 * (kHalf + tok * kRow) <= kHalfRing; }  // three stages
 template <bool F8, int N>
 int tile_blocks_at_once(int cluster, int* blocks) {
     static bool seen[kMaxDevices] = {};
-    static int most[kMaxDevices][4] = {};
+    static int most[kMaxDevices][kMaxSplits + 1] = {};
     auto kernel = tile_kernel<F8, N>;
     if (first_on_device(seen)) {
         TTC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448));
-        for (int i = 0; i < 4; ++i) {
-            const TileLaunch l(rt().sm_count / (1 << i) << i, 1 << i, kFullRing);
+        for (int c = 1; c <= kMaxSplits; ++c) {
+            const TileLaunch l(rt().sm_count / c * c, c, kFullRing);
             int n = 0;
             if (cudaOccupancyMaxActiveClusters(&n, kernel, &l.cfg) != cudaSuccess || n < 1) {
                 cudaGetLastError();
-                n = rt().sm_count >> i;
+                n = rt().sm_count / c;
             }
-            most[rt().device][i] = n << i;
+            most[rt().device][c] = n * c;
         }
     }
-    *blocks = most[rt().device][cluster >= 8 ? 3 : cluster >> 1];
+    *blocks = most[rt().device][cluster];
     return TTC_OK;
 }
 
@@ -1207,25 +1207,22 @@ int plan_product(ProductParams& q, bool* pair) {
     // each, and two each for few rows, whose CTAs spend their time waiting for the
     // weight (1 x 4096 x 16384: 24.2 us with 256 CTAs, 28.0 with 128; 64 x 4096 x
     // 4096: 13.1 us with 128, 15.8 with 256), while every share has at least
-    // four k-blocks (two for a few rows, where joining the shares is quick).
+    // four k-blocks (two for a few rows, where joining the shares is quick). One CTA
+    // an SM takes any number of shares whose clusters run at once (256 x 4608 x 4608:
+    // three 20.9 us, two 25.0, four in two rounds 34.1); two an SM take powers of two
+    // (clusters of five or seven leave SMs out: 32 x 5120 x 5120 four 14.8, seven 22.4).
     const int unit = p.a_mn ? 64 : 16, width = p.gated ? 64 : 128;
     const int least = p.M <= 16 ? 2 : 4;
     q.n_tiles = (p.N + width - 1) / width;
-    int most_splits = 1;
-    while (most_splits < 8 && q.kb_total >= 2 * most_splits * least) most_splits *= 2;
+    const int most_splits = std::max(1, std::min(kMaxSplits, q.kb_total / least));
     q.tok = std::min(256, (p.M + unit - 1) / unit * unit);
     auto tiles = [&] { return ((long long)p.M + q.tok - 1) / q.tok * q.n_tiles; };
     while (q.tok > std::max(32, unit) && tiles() * most_splits < sms) q.tok = (q.tok / 2 + unit - 1) / unit * unit;
-    q.splits = 1;
-    auto room_for = [&](int splits, long long* blocks) {  // CTAs that run at once
+    for (q.splits = most_splits; q.splits > 1; --q.splits) {
         int at_once = 0;
-        const int rc = tile_blocks_at_once<false, 1>(splits, &at_once);
-        *blocks = q.tok <= 32 ? 2 * sms : half_ring_holds(q.tok) ? sms : at_once;
-        return rc;
-    };
-    for (long long blocks; q.splits < most_splits; q.splits *= 2) {
-        if (int rc = room_for(2 * q.splits, &blocks)) return rc;
-        if (tiles() * q.splits * 2 > blocks) break;
+        if (int rc = tile_blocks_at_once<false, 1>(q.splits, &at_once)) return rc;
+        if (q.tok <= 32 && (q.splits & (q.splits - 1))) continue;
+        if (tiles() * q.splits <= (q.tok <= 32 ? 2 * sms : half_ring_holds(q.tok) ? sms : at_once)) break;
     }
 
     // Which kernel: the shorter estimate, from k-blocks times their measured cost
