@@ -353,29 +353,32 @@ template <int DT, bool GATED>
 __device__ __forceinline__ void finish_column(const ProductEpilogue& e, int row, int step, int count, int col,
                                               float (&v)[8], float (&u)[8], float s0, float s1, float bias) {
     using E = Element<DT>;
-    auto each = [&](auto f) {
+    // f(i, index): the rows' indices into a matrix of pitch ld, from one multiplication
+    auto each = [&](long long ld, int first, int column, auto f) {
+        long long at = first * ld + column;
+        const long long down = step * ld;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < count) f(i, row + i * step);
+        for (int i = 0; i < 8; ++i, at += down)
+            if (i < count) f(i, at);
     };
     float res[8];
-    if (!GATED && e.residual) each([&](int i, int r) { res[i] = E::load(e.residual, r * e.ldr + col); });
+    if (!GATED && e.residual) each(e.ldr, row, col, [&](int i, long long at) { res[i] = E::load(e.residual, at); });
     if (e.row_scales)
-        each([&](int i, int r) {
-            const float rs = e.row_scales[r];
+        each(1, row, 0, [&](int i, long long at) {
+            const float rs = e.row_scales[at];
             v[i] = v[i] * rs * s0;
             if (GATED) u[i] = u[i] * rs * s1;
         });
     if (GATED) {
         if (e.gate)
-            each([&](int i, int r) {
-                E::store(e.gate, r * e.ldp + col, v[i]);
-                E::store(e.up, r * e.ldp + col, u[i]);
+            each(e.ldp, row, col, [&](int i, long long at) {
+                E::store(e.gate, at, v[i]);
+                E::store(e.up, at, u[i]);
             });
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] += bias;
-        if (e.pre) each([&](int i, int r) { E::store(e.pre, r * e.ldp + col, v[i]); });
+        if (e.pre) each(e.ldp, row, col, [&](int i, long long at) { E::store(e.pre, at, v[i]); });
     }
     activate_all<8>(e.act, v);
     if (GATED) {
@@ -386,8 +389,8 @@ __device__ __forceinline__ void finish_column(const ProductEpilogue& e, int row,
         for (int i = 0; i < 8; ++i) v[i] += res[i];
     }
     if (e.split_rows > 0) {
-        each([&](int i, int r) {
-            const int second = r - e.split_rows - e.split_skip;
+        each(1, row, 0, [&](int i, long long r) {
+            const long long second = r - e.split_rows - e.split_skip;
             if (r < e.split_rows)
                 E::store(e.out, r * e.ldo + col, v[i]);
             else if (second >= 0)
@@ -401,7 +404,7 @@ __device__ __forceinline__ void finish_column(const ProductEpilogue& e, int row,
         if (col < 0) return;
         out = e.out2;
     }
-    each([&](int i, int r) { E::store(out, r * e.ldo + col, v[i]); });
+    each(e.ldo, row, col, [&](int i, long long at) { E::store(out, at, v[i]); });
 }
 __device__ __forceinline__ float bias_at(const ProductEpilogue& e, int col) {
     if (!e.bias) return 0.0f;
