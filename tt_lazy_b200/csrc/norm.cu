@@ -359,6 +359,7 @@ struct RingParams {
     int stages, row_bytes;
     int* status;
     long long wait_limit;
+    int stall;  // failure-detection test: no loads at all
 };
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
@@ -390,8 +391,9 @@ __global__ void __launch_bounds__(MAX, 512 / MAX) rms_norm_backward_ring_kernel(
         mbar_fence_init();
     }
     __syncthreads();
-    if (t == 0)
-        for (int i = 0; i < q.stages && i < mine; ++i) issue(i, i);
+    int issued = 0;  // rows that thread 0 has sent for
+    if (t == 0 && !q.stall)
+        for (; issued < q.stages && issued < mine; ++issued) issue(issued, issued);
     uint4 w[C];
     float dw[C][kPer<T>] = {};
 #pragma unroll
@@ -476,12 +478,17 @@ __global__ void __launch_bounds__(MAX, 512 / MAX) rms_norm_backward_ring_kernel(
             store_row<T, T, true, 1>(static_cast<T*>(p.dx) + r * p.lddx, p.cols, Lane{c * threads + t, 0}, out);
         }
         __syncthreads();
-        if (t == 0 && i + q.stages < mine) issue(i + q.stages, s);
+        // After a wait that ran out the stage may still be filled, so nothing more is
+        // sent for: its barrier must not be armed again, nor its buffer written.
+        if (t == 0 && !failed && i + q.stages < mine) {
+            issue(i + q.stages, s);
+            ++issued;
+        }
         if (++s == q.stages) s = 0;
     }
     if (failed) *(volatile int*)q.status = 1;
-    if (t == 0 && failed)  // never leave with copies in flight
-        for (int i = mine > q.stages ? mine - q.stages : 0; i < mine; ++i)
+    if (t == 0 && failed)  // never leave with copies in flight: the last rows that were sent for
+        for (int i = max(0, issued - q.stages); i < issued; ++i)
             mbar_wait(smem_u32(&bars[i % q.stages]), (uint32_t)(i / q.stages) & 1, q.wait_limit);
     if (!p.partials) return;
     float* part = p.partials + (long long)blockIdx.x * p.cols;
@@ -773,7 +780,8 @@ int launch_ring(const NormBackwardParams& p, const RingShape& s, int& blocks) {
     q.p = p;
     q.stages = s.stages;
     q.row_bytes = p.cols * (int)sizeof(T);
-    q.wait_limit = kWaitLimitCycles;
+    q.stall = stall_test("norm") ? 1 : 0;
+    q.wait_limit = q.stall ? kStallTestLimitCycles : kWaitLimitCycles;
     if (int rc = device_status_ptr(&q.status)) return rc;
     const int smem = s.stages * q.row_bytes * (p.dhidden ? 3 : 2);
     auto kernel = s.threads <= 256 ? rms_norm_backward_ring_kernel<T, 2, 256>

@@ -23,9 +23,10 @@ int device_status_ptr(int** dptr);
 
 constexpr long long kWaitLimitCycles = 4000000000ll;  // ~2 s at 1.9 GHz
 // Failure-detection test switch, read at every launch: TTC_TEST_STALL=gemm
-// (the TF32 GEMM kernels), =linear (the 16- and 8-bit products) or =chain (the
-// TMA-staged chain kernel) makes the kernel's TMA producer issue no loads at all, so nothing is ever in flight
-// and the consumers' waits run out after kStallTestLimitCycles (~1 ms); they
+// (the TF32 GEMM kernels), =linear (the 16- and 8-bit products), =norm (the norm's
+// gradients of long rows) or =chain (the TMA-staged chain kernel) makes the
+// kernel's producer issue no loads at all, so nothing is ever in flight and the
+// consumers' waits run out after kStallTestLimitCycles (~1 ms); they
 // set the status word, free what they hold and return, and the next
 // synchronisation reports TTC_ERR_TIMEOUT. Returns whether `family` stalls.
 constexpr long long kStallTestLimitCycles = 2000000ll;
