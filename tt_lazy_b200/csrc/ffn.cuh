@@ -52,6 +52,29 @@ inline int check_tensor(const char* op, const char* name, const void* p, int dty
     return TTC_OK;
 }
 
+#ifdef __CUDACC__
+#define TTC_HOST_DEVICE __host__ __device__ __forceinline__
+#else
+#define TTC_HOST_DEVICE inline
+#endif
+
+// Copies on their way into a warp's buffers, each with an mbarrier of its own: a bit
+// a buffer. One whose wait ran out stays on its way, and its barrier in the same
+// phase, so that it is waited for once more before the kernel leaves.
+struct CopiesInFlight {
+    uint32_t phase = 0, pending = 0;
+    TTC_HOST_DEVICE void sent(int buffer) { pending |= 1u << buffer; }
+    TTC_HOST_DEVICE bool on_its_way(int buffer) const { return pending >> buffer & 1; }
+    TTC_HOST_DEVICE uint32_t parity(int buffer) const { return phase >> buffer & 1; }
+    TTC_HOST_DEVICE bool waited(int buffer, bool landed) {
+        if (landed) {
+            phase ^= 1u << buffer;
+            pending &= ~(1u << buffer);
+        }
+        return landed;
+    }
+};
+
 inline size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
 
 // True when groups of 8 elements of `p` can be read with 16-byte accesses (two

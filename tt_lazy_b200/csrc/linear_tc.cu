@@ -191,7 +191,7 @@ __device__ __forceinline__ bool pair_epilogue(const ProductParams& q, uint8_t* s
     const uint32_t mine_addr = smem_u32(mine), res_bar = bar0 + 8u * (2 * kStages + 4 + 2 * w);
     const int tile_cols = GATED ? 128 : 256, chunks = tile_cols / W;
     const int num_tiles = q.m_tiles * q.n_tiles, nclusters = gridDim.x >> 1;
-    uint32_t res_phase = 0, res_pending = 0;  // a bit a buffer
+    CopiesInFlight residuals;
     int seq = 0;             // chunks sent so far: the next one goes through buffer seq & 1
     auto slot = [&](int buffer, int i) -> uint4& {  // 16-byte group i of this lane's row
         return *reinterpret_cast<uint4*>(mine + buffer * kBuffer + lane * kRow + ((i ^ (lane & 7)) << 4));
@@ -206,22 +206,20 @@ __device__ __forceinline__ bool pair_epilogue(const ProductParams& q, uint8_t* s
         return true;
     };
     auto fetch_residual = [&](int buffer, int row0, int first) {
-        res_pending |= 1u << buffer;
+        residuals.sent(buffer);
         if (lane == 0) {
             mbar_arrive_expect_tx(res_bar + 8u * buffer, kBuffer);
             tma_load_2d(mine_addr + buffer * kBuffer, &q.residual, res_bar + 8u * buffer, first, row0);
         }
     };
     auto await_residual = [&](int buffer) {
-        const bool ok = __all_sync(0xffffffffu, mbar_wait(res_bar + 8u * buffer, res_phase >> buffer & 1, q.wait_limit));
-        res_phase ^= 1u << buffer;
-        res_pending &= ~(1u << buffer);
-        return ok;
+        return residuals.waited(buffer, __all_sync(0xffffffffu, mbar_wait(res_bar + 8u * buffer, residuals.parity(buffer),
+                                                                          q.wait_limit)));
     };
     // Never leave with copies in flight.
     auto leave = [&](bool failed) {
         for (int k = 0; k < 2; ++k)
-            if (res_pending >> k & 1) await_residual(k);
+            if (residuals.on_its_way(k)) await_residual(k);
         if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         return failed;
     };
