@@ -24,7 +24,23 @@ static void copies_in_flight() {
     std::printf("copies_in_flight=ok\n");
 }
 
+static void set_up_once() {
+    ttc::OncePerDevice once;
+    int calls = 0, answer = TTC_ERR_CUDA;
+    auto prepare = [&] {
+        ++calls;
+        return answer;
+    };
+    expect(once(1, prepare) == TTC_ERR_CUDA && calls == 1, "a set-up that fails says so");
+    answer = TTC_OK;
+    expect(once(1, prepare) == TTC_OK && calls == 2, "and is tried again by the next call");
+    expect(once(1, prepare) == TTC_OK && calls == 2, "one that succeeded is not");
+    expect(once(0, prepare) == TTC_OK && calls == 3, "each device has its own");
+    std::printf("set_up_once=ok\n");
+}
+
 int main() {
     copies_in_flight();
+    set_up_once();
     return 0;
 }

@@ -27,3 +27,7 @@ def lines(tmp_path_factory):
 
 def test_a_copy_whose_wait_ran_out_is_waited_for_again(lines):
     assert "copies_in_flight=ok" in lines
+
+
+def test_a_set_up_that_failed_is_tried_again(lines):
+    assert "set_up_once=ok" in lines

@@ -52,6 +52,22 @@ inline int check_tensor(const char* op, const char* name, const void* p, int dty
     return TTC_OK;
 }
 
+// Set-up that a kernel needs once on each device. Counts as done only where
+// prepare() returned TTC_OK: after a failure the next call tries again.
+class OncePerDevice {
+   public:
+    template <class F>
+    int operator()(int device, F&& prepare) {
+        if (done_[device]) return TTC_OK;
+        if (int rc = prepare()) return rc;
+        done_[device] = true;
+        return TTC_OK;
+    }
+
+   private:
+    bool done_[kMaxDevices] = {};
+};
+
 #ifdef __CUDACC__
 #define TTC_HOST_DEVICE __host__ __device__ __forceinline__
 #else

@@ -1035,17 +1035,10 @@ unsigned instruction(const Product& p, bool a_mn, bool b_mn, int m, int n) {
            ((unsigned)(n >> 3) << 17) | ((unsigned)(m >> 4) << 24);
 }
 
-bool first_on_device(bool (&seen)[kMaxDevices]) {
-    bool& s = seen[rt().device];
-    const bool first = !s;
-    s = true;
-    return first;
-}
-
 template <bool F8, bool GATED, int DT>
 int launch_pair_as(ProductParams& q) {
     auto kernel = pair_kernel<F8, GATED, DT>;
-    static bool seen[kMaxDevices] = {};
+    static OncePerDevice once;
     static int most[kMaxDevices] = {};
     cudaLaunchConfig_t cfg;
     std::memset(&cfg, 0, sizeof cfg);
@@ -1056,14 +1049,16 @@ int launch_pair_as(ProductParams& q) {
     cfg.dynamicSmemBytes = kPairSmem;
     cfg.stream = rt().stream;
     int& clusters = most[rt().device];
-    if (first_on_device(seen)) {
-        TTC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
-        cfg.gridDim = dim3(2 * (rt().sm_count / 2), 1, 1);
-        if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess || clusters < 1) {
-            cudaGetLastError();
-            clusters = rt().sm_count / 2;
-        }
-    }
+    if (int rc = once(rt().device, [&]() -> int {
+            TTC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
+            cfg.gridDim = dim3(2 * (rt().sm_count / 2), 1, 1);
+            if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess || clusters < 1) {
+                cudaGetLastError();
+                clusters = rt().sm_count / 2;
+            }
+            return TTC_OK;
+        }))
+        return rc;
     const long long tiles = (long long)q.m_tiles * q.n_tiles;
     cfg.gridDim = dim3(2u * (unsigned)std::min<long long>(tiles, clusters), 1, 1);
     TTC_CUDA(cudaLaunchKernelEx(&cfg, kernel, q));
@@ -1109,21 +1104,23 @@ constexpr int kFullRing = 200 * 1024, kHalfRing = 104 * 1024;
 bool half_ring_holds(int tok) { return 3 * (kHalf + tok * kRow) <= kHalfRing; }  // three stages
 template <bool F8, int N>
 int tile_blocks_at_once(int cluster, int* blocks) {
-    static bool seen[kMaxDevices] = {};
+    static OncePerDevice once;
     static int most[kMaxDevices][kMaxSplits + 1] = {};
     auto kernel = tile_kernel<F8, N>;
-    if (first_on_device(seen)) {
-        TTC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448));
-        for (int c = 1; c <= kMaxSplits; ++c) {
-            const TileLaunch l(rt().sm_count / c * c, c, kFullRing);
-            int n = 0;
-            if (cudaOccupancyMaxActiveClusters(&n, kernel, &l.cfg) != cudaSuccess || n < 1) {
-                cudaGetLastError();
-                n = rt().sm_count / c;
+    if (int rc = once(rt().device, [&]() -> int {
+            TTC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448));
+            for (int c = 1; c <= kMaxSplits; ++c) {
+                const TileLaunch l(rt().sm_count / c * c, c, kFullRing);
+                int n = 0;
+                if (cudaOccupancyMaxActiveClusters(&n, kernel, &l.cfg) != cudaSuccess || n < 1) {
+                    cudaGetLastError();
+                    n = rt().sm_count / c;
+                }
+                most[rt().device][c] = n * c;
             }
-            most[rt().device][c] = n * c;
-        }
-    }
+            return TTC_OK;
+        }))
+        return rc;
     *blocks = most[rt().device][cluster];
     return TTC_OK;
 }

@@ -787,12 +787,12 @@ int launch_ring(const NormBackwardParams& p, const RingShape& s, int& blocks) {
     auto kernel = s.threads <= 256 ? rms_norm_backward_ring_kernel<T, 2, 256>
                   : s.chunks == 2  ? rms_norm_backward_ring_kernel<T, 2, 512>
                                    : rms_norm_backward_ring_kernel<T, 4, 512>;
-    static bool seen[kMaxDevices][3] = {};
-    bool& ready = seen[rt().device][s.threads <= 256 ? 0 : s.chunks / 2];
-    if (!ready) {
-        TTC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes));
-        ready = true;
-    }
+    static OncePerDevice once[3];  // one for each of the kernels
+    if (int rc = once[s.threads <= 256 ? 0 : s.chunks / 2](rt().device, [&]() -> int {
+            TTC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes));
+            return TTC_OK;
+        }))
+        return rc;
     blocks = (int)std::min<long long>(p.rows, (long long)s.per_sm * std::min(rt().sm_count, 148));
     kernel<<<(unsigned)blocks, s.threads, smem, rt().stream>>>(q);
     return check_cuda(cudaGetLastError(), "rms_norm_backward launch");
