@@ -333,7 +333,9 @@ int ttc_gemm_select_path(const ttc_gemm_desc* desc);
  * write e4m3 with one scale per row, which is the form the 8-bit products
  * read. The products take F16, BF16 and (forward only) E4M3 operands; fp32
  * products are ttc_gemm's. Every sum, norm and activation is computed in fp32
- * and rounded once, where a value is stored in its tensor's type.
+ * and rounded once, where a value is stored in its tensor's type. An activation
+ * z s (s the factor in [0, 1] of its definition) is off by 2^-21 (1 + |ln s|) of
+ * its value before that rounding, in the negative tail too; below 2^-119 it may be 0.
  *
  * Layout. Matrices are row-major with a leading dimension in elements. With
  * trans_w = 0 a weight is stored [K, N] as for ttc_gemm, with trans_w = 1

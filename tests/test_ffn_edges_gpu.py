@@ -2,12 +2,12 @@
 values near the limits of the types, special values, and variants that ordinary
 shapes seldom take. Tolerances as in test_ffn_gpu.py (u(t) is half a step of the
 type t relative to the value), unless a test states its own."""
-import math  # noqa: F401
+import math
 
 import pytest
 import torch
 
-from test_ffn_gpu import EPS, TINY, U, Mat, act64, gen, lib, norm64, normwise, product64, product_inputs, ptr, rand, scratch, within  # noqa: F401,E501
+from test_ffn_gpu import EPS, T, TINY, U, Mat, act64, gen, lib, norm64, normwise, product64, product_inputs, ptr, rand, scratch, within  # noqa: F401,E501
 
 pytestmark = pytest.mark.gpu
 
@@ -47,3 +47,97 @@ def test_norm_gradient_wait_expiry_is_reported_and_the_context_stays_usable(lib,
     lib.synchronize()
     for a, b in zip(first[:2], again[:2]):
         assert torch.isfinite(a.t).all() and torch.equal(a.t, b.t)
+
+
+# ------------------------------------------------------------------------------------------------ activations
+ACTS = ["none", "relu", "silu", "gelu", "gelu_tanh"]
+
+
+def factor64(act, z):
+    """(s, s') of act(z) = z s(z): the factor of each activation and its derivative."""
+    if act == "silu":
+        s = torch.sigmoid(z)
+        return s, s * torch.sigmoid(-z)
+    if act == "gelu":
+        # by erfc: torch.special.ndtr is (1 + erf) / 2, which keeps nothing of the tail
+        return torch.special.erfc(-z / math.sqrt(2)) / 2, torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    if act == "gelu_tanh":
+        a = math.sqrt(8 / math.pi)
+        t = a * (z + 0.044715 * z ** 3)
+        s = torch.sigmoid(t)
+        return s, s * torch.sigmoid(-t) * a * (1 + 0.134145 * z * z)
+    s = (z > 0).double() if act == "relu" else torch.ones_like(z)
+    return s, torch.zeros_like(z)
+
+
+def tail(dtype, n):
+    """n values over [-10, 0] and a few positive ones, in the type."""
+    z = torch.linspace(-10, 0, n - 40, dtype=torch.float64, device="cuda")
+    return torch.cat([z, torch.linspace(0, 10, 40, dtype=torch.float64, device="cuda")]).to(T[dtype])
+
+
+def relative(act, z):
+    """How far an activation's factor may be off: 2^-21 (1 + |ln s|) of itself. The argument of its exponential is
+    |ln s| large and goes through at most five roundings (2^-24 of it each), 2^x and 1 / x are good to 2^-22, and the
+    fitted factor of the normal distribution to 2^-23."""
+    s = factor64(act, z)[0]
+    return 2.0 ** -21 * (1 - torch.log(s.clamp_min(1e-300)))
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("dtype,out", [("f16", "f16"), ("bf16", "bf16"), ("bf16", "f32"), ("f16", "f32")])
+@pytest.mark.parametrize("M,N,odd", [(300, 72, False), (300, 67, True), (2560, 2048, False), (2560, 2050, True)])
+def test_activation_tails_keep_their_relative_accuracy(lib, act, dtype, out, M, N, odd):
+    """act(z) itself: one term a product (exact in fp32), w = 1. On each kernel, and where results leave by
+    elements. The gated product with up = 1 likewise."""
+    K = 8
+    z = tail(dtype, M)
+    x, w, wu = Mat(M, K, dtype, fill=0), Mat(N, K, dtype, fill=0), Mat(N, K, dtype, fill=0)
+    x.t[:, 0] = z
+    x.t[:, 1] = 1
+    w.t[:, 0] = 1
+    wu.t[:, 1] = 1
+    zz = z.double()
+    want = (zz * factor64(act, zz)[0]).view(M, 1).expand(M, N)
+    tol = (U[out] + relative(act, zz).view(M, 1)) * want.abs() + TINY[out] + 2.0 ** -119
+    pad = 3 if odd else 0
+    for gated in (False, True):
+        y = Mat(M, N, out, pad)
+        common = dict(dtype=lib.DTYPES[dtype], y_dtype=lib.DTYPES[out], trans_w=True, act=lib.ACTIVATIONS[act])
+        if gated:
+            d = lib.gated_linear_desc(M, N, K, x.ptr, K, w.ptr, wu.ptr, K, y.ptr, y.ld, **common)
+            lib.gated_linear(d, scratch(lib, d))
+        else:
+            d = lib.linear_desc(M, N, K, x.ptr, K, w.ptr, K, y.ptr, y.ld, **common)
+            lib.linear(d, scratch(lib, d))
+        within(y.t, want, tol, f"{act} gated {gated}")
+        assert y.untouched_outside()
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("pad", [0, 3])
+def test_activation_gradients_in_the_tails(lib, act, dtype, pad):
+    """dz, dg and du themselves: dx with w = 1 in one row and dy = 1 (up = 1). dz = s + z s' is off by what s is, and
+    s' (a product of s, 1 - s or the same exponential, at most three factors) by three times that."""
+    M, K = 300, 8
+    z = tail(dtype, M)
+    zz = z.double()
+    s, ds = factor64(act, zz)
+    slope = s + zz * ds
+    rel = relative(act, zz)
+    tol_slope = U[dtype] * slope.abs() + rel * s + 3 * rel * (zz * ds).abs() + TINY[dtype] + 2.0 ** -119
+    tol_value = (U[dtype] + rel) * (zz * s).abs() + TINY[dtype] + 2.0 ** -119
+    pre, one = Mat(M, 1, dtype, pad, fill=z.view(M, 1)), Mat(M, 1, dtype, pad, fill=1)
+    x = Mat(M, K, dtype, fill=1)
+    w1, w0 = Mat(1, K, dtype, fill=1), Mat(1, K, dtype, fill=0)
+    dx = Mat(M, K, dtype)
+    d = lib.linear_backward_desc(M, 1, K, one.ptr, one.ld, x.ptr, K, w1.ptr, K, lib.DTYPES[dtype], trans_w=True,
+                                 act=lib.ACTIVATIONS[act], pre=pre.ptr, ldp=pre.ld, dx=dx.ptr, lddx=K)
+    lib.linear_backward(d, scratch(lib, d))
+    within(dx.t, slope.view(M, 1).expand(M, K), tol_slope.view(M, 1), "dz")
+    for wg, wu, want, tol, name in ((w1, w0, slope, tol_slope, "dg"), (w0, w1, zz * s, tol_value, "du")):
+        d = lib.gated_linear_backward_desc(M, 1, K, one.ptr, one.ld, x.ptr, K, wg.ptr, wu.ptr, K, pre.ptr, one.ptr, pre.ld,
+                                           lib.DTYPES[dtype], trans_w=True, act=lib.ACTIVATIONS[act], dx=dx.ptr, lddx=K)
+        lib.gated_linear_backward(d, scratch(lib, d))
+        within(dx.t, want.view(M, 1).expand(M, K), tol.view(M, 1), name)

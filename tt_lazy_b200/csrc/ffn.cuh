@@ -280,9 +280,12 @@ __device__ __forceinline__ void store8(T* p, int n, bool vec, const float (&v)[8
 }
 
 // Activations in fp32, with the hardware's approximate 2^x and 1 / x (good to
-// 2^-22; 2^x takes the rounding of its argument besides), far below the 2^-8
-// .. 2^-11 of the types the results are rounded to; an fp32 result of the
-// products carries their accumulation error already.
+// 2^-22). Each is z times a factor s in [0, 1] and is off by at most
+// 2^-21 (1 + |ln s|) of its own value: s is an exponential of a rounded argument,
+// and that of -80 is known to 80 roundings. So the tails keep their leading digits
+// (f16 and bf16 results are the exact ones to within half a step and 2^-15), down to
+// 2^-119, below which a result may come out as 0: the approximations flush what is
+// below 2^-126.
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -295,18 +298,26 @@ __device__ __forceinline__ float rcp_approx(float x) {
 }
 constexpr float kLog2E = 1.4426950408889634f;
 __device__ __forceinline__ float sigmoid_f32(float z) { return rcp_approx(1.0f + exp2_approx(-kLog2E * z)); }
-// The normal distribution function at z by Abramowitz and Stegun 7.1.26,
-// erfc(x) = (a1 t + ... + a5 t^5) e^(-x^2) + 1.5e-7 at most, t = 1 / (1 + p x):
-// one exponential, which the density needs too, and one reciprocal: half the
-// instructions of erff with a separate exponential.
+// The normal distribution function at z, and e = e^(-z^2 / 2), which its density
+// needs too. For x >= 0 the function at -x is e times a smooth decreasing factor
+// (half the scaled complementary error function of x / sqrt(2)), here t P(t) with
+// t = 1 / (1 + 0.305 x) and P of degree 7: fitted to that factor over 0 <= x <= 14
+// (past 13.2 e is 0), minimising the greatest relative error by iterated reweighting
+// (Lawson), 1e-7. Relative, since gelu's negative tail is this value itself: a form
+// with a bounded absolute error (1.5e-7) was off by 5e-4 of it at -4 and 1e-2 at -8.
+// Three multiply-adds more than that form, and half the instructions of erff with a
+// separate exponential.
 __device__ __forceinline__ float normal_cdf(float z, float& e) {
-    const float t = rcp_approx(fmaf(0.3275911f * 0.70710678118654752f, fabsf(z), 1.0f));
+    const float t = rcp_approx(fmaf(0.305f, fabsf(z), 1.0f));
     e = exp2_approx(-0.5f * kLog2E * z * z);
-    float q = fmaf(t, 1.061405429f, -1.453152027f);
-    q = fmaf(t, q, 1.421413741f);
-    q = fmaf(t, q, -0.284496736f);
-    q = fmaf(t, q, 0.254829592f);
-    q = 0.5f * t * q * e;
+    float q = fmaf(t, 0.036699191f, -0.1529883f);
+    q = fmaf(t, q, 0.18571687f);
+    q = fmaf(t, q, -0.037976794f);
+    q = fmaf(t, q, 0.12102166f);
+    q = fmaf(t, q, 0.10342088f);
+    q = fmaf(t, q, 0.1224668f);
+    q = fmaf(t, q, 0.12163974f);
+    q = t * q * e;
     return z < 0.0f ? q : 1.0f - q;
 }
 constexpr float kGeluTanhScale = 1.5957691216057308f;  // 2 sqrt(2 / pi): (1 + tanh t) / 2 = sigmoid(2 t)
