@@ -376,7 +376,8 @@ typedef enum {
  * x + residual; `hidden` receives that sum rounded to dtype.
  * y_dtype is dtype, or E4M3: then scales[r] = max(max_c |y(r, c)| / 448, 2^-126)
  * and y holds e4m3(y(r, c) * (1 / scales[r])), rounded to nearest even and
- * saturated at +-448 (NaN stays NaN).
+ * saturated at +-448. A row with a NaN or an infinity among its sums h has the
+ * scale NaN and NaN in all of q.
  * `hidden` and `y` may be `x` or `residual` themselves (same address and
  * leading dimension, same type); no other overlap is allowed. */
 typedef struct {

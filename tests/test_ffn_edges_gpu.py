@@ -141,3 +141,43 @@ def test_activation_gradients_in_the_tails(lib, act, dtype, pad):
                                            lib.DTYPES[dtype], trans_w=True, act=lib.ACTIVATIONS[act], dx=dx.ptr, lddx=K)
         lib.gated_linear_backward(d, scratch(lib, d))
         within(dx.t, want.view(M, 1).expand(M, K), tol.view(M, 1), name)
+
+
+# ----------------------------------------------------------------------------------------------- rows of the norm
+# One row length for each of the norm's kernels: a warp a row (one, two, four chunks), a block, a cluster, two passes.
+ROW_LENGTHS = [64, 300, 1000, 2000, 6000, 40000]
+
+
+def run_norm(lib, x, w, dtype, out, pad=0, eps=EPS, residual=None):
+    """(y, scales, hidden) of the rows of x, the two last ones where they exist."""
+    rows, cols = x.shape
+    X, W = Mat(rows, cols, dtype, pad, fill=x), Mat(1, cols, dtype, fill=w)
+    res, hid = (Mat(rows, cols, dtype, pad, fill=residual), Mat(rows, cols, dtype, pad)) if residual is not None else (None, None)
+    y, sc = Mat(rows, cols, out, pad), Mat(1, rows, "f32") if out == "e4m3" else None
+    lib.rms_norm(lib.rms_norm_desc(rows, cols, X.ptr, X.ld, W.ptr, y.ptr, y.ld, lib.DTYPES[dtype], y_dtype=lib.DTYPES[out],
+                                   eps=eps, scales=ptr(sc), residual=ptr(res), ldr=X.ld, hidden=ptr(hid), ldh=X.ld))
+    assert y.untouched_outside()
+    return y.t, None if sc is None else sc.t[0], None if hid is None else hid.t
+
+
+@pytest.mark.parametrize("cols", ROW_LENGTHS)
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("pad", [0, 3])
+def test_e4m3_scales_show_rows_with_nan_and_infinities(lib, cols, dtype, pad):
+    """Such a row has the scale NaN and NaN throughout, wherever in the row it is; a row of zeros has the smallest
+    scale; the rows beside them are what they are without it."""
+    g = gen(cols)
+    x, w = rand(g, 9, cols), 1 + rand(g, 1, cols, 0.1)
+    clean = run_norm(lib, x, w, dtype, "e4m3", pad)
+    bad = {1: (0, "nan"), 3: (cols - 1, "nan"), 5: (cols // 2, "inf"), 7: (cols - 1, "-inf")}
+    for r, (c, v) in bad.items():
+        x[r, c] = float(v)
+    x[4] = 0
+    y, sc, _ = run_norm(lib, x, w, dtype, "e4m3", pad)
+    for r in range(9):
+        if r in bad:
+            assert torch.isnan(sc[r]) and torch.isnan(y[r].double()).all(), r
+        elif r == 4:
+            assert sc[r] == 2.0 ** -126 and (y[r].double() == 0).all()
+        else:
+            assert sc[r] == clean[1][r] and torch.equal(y[r].double(), clean[0][r].double()), r

@@ -114,6 +114,14 @@ __device__ __forceinline__ void load_weight(const void* weight, bool f32, int co
         }
 }
 
+// The larger, or NaN where either is: a row's e4m3 scale has to show that the row
+// holds one.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+    return m;
+}
+
 // Reduces a and b over a row's threads, in a fixed order; MAX: b is a maximum.
 // ONE: the row is one warp's. Else `slots` is one of two buffers that the rows
 // use in turn, so that one barrier a row is enough; in a cluster of more than
@@ -127,7 +135,7 @@ __device__ __forceinline__ void reduce_row(float& a, float& b, float2* slots, in
         for (int o = 16; o > 0; o >>= 1) {
             a += __shfl_xor_sync(0xffffffffu, a, o);
             const float x = __shfl_xor_sync(0xffffffffu, b, o);
-            b = MAX ? fmaxf(b, x) : b + x;
+            b = MAX ? max_nan(b, x) : b + x;
         }
     };
     warp();
@@ -141,7 +149,7 @@ __device__ __forceinline__ void reduce_row(float& a, float& b, float2* slots, in
             for (int i = 1; i < warps; ++i) {
                 const float2 s = slots[i];
                 a += s.x;
-                b = MAX ? fmaxf(b, s.y) : b + s.y;
+                b = MAX ? max_nan(b, s.y) : b + s.y;
             }
         } else {
             if (lane < blocks)
@@ -155,7 +163,7 @@ __device__ __forceinline__ void reduce_row(float& a, float& b, float2* slots, in
             const float2 s = lane < n ? slots[lane] : make_float2(0.0f, 0.0f);
             const float2 s2 = lane + 32 < n ? slots[lane + 32] : make_float2(0.0f, 0.0f);
             a = s.x + s2.x;
-            b = MAX ? fmaxf(s.y, s2.y) : s.y + s2.y;
+            b = MAX ? max_nan(s.y, s2.y) : s.y + s2.y;
             warp();
         }
     }
@@ -226,7 +234,7 @@ __global__ void __launch_bounds__(ONE ? 32 * kWarpRows : kMaxBlock) rms_norm_ker
 #pragma unroll
             for (int i = 0; i < kPer<T>; ++i) {
                 sum += h[c][i] * h[c][i];
-                if (sizeof(Y) == 1) top = fmaxf(top, fabsf(h[c][i] * w[c][i]));
+                if (sizeof(Y) == 1) top = max_nan(top, fabsf(h[c][i] * w[c][i]));
             }
         }
         fetch(r + step);
@@ -236,7 +244,7 @@ __global__ void __launch_bounds__(ONE ? 32 * kWarpRows : kMaxBlock) rms_norm_ker
         float k = rsqrtf(sum / (float)p.cols + p.eps);
         float inv = 1.0f;
         if (sizeof(Y) == 1) {
-            const float scale = fmaxf(top * k * (1.0f / 448.0f), kMinScale);
+            const float scale = max_nan(top * k * (1.0f / 448.0f), kMinScale);
             inv = 1.0f / scale;
             if (l.t == 0) p.scales[r] = scale;
         }
@@ -523,13 +531,13 @@ __global__ void __launch_bounds__(kWide) rms_norm_wide_kernel(const __grid_const
             float h = to_f32<T>(x[c]);
             if (res) h += to_f32<T>(res[c]);
             sum += h * h;
-            if (sizeof(Y) == 1) top = fmaxf(top, fabsf(h * weight(c)));
+            if (sizeof(Y) == 1) top = max_nan(top, fabsf(h * weight(c)));
         }
         reduce_row<false, true>(sum, top, slots[parity], 1);
         const float k = rsqrtf(sum / (float)p.cols + p.eps);
         float inv = 1.0f;
         if (sizeof(Y) == 1) {
-            const float scale = fmaxf(top * k * (1.0f / 448.0f), kMinScale);
+            const float scale = max_nan(top * k * (1.0f / 448.0f), kMinScale);
             inv = 1.0f / scale;
             if (threadIdx.x == 0) p.scales[r] = scale;
         }
