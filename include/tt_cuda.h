@@ -373,7 +373,9 @@ typedef enum {
 
 /* Root-mean-square norm over the last dimension of x [rows, cols], with the
  * residual stream's addition in front. The norm is of the fp32 sum
- * x + residual; `hidden` receives that sum rounded to dtype.
+ * x + residual; `hidden` receives that sum rounded to dtype. Finite rows whose
+ * squares leave fp32's range (|h| above 2^64, or tiny with eps below 2^-100) are
+ * summed times a power of two, here and in the gradients.
  * y_dtype is dtype, or E4M3: then scales[r] = max(max_c |y(r, c)| / 448, 2^-126)
  * and y holds e4m3(y(r, c) * (1 / scales[r])), rounded to nearest even and
  * saturated at +-448. A row with a NaN or an infinity among its sums h has the

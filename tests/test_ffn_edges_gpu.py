@@ -181,3 +181,95 @@ def test_e4m3_scales_show_rows_with_nan_and_infinities(lib, cols, dtype, pad):
             assert sc[r] == 2.0 ** -126 and (y[r].double() == 0).all()
         else:
             assert sc[r] == clean[1][r] and torch.equal(y[r].double(), clean[0][r].double()), r
+
+
+def far_rows(g, rows, cols):
+    """Rows of ordinary size, of 1e25, close to the largest value, of 1e-25 and of 1e-30, in turn."""
+    x = rand(g, rows, cols)
+    size = torch.tensor([1.0, 1e25, 1.0, 1e-25, 1e-30], device="cuda", dtype=torch.float64).repeat(rows // 5 + 1)[:rows]
+    x = x * size.view(rows, 1)
+    x[2::5] *= 1.5e38 / x[2::5].abs().amax(dim=1, keepdim=True)
+    return x
+
+
+FAR = [(2500, 64), (2500, 300), (2500, 1000), (2500, 2000), (700, 6000), (330, 40000)]
+
+
+@pytest.mark.parametrize("rows,cols", FAR)
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("form", ["plain", "residual odd", "e4m3", "e4m3 residual odd"])
+@pytest.mark.parametrize("eps", [EPS, 0.0])
+def test_norm_of_rows_whose_squares_leave_fp32(lib, rows, cols, dtype, form, eps):
+    """Finite rows have their formula's value whatever their size, beside ordinary rows; scaling by a power of two
+    is exact, so the bounds are those of ordinary rows."""
+    g = gen(rows + cols)
+    pad = 3 if "odd" in form else 0
+    x = Mat(rows, cols, dtype, fill=far_rows(g, rows, cols)).f64()
+    res = Mat(rows, cols, dtype, fill=far_rows(g, rows, cols)).f64() if "residual" in form else None
+    w = Mat(1, cols, dtype, fill=1 + rand(g, 1, cols, 0.1)).f64()
+    out = "e4m3" if "e4m3" in form else dtype
+    y, sc, hid = run_norm(lib, x, w, dtype, out, pad, eps, res)
+    h = x if res is None else x + res
+    want = h / torch.sqrt((h * h).mean(dim=1, keepdim=True) + eps) * w
+    rel = ((cols / 32 + 16) / 2 + 10) * 2.0 ** -24
+    if out != "e4m3":
+        within(y, want, (U[out] + rel) * want.abs() + TINY[out], "y")
+    else:
+        scale = (want.abs().amax(dim=1) / 448).clamp_min(2.0 ** -126)
+        within(sc, scale, (rel + 2.0 ** -22) * scale, "scales")
+        q = want / scale[:, None]
+        within(y, q, (U["e4m3"] + 2 * rel + 2.0 ** -22) * q.abs() + TINY["e4m3"], "q")
+    if hid is not None:
+        within(hid, h, (U[dtype] + 2.0 ** -24) * h.abs() + TINY[dtype], "hidden")
+
+
+@pytest.mark.parametrize("rows,cols", FAR)
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_norm_of_far_rows_in_place(lib, rows, cols, dtype):
+    g = gen(rows)
+    x, res = (Mat(rows, cols, dtype, fill=far_rows(g, rows, cols)) for _ in range(2))
+    w = Mat(1, cols, dtype, fill=1 + rand(g, 1, cols, 0.1))
+    want, _, want_h = run_norm(lib, x.f64(), w.f64(), dtype, dtype, eps=0.0, residual=res.f64())
+    lib.rms_norm(lib.rms_norm_desc(rows, cols, x.ptr, cols, w.ptr, x.ptr, cols, lib.DTYPES[dtype], eps=0.0,
+                                   residual=res.ptr, ldr=cols, hidden=res.ptr, ldh=cols))
+    assert torch.equal(x.t, want) and torch.equal(res.t, want_h)
+
+
+@pytest.mark.parametrize("rows,cols", FAR)
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("form", ["plain", "dhidden", "odd"])
+@pytest.mark.parametrize("eps", [EPS, 0.0])
+def test_norm_gradients_of_rows_whose_squares_leave_fp32(lib, rows, cols, dtype, form, eps):
+    """As above, for the gradients; dx over dy gives the same, and so does a call without dweight."""
+    g = gen(rows + 3 * cols)
+    pad = 3 if form == "odd" else 0
+    hid = Mat(rows, cols, dtype, pad, fill=far_rows(g, rows, cols))
+    dy = Mat(rows, cols, dtype, pad, fill=rand(g, rows, cols))
+    dh = Mat(rows, cols, dtype, pad, fill=rand(g, rows, cols)) if form == "dhidden" else None
+    w = Mat(1, cols, dtype, fill=1 + rand(g, 1, cols, 0.1))
+    dx, dw = Mat(rows, cols, dtype, pad), Mat(1, cols, dtype)
+
+    def call(dx, dw):
+        d = lib.rms_norm_backward_desc(rows, cols, dy.ptr, dy.ld, hid.ptr, hid.ld, w.ptr, dx.ptr, dx.ld, ptr(dw),
+                                       lib.DTYPES[dtype], eps=eps, dhidden=ptr(dh), lddh=cols)
+        lib.rms_norm_backward(d, scratch(lib, d))
+
+    call(dx, dw)
+    h, e, ww = hid.f64(), dy.f64(), w.f64()
+    r = 1 / torch.sqrt((h * h).mean(dim=1, keepdim=True) + eps)
+    first = r * e * ww
+    unit = h * r
+    second = r * unit * (e * ww * unit).sum(1, keepdim=True) / cols
+    spread = r * unit.abs() * (e * ww * unit).abs().sum(1, keepdim=True) / cols
+    want = first - second + (dh.f64() if dh else 0)
+    rel = (1.5 * (cols / 32 + 16) + 20) * 2.0 ** -24
+    within(dx.t, want, U[dtype] * want.abs() + rel * (first.abs() + spread) + 2.0 ** -23 * want.abs() + TINY[dtype], "dx")
+    terms = e * unit
+    relw = rel + (min(rows, rows / 148 + 2) + 700) * 2.0 ** -24
+    within(dw.t[0], terms.sum(0), U[dtype] * terms.sum(0).abs() + relw * terms.abs().sum(0) + TINY[dtype], "dweight")
+    assert dx.untouched_outside() and dw.untouched_outside()
+    without = Mat(rows, cols, dtype, pad)
+    call(without, None)
+    assert torch.equal(without.t, dx.t)
+    call(dy, None)
+    assert torch.equal(dy.t, dx.t)

@@ -2,6 +2,7 @@
 // (ttc_rms_norm) and its gradients (ttc_rms_norm_backward).
 #include <algorithm>
 #include <cstring>
+#include <type_traits>
 
 #include "ffn.cuh"
 #include "tc_util.cuh"
@@ -171,6 +172,19 @@ __device__ __forceinline__ void reduce_row(float& a, float& b, float2* slots, in
 
 constexpr float kMinScale = 1.17549435e-38f;  // 2^-126
 
+// Squares of finite values can leave fp32: |h| from 2^64, and below 2^-63 where eps
+// does not cover them. The sums of such a row, infinite or next to nothing, are
+// taken again with the row times this power of two, exactly; 1 for any other row,
+// which pays a comparison. With it the squares of 2^30 values of 2^128 add up to
+// 2^126, and values of which the sum of squares was below 2^-90 to at most 2^110.
+// F16 rows cannot get there.
+template <class T>
+__device__ __forceinline__ float range_factor(float sum, float eps) {
+    if (std::is_same<T, __half>::value) return 1.0f;
+    if (sum > 3.402823466e38f) return 8.271806126e-25f;                                // 2^-80
+    return sum < 8.077935669e-28f && eps < 7.888609052e-31f ? 1.267650600e30f : 1.0f;  // 2^-90, 2^-100, 2^100
+}
+
 struct NormParams {
     long long rows;
     int cols;
@@ -203,6 +217,73 @@ __device__ __forceinline__ RowPlace row_place(int cluster) {
 constexpr int kWarpRows = 4;  // rows of a block whose rows are one warp's
 constexpr int kMaxBlock = 256;
 
+// a and b over the block; MAX: b is a maximum.
+template <bool MAX>
+__device__ __forceinline__ float2 reduce_block(float a, float b) {
+    __shared__ float2 of_warp[32];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        a += __shfl_xor_sync(0xffffffffu, a, o);
+        const float x = __shfl_xor_sync(0xffffffffu, b, o);
+        b = MAX ? max_nan(b, x) : b + x;
+    }
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) of_warp[threadIdx.x >> 5] = make_float2(a, b);
+    __syncthreads();
+    float2 s = of_warp[0];
+    for (int i = 1; i < (int)blockDim.x / 32; ++i) {
+        s.x += of_warp[i].x;
+        s.y = MAX ? max_nan(s.y, of_warp[i].y) : s.y + of_warp[i].y;
+    }
+    return s;
+}
+
+// The rows of this block (of this cluster, by its first block) that need a
+// range_factor. The kernels pass over them, leaving every tensor as it is, and come
+// here at their end, so that the usual rows pay a comparison and few registers:
+// nothing to 5 % (gradients of 16384 x 4096 in bf16 94.6 -> 96.0 us, of 4096 x 16384
+// 125 -> 131; second sums inside the rows' loop spilled 70 bytes of that kernel, and
+// 64 rows of 40000 took 45 us instead of 30). `n` rows of the block at a time, as its
+// loop takes them.
+template <class T, class Y>
+__device__ __forceinline__ void late_rows(const NormParams& p, int n) {
+    auto weight = [&](int c) {
+        return p.weight_f32 ? static_cast<const float*>(p.weight)[c] : to_f32<T>(static_cast<const T*>(p.weight)[c]);
+    };
+    const long long step = (long long)(gridDim.x / p.cluster) * n;
+    for (long long base = (long long)(blockIdx.x / p.cluster) * n; base < p.rows; base += step)
+        for (long long r = base; r < min(base + n, p.rows); ++r) {
+            const T* x = static_cast<const T*>(p.x) + r * p.ldx;
+            const T* res = p.residual ? static_cast<const T*>(p.residual) + r * p.ldr : nullptr;
+            T* hid = p.hidden ? static_cast<T*>(p.hidden) + r * p.ldh : nullptr;
+            Y* y = static_cast<Y*>(p.y) + r * p.ldy;
+            auto row = [&](int c) { return res ? to_f32<T>(x[c]) + to_f32<T>(res[c]) : to_f32<T>(x[c]); };
+            float sum = 0.0f, top = 0.0f;
+            for (int c = threadIdx.x; c < p.cols; c += blockDim.x) sum += row(c) * row(c);
+            const float f = range_factor<T>(reduce_block<true>(sum, 0.0f).x, p.eps);
+            if (f == 1.0f) continue;
+            sum = 0.0f;
+            for (int c = threadIdx.x; c < p.cols; c += blockDim.x) {
+                const float h = row(c) * f;
+                sum += h * h;
+                if (sizeof(Y) == 1) top = max_nan(top, fabsf(h * weight(c)));
+            }
+            const float2 s = reduce_block<true>(sum, top);
+            const float k = rsqrtf(s.x / (float)p.cols + p.eps * f * f);
+            float inv = 1.0f;
+            if (sizeof(Y) == 1) {
+                const float scale = max_nan(s.y * k * (1.0f / 448.0f), kMinScale);
+                inv = 1.0f / scale;
+                if (threadIdx.x == 0) p.scales[r] = scale;
+            }
+            for (int c = threadIdx.x; c < p.cols; c += blockDim.x) {  // an element is read before it may be written over
+                const float h = row(c);
+                if (hid) hid[c] = from_f32<T>(h);
+                y[c] = from_f32<Y>(h * f * k * weight(c) * inv);
+            }
+        }
+}
+
 template <class T, class Y, bool VEC, bool ONE, int C>
 __global__ void __launch_bounds__(ONE ? 32 * kWarpRows : kMaxBlock) rms_norm_kernel(const __grid_constant__ NormParams p) {
     __shared__ float2 slots[2][kSlots];
@@ -220,6 +301,7 @@ __global__ void __launch_bounds__(ONE ? 32 * kWarpRows : kMaxBlock) rms_norm_ker
         if (res) load_row<T, VEC, C>(res + row * p.ldr, p.cols, l, rs);
     };
     fetch(r);
+    bool late = false;
     for (int parity = 0; r < p.rows; r += step, parity ^= 1) {
         float h[C][kPer<T>], sum = 0.0f, top = 0.0f;
 #pragma unroll
@@ -240,20 +322,35 @@ __global__ void __launch_bounds__(ONE ? 32 * kWarpRows : kMaxBlock) rms_norm_ker
         fetch(r + step);
         reduce_row<ONE, true>(sum, top, slots[parity], p.cluster);
         // All of the row is in registers now: x, residual, hidden and y may be the same memory.
-        if (p.hidden) store_row<T, T, VEC, C>(static_cast<T*>(p.hidden) + r * p.ldh, p.cols, l, h);
+        const bool usual = range_factor<T>(sum, p.eps) == 1.0f;  // the same for all of the row's threads
+        late |= !usual;
+        if (p.hidden && usual) store_row<T, T, VEC, C>(static_cast<T*>(p.hidden) + r * p.ldh, p.cols, l, h);
         float k = rsqrtf(sum / (float)p.cols + p.eps);
         float inv = 1.0f;
         if (sizeof(Y) == 1) {
             const float scale = max_nan(top * k * (1.0f / 448.0f), kMinScale);
             inv = 1.0f / scale;
-            if (l.t == 0) p.scales[r] = scale;
+            if (l.t == 0 && usual) p.scales[r] = scale;
         }
 #pragma unroll
         for (int c = 0; c < C; ++c)
 #pragma unroll
             for (int i = 0; i < kPer<T>; ++i) h[c][i] = h[c][i] * k * w[c][i] * inv;
-        store_row<T, Y, VEC, C>(static_cast<Y*>(p.y) + r * p.ldy, p.cols, l, h);
+        if (usual) store_row<T, Y, VEC, C>(static_cast<Y*>(p.y) + r * p.ldy, p.cols, l, h);
     }
+    if (ONE && !std::is_same<T, __half>::value) late = __syncthreads_or(late);
+    if (late) {
+        if (p.cluster > 1) cluster_sync();
+        if (blockIdx.x % p.cluster == 0) late_rows<T, Y>(p, ONE ? kWarpRows : 1);
+    }
+}
+
+// What a row's gradients need, from its sums of the row times f (range_factor):
+// rstd, and k with hidden rstd^2 mean(dy weight hidden) = hidden k.
+__device__ __forceinline__ void gradient_scalars(float sum, float dot, float eps, int cols, float f, float& rstd, float& k) {
+    const float scaled = rsqrtf(sum / (float)cols + eps * f * f);
+    rstd = scaled * f;
+    k = dot * scaled * scaled / (float)cols * f;
 }
 
 struct NormBackwardParams {
@@ -267,6 +364,43 @@ struct NormBackwardParams {
     int weight_f32, weight_vec;  // weight_vec: of dtype, 16-byte aligned
     int cluster;
 };
+
+// The gradients of such rows; `part` is the block's or cluster's row of the partials,
+// complete but for these.
+template <class T>
+__device__ __forceinline__ void late_rows(const NormBackwardParams& p, int n, float* part) {
+    auto weight = [&](int c) {
+        return p.weight_f32 ? static_cast<const float*>(p.weight)[c] : to_f32<T>(static_cast<const T*>(p.weight)[c]);
+    };
+    const long long step = (long long)(gridDim.x / p.cluster) * n;
+    for (long long base = (long long)(blockIdx.x / p.cluster) * n; base < p.rows; base += step)
+        for (long long r = base; r < min(base + n, p.rows); ++r) {
+            const T* dy = static_cast<const T*>(p.dy) + r * p.lddy;
+            const T* hid = static_cast<const T*>(p.hidden) + r * p.ldh;
+            const T* dh = p.dhidden ? static_cast<const T*>(p.dhidden) + r * p.lddh : nullptr;
+            T* dx = static_cast<T*>(p.dx) + r * p.lddx;
+            float sum = 0.0f, dot = 0.0f;
+            for (int c = threadIdx.x; c < p.cols; c += blockDim.x) sum += to_f32<T>(hid[c]) * to_f32<T>(hid[c]);
+            const float f = range_factor<T>(reduce_block<false>(sum, 0.0f).x, p.eps);
+            if (f == 1.0f) continue;
+            sum = 0.0f;
+            for (int c = threadIdx.x; c < p.cols; c += blockDim.x) {
+                const float h = to_f32<T>(hid[c]) * f;
+                sum += h * h;
+                dot += to_f32<T>(dy[c]) * weight(c) * h;
+            }
+            const float2 s = reduce_block<false>(sum, dot);
+            float rstd, k;
+            gradient_scalars(s.x, s.y, p.eps, p.cols, f, rstd, k);
+            for (int c = threadIdx.x; c < p.cols; c += blockDim.x) {
+                const float h = to_f32<T>(hid[c]), g = to_f32<T>(dy[c]);
+                float d = rstd * (g * weight(c) - h * k);
+                if (dh) d += to_f32<T>(dh[c]);
+                if (part) part[c] += g * (h * rstd);
+                dx[c] = from_f32<T>(d);
+            }
+        }
+}
 
 // The weight's gradient stays in registers over all of a block's rows and goes
 // out once as the block's row of the partials; no atomics.
@@ -291,6 +425,7 @@ __global__ void __launch_bounds__(ONE ? 32 * kWarpRows : kMaxBlock, ONE ? (C == 
         if (dh) load_row<T, VEC, C>(dh + row * p.lddh, p.cols, l, ds);
     };
     fetch(r);
+    bool late = false;
     for (int parity = 0; r < p.rows; r += step, parity ^= 1) {
         float sum = 0.0f, dot = 0.0f;
         uint4 g[C], h[C], d[C];
@@ -310,8 +445,11 @@ __global__ void __launch_bounds__(ONE ? 32 * kWarpRows : kMaxBlock, ONE ? (C == 
         }
         fetch(r + step);
         reduce_row<ONE, false>(sum, dot, slots[parity], p.cluster);
-        const float rstd = rsqrtf(sum / (float)p.cols + p.eps);
-        const float k = dot * rstd * rstd / (float)p.cols;
+        const bool usual = range_factor<T>(sum, p.eps) == 1.0f;  // the same for all of the row's threads
+        late |= !usual;
+        float rstd, k;
+        gradient_scalars(sum, dot, p.eps, p.cols, 1.0f, rstd, k);
+        if (!usual) rstd = 0.0f;  // nothing of it in dw
         float out[C][kPer<T>];
 #pragma unroll
         for (int c = 0; c < C; ++c) {
@@ -321,7 +459,7 @@ __global__ void __launch_bounds__(ONE ? 32 * kWarpRows : kMaxBlock, ONE ? (C == 
 #pragma unroll
             for (int i = 0; i < kPer<T>; ++i) {
                 out[c][i] = rstd * (gv[i] * w[c][i] - hv[i] * k);
-                dw[c][i] += gv[i] * hv[i] * rstd;
+                dw[c][i] += gv[i] * (hv[i] * rstd);
             }
             if (dh) {
                 unpack<T>(d[c], gv);
@@ -329,31 +467,42 @@ __global__ void __launch_bounds__(ONE ? 32 * kWarpRows : kMaxBlock, ONE ? (C == 
                 for (int i = 0; i < kPer<T>; ++i) out[c][i] += gv[i];
             }
         }
-        store_row<T, T, VEC, C>(static_cast<T*>(p.dx) + r * p.lddx, p.cols, l, out);
+        if (usual) store_row<T, T, VEC, C>(static_cast<T*>(p.dx) + r * p.lddx, p.cols, l, out);
     }
-    if (!p.partials) return;
-    float* part = p.partials + (long long)(blockIdx.x / p.cluster) * p.cols;
+    float* part = p.partials ? p.partials + (long long)(blockIdx.x / p.cluster) * p.cols : nullptr;
     if constexpr (!ONE) {
+        if (part) {
 #pragma unroll
-        for (int c = 0; c < C; ++c)
+            for (int c = 0; c < C; ++c)
 #pragma unroll
-            for (int i = 0; i < kPer<T>; ++i) {
-                const int col = column<T, VEC>(c, i, l);
-                if (col < p.cols) part[col] = dw[c][i];
-            }
+                for (int i = 0; i < kPer<T>; ++i) {
+                    const int col = column<T, VEC>(c, i, l);
+                    if (col < p.cols) part[col] = dw[c][i];
+                }
+        }
+        if (late) {  // the same for all blocks of the cluster
+            if (p.cluster > 1) cluster_sync();
+            __syncthreads();
+            if (blockIdx.x % p.cluster == 0) late_rows<T>(p, 1, part);
+        }
     } else {  // the block's warps side by side, added in order
         __shared__ float rows[kWarpRows][32 * C * kPer<T>];
+        if (part) {
 #pragma unroll
-        for (int c = 0; c < C; ++c)
+            for (int c = 0; c < C; ++c)
 #pragma unroll
-            for (int i = 0; i < kPer<T>; ++i) rows[threadIdx.x / 32][column<T, VEC>(c, i, l)] = dw[c][i];
-        __syncthreads();
-        for (int col = threadIdx.x; col < p.cols; col += 32 * kWarpRows) {
-            float s = rows[0][col];
-#pragma unroll
-            for (int k = 1; k < kWarpRows; ++k) s += rows[k][col];
-            part[col] = s;
+                for (int i = 0; i < kPer<T>; ++i) rows[threadIdx.x / 32][column<T, VEC>(c, i, l)] = dw[c][i];
         }
+        late = __syncthreads_or(late);
+        if (part) {
+            for (int col = threadIdx.x; col < p.cols; col += 32 * kWarpRows) {
+                float s = rows[0][col];
+#pragma unroll
+                for (int k = 1; k < kWarpRows; ++k) s += rows[k][col];
+                part[col] = s;
+            }
+        }
+        if (late) late_rows<T>(p, kWarpRows, part);  // a thread's columns are the same there
     }
 }
 
@@ -431,6 +580,11 @@ __global__ void __launch_bounds__(MAX, 512 / MAX) rms_norm_backward_ring_kernel(
     bool failed = false;
     int next = 0;  // the stage of the next row to add up, and its parity
     uint32_t parity = 0;
+    auto put_sums = [&](float sum, float dot, int to) {
+        sum = warp_sum(sum);
+        dot = warp_sum(dot);
+        if ((t & 31) == 0) slots[to][t >> 5] = make_float2(sum, dot);
+    };
     auto add_up = [&](int to) {
         if (!failed) failed = !mbar_wait(smem_u32(&bars[next]), parity, q.wait_limit);
         float sum = 0.0f, dot = 0.0f;
@@ -446,27 +600,33 @@ __global__ void __launch_bounds__(MAX, 512 / MAX) rms_norm_backward_ring_kernel(
                 dot += g[k] * wv[k] * h[k];
             }
         }
-        sum = warp_sum(sum);
-        dot = warp_sum(dot);
-        if ((t & 31) == 0) slots[to][t >> 5] = make_float2(sum, dot);
+        put_sums(sum, dot, to);
         if (++next == q.stages) {
             next = 0;
             parity ^= 1;
         }
     };
+    auto totals = [&](int from) {
+        float2 total = slots[from][0];
+        for (int k = 1; k < threads / 32; ++k) {
+            total.x += slots[from][k].x;
+            total.y += slots[from][k].y;
+        }
+        return total;
+    };
     add_up(0);
     __syncthreads();
+    bool late = false;
     int s = 0;  // this row's stage
     for (int i = 0; i < mine; ++i) {
         const long long r = blockIdx.x + (long long)i * gridDim.x;
-        float2 total = slots[i & 1][0];
-        for (int k = 1; k < threads / 32; ++k) {
-            total.x += slots[i & 1][k].x;
-            total.y += slots[i & 1][k].y;
-        }
+        float2 total = totals(i & 1);
         if (i + 1 < mine) add_up((i + 1) & 1);
-        const float rstd = rsqrtf(total.x / (float)p.cols + p.eps);
-        const float k2 = total.y * rstd * rstd / (float)p.cols;
+        float rstd, k2;
+        gradient_scalars(total.x, total.y, p.eps, p.cols, 1.0f, rstd, k2);
+        const bool usual = range_factor<T>(total.x, p.eps) == 1.0f;  // the same for all threads
+        late |= !usual;
+        if (!usual) rstd = 0.0f;  // nothing of it in dw
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             float g[kPer<T>], h[kPer<T>], wv[kPer<T>], out[1][kPer<T>];
@@ -476,14 +636,14 @@ __global__ void __launch_bounds__(MAX, 512 / MAX) rms_norm_backward_ring_kernel(
 #pragma unroll
             for (int k = 0; k < kPer<T>; ++k) {
                 out[0][k] = rstd * (g[k] * wv[k] - h[k] * k2);
-                dw[c][k] += g[k] * h[k] * rstd;
+                dw[c][k] += g[k] * (h[k] * rstd);
             }
             if (p.dhidden) {
                 chunk(s, 2, c, g);
 #pragma unroll
                 for (int k = 0; k < kPer<T>; ++k) out[0][k] += g[k];
             }
-            store_row<T, T, true, 1>(static_cast<T*>(p.dx) + r * p.lddx, p.cols, Lane{c * threads + t, 0}, out);
+            if (usual) store_row<T, T, true, 1>(static_cast<T*>(p.dx) + r * p.lddx, p.cols, Lane{c * threads + t, 0}, out);
         }
         __syncthreads();
         // After a wait that ran out the stage may still be filled, so nothing more is
@@ -498,16 +658,19 @@ __global__ void __launch_bounds__(MAX, 512 / MAX) rms_norm_backward_ring_kernel(
     if (t == 0 && failed)  // never leave with copies in flight: the last rows that were sent for
         for (int i = max(0, issued - q.stages); i < issued; ++i)
             mbar_wait(smem_u32(&bars[i % q.stages]), (uint32_t)(i / q.stages) & 1, q.wait_limit);
-    if (!p.partials) return;
-    float* part = p.partials + (long long)blockIdx.x * p.cols;
+    float* part = p.partials ? p.partials + (long long)blockIdx.x * p.cols : nullptr;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
         const int k = (c * threads + t) * kPer<T>;
-        if (k < p.cols) {
+        if (part && k < p.cols) {
 #pragma unroll
             for (int i = 0; i < kPer<T>; i += 4)
                 *reinterpret_cast<float4*>(part + k + i) = make_float4(dw[c][i], dw[c][i + 1], dw[c][i + 2], dw[c][i + 3]);
         }
+    }
+    if (late) {
+        __syncthreads();
+        late_rows<T>(p, 1, part);
     }
 }
 
@@ -522,6 +685,7 @@ __global__ void __launch_bounds__(kWide) rms_norm_wide_kernel(const __grid_const
         return p.weight_f32 ? static_cast<const float*>(p.weight)[c] : to_f32<T>(static_cast<const T*>(p.weight)[c]);
     };
     int parity = 0;
+    bool late = false;
     for (long long r = blockIdx.x; r < p.rows; r += gridDim.x, parity ^= 1) {
         const T* x = static_cast<const T*>(p.x) + r * p.ldx;
         const T* res = p.residual ? static_cast<const T*>(p.residual) + r * p.ldr : nullptr;
@@ -534,6 +698,9 @@ __global__ void __launch_bounds__(kWide) rms_norm_wide_kernel(const __grid_const
             if (sizeof(Y) == 1) top = max_nan(top, fabsf(h * weight(c)));
         }
         reduce_row<false, true>(sum, top, slots[parity], 1);
+        const bool usual = range_factor<T>(sum, p.eps) == 1.0f;  // the same for all threads
+        late |= !usual;
+        if (!usual) continue;
         const float k = rsqrtf(sum / (float)p.cols + p.eps);
         float inv = 1.0f;
         if (sizeof(Y) == 1) {
@@ -551,6 +718,7 @@ __global__ void __launch_bounds__(kWide) rms_norm_wide_kernel(const __grid_const
             y[c] = from_f32<Y>(h * k * weight(c) * inv);
         }
     }
+    if (late) late_rows<T, Y>(p, 1);
 }
 
 template <class T>
@@ -563,6 +731,7 @@ __global__ void __launch_bounds__(kWide) rms_norm_backward_wide_kernel(const __g
         return p.weight_f32 ? static_cast<const float*>(p.weight)[c] : to_f32<T>(static_cast<const T*>(p.weight)[c]);
     };
     int parity = 0;
+    bool late = false;
     for (long long r = blockIdx.x; r < p.rows; r += gridDim.x, parity ^= 1) {
         const T* dy = static_cast<const T*>(p.dy) + r * p.lddy;
         const T* hid = static_cast<const T*>(p.hidden) + r * p.ldh;
@@ -576,6 +745,9 @@ __global__ void __launch_bounds__(kWide) rms_norm_backward_wide_kernel(const __g
             dot += to_f32<T>(dy[c]) * weight(c) * h;
         }
         reduce_row<false, false>(sum, dot, slots[parity], 1);
+        const bool usual = range_factor<T>(sum, p.eps) == 1.0f;  // the same for all threads
+        late |= !usual;
+        if (!usual) continue;
         const float rstd = rsqrtf(sum / (float)p.cols + p.eps);
         const float k = dot * rstd * rstd / (float)p.cols;
 #pragma unroll 4
@@ -587,6 +759,7 @@ __global__ void __launch_bounds__(kWide) rms_norm_backward_wide_kernel(const __g
             dx[c] = from_f32<T>(d);
         }
     }
+    if (late) late_rows<T>(p, 1, part);
 }
 
 // out[c] = sum over b < n of partials[b][c]: 32 columns a block, 32 threads a
@@ -786,6 +959,7 @@ template <class T>
 int launch_ring(const NormBackwardParams& p, const RingShape& s, int& blocks) {
     RingParams q;
     q.p = p;
+    q.p.cluster = 1;  // a block a row, however long
     q.stages = s.stages;
     q.row_bytes = p.cols * (int)sizeof(T);
     q.stall = stall_test("norm") ? 1 : 0;
