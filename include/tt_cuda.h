@@ -420,7 +420,8 @@ int ttc_rms_norm_backward(const ttc_rms_norm_backward_desc* desc);
 int ttc_rms_norm_backward_workspace(const ttc_rms_norm_backward_desc* desc, size_t* bytes);
 
 /* y [M, N] = act(x [M, K] W + bias) + residual. With dtype E4M3 the product is
- * scaled before the bias: x_scales[m] * w_scales[n] * (x W)(m, n).
+ * scaled before the bias: (x_scales[m] * w_scales[n]) * (x W)(m, n), by the fp32
+ * product of the two scales.
  * y, bias, residual and pre have y_dtype: dtype or F32 for 16-bit operands;
  * F16, BF16 or F32 for E4M3. y may be `residual` itself (same address and leading
  * dimension); no other overlap is allowed. */

@@ -273,3 +273,27 @@ def test_norm_gradients_of_rows_whose_squares_leave_fp32(lib, rows, cols, dtype,
     assert torch.equal(without.t, dx.t)
     call(dy, None)
     assert torch.equal(dy.t, dx.t)
+
+
+# ----------------------------------------------------------------------------------------------- e4m3 scales
+@pytest.mark.parametrize("M,N,pad", [(3, 256, 0), (3, 256, 3), (300, 256, 0), (2560, 2048, 0), (2560, 2050, 0)])
+@pytest.mark.parametrize("xs,ws", [(2.0 ** 110, 2.0 ** -100), (2.0 ** -120, 2.0 ** 110), (2.0 ** -60, 2.0 ** -60), (1.0, 0.75)])
+def test_scales_are_multiplied_with_one_another_first(lib, M, N, pad, xs, ws):
+    """On every kernel and path the same: the values here are whole numbers times a power of two, exact in fp32, and
+    only the product of the scales keeps them in range."""
+    K = 64
+    g = gen(M)
+    x, w = Mat(M, K, "e4m3", fill=448), Mat(N, K, "e4m3", fill=448)
+    x.t[1:].copy_(torch.randint(-8, 9, (M - 1, K), generator=g, device="cuda").float())
+    w.t[1:].copy_(torch.randint(-8, 9, (N - 1, K), generator=g, device="cuda").float())
+    XS, WS = Mat(1, M, "f32", fill=xs), Mat(1, N, "f32", fill=ws)
+    want = (x.f64() @ w.f64().t()) * (xs * ws)
+    y = Mat(M, N, "f32", pad)
+    lib.linear(lib.linear_desc(M, N, K, x.ptr, K, w.ptr, K, y.ptr, y.ld, lib.E4M3, y_dtype=lib.F32, trans_w=True,
+                               x_scales=XS.ptr, w_scales=WS.ptr))
+    assert torch.equal(y.f64(), want)
+    gate, up = Mat(M, N, "f32", pad), Mat(M, N, "f32", pad)
+    lib.gated_linear(lib.gated_linear_desc(M, N, K, x.ptr, K, w.ptr, w.ptr, K, y.ptr, y.ld, lib.E4M3, y_dtype=lib.F32,
+                                           trans_w=True, gate=gate.ptr, up=up.ptr, ldp=up.ld, x_scales=XS.ptr,
+                                           wg_scales=WS.ptr, wu_scales=WS.ptr))
+    assert torch.equal(gate.f64(), want) and torch.equal(up.f64(), want)

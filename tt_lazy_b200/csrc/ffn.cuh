@@ -419,8 +419,8 @@ __device__ __forceinline__ void finish_column(const ProductEpilogue& e, int row,
     if (e.row_scales)
         each(1, row, 0, [&](int i, long long at) {
             const float rs = e.row_scales[at];
-            v[i] = v[i] * rs * s0;
-            if (GATED) u[i] = u[i] * rs * s1;
+            v[i] *= rs * s0;
+            if (GATED) u[i] *= rs * s1;
         });
     if (GATED) {
         if (e.gate)

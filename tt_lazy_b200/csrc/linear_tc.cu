@@ -256,10 +256,10 @@ __device__ __forceinline__ bool pair_epilogue(const ProductParams& q, uint8_t* s
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
                 const float4 s = *reinterpret_cast<const float4*>(scales + col + i);
-                v[i] = v[i] * row_scale * s.x;
-                v[i + 1] = v[i + 1] * row_scale * s.y;
-                v[i + 2] = v[i + 2] * row_scale * s.z;
-                v[i + 3] = v[i + 3] * row_scale * s.w;
+                v[i] *= row_scale * s.x;
+                v[i + 1] *= row_scale * s.y;
+                v[i + 2] *= row_scale * s.z;
+                v[i + 3] *= row_scale * s.w;
             }
         };
         // the value of 32 columns before the activation
