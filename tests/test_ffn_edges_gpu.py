@@ -297,3 +297,155 @@ def test_scales_are_multiplied_with_one_another_first(lib, M, N, pad, xs, ws):
                                            trans_w=True, gate=gate.ptr, up=up.ptr, ldp=up.ld, x_scales=XS.ptr,
                                            wg_scales=WS.ptr, wu_scales=WS.ptr))
     assert torch.equal(gate.f64(), want) and torch.equal(up.f64(), want)
+
+
+# ------------------------------------------------------------------------------------------------ seldom taken
+def pre_values(g, M, N, dtype):
+    """What the gradients' activations see: ordinary values, zeros of both signs and the negative tail."""
+    z = rand(g, M, N, 2.0)
+    pick = torch.rand(M, N, generator=g, device="cuda")
+    z = torch.where(pick < 0.1, torch.zeros_like(z), z)
+    z = torch.where(pick < 0.05, -torch.zeros_like(z), z)
+    z = torch.where(pick > 0.8, -2.0 - 8.0 * torch.rand(M, N, generator=g, device="cuda", dtype=torch.float64), z)
+    return z.to(T[dtype])
+
+
+# the tile kernel with both products in one launch, its column path, the pair kernel, its element path
+GRADIENT_SHAPES = [(40, 200, 72, 0), (67, 129, 257, 3), (2304, 2080, 136, 0), (2560, 2050, 72, 3)]
+
+
+@pytest.mark.parametrize("M,N,K,pad", GRADIENT_SHAPES)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("dtype,trans_w", [("bf16", True), ("f16", True), ("bf16", False)])
+def test_linear_gradients_of_every_activation(lib, M, N, K, pad, act, dtype, trans_w):
+    """Bounds as in test_ffn_gpu.test_linear_backward, and the norm-wise one for f16 too."""
+    g = gen(M + N + K)
+    x, (w,), xv, (wv,), _, _ = product_inputs(g, M, N, K, dtype, trans_w, pad, 0)
+    dy, pre = Mat(M, N, dtype, pad, fill=rand(g, M, N)), Mat(M, N, dtype, pad, fill=pre_values(g, M, N, dtype))
+    dx, db = Mat(M, K, dtype, pad), Mat(1, N, dtype)
+    dw = Mat(N, K, dtype, pad) if trans_w else Mat(K, N, dtype, pad)
+    d = lib.linear_backward_desc(M, N, K, dy.ptr, dy.ld, x.ptr, x.ld, w.ptr, w.ld, lib.DTYPES[dtype], trans_w=trans_w,
+                                 act=lib.ACTIVATIONS[act], pre=pre.ptr, ldp=pre.ld, dx=dx.ptr, lddx=dx.ld, dw=dw.ptr,
+                                 lddw=dw.ld, dbias=db.ptr)
+    lib.linear_backward(d, scratch(lib, d))
+    dz = dy.f64() * act64(act, pre.f64())[1]
+    ddz = (U[dtype] + 2.0 ** -20) * dz.abs() + 2.0 ** -20 * dy.f64().abs() + TINY[dtype]
+    for got, a, da, b, name in ((dx.t, dz, ddz, wv.t(), "dx"), (dw.t if trans_w else dw.t.t(), dz.t(), ddz.t(), xv, "dw")):
+        want, acc = product64(a, b)
+        within(got, want, U[dtype] * want.abs() + da @ b.abs() + acc + TINY[dtype], name)
+        normwise(got, want, dtype, name, (a, b))
+    tol = U[dtype] * dz.sum(0).abs() + (M / 64 + 300) * 2.0 ** -24 * dz.abs().sum(0) + 2.0 ** -20 * dy.f64().abs().sum(0)
+    within(db.t[0], dz.sum(0), tol + TINY[dtype], "dbias")
+    assert dx.untouched_outside() and dw.untouched_outside() and db.untouched_outside()
+
+
+@pytest.mark.parametrize("M,N,K,pad", GRADIENT_SHAPES)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("dtype,trans_w", [("bf16", True), ("f16", True), ("bf16", False)])
+def test_gated_gradients_of_every_activation(lib, M, N, K, pad, act, dtype, trans_w):
+    """Bounds as in test_ffn_gpu.test_gated_linear_backward, and the norm-wise one for f16 too."""
+    g = gen(M + N + 3 * K)
+    x, (wg, wu), xv, (gv, uv), _, _ = product_inputs(g, M, N, K, dtype, trans_w, pad, 0, ("wg", "wu"))
+    dy, up = (Mat(M, N, dtype, pad, fill=rand(g, M, N)) for _ in range(2))
+    gate = Mat(M, N, dtype, pad, fill=pre_values(g, M, N, dtype))
+    dx = Mat(M, K, dtype, pad)
+    dwg, dwu = (Mat(N, K, dtype, pad) if trans_w else Mat(K, N, dtype, pad) for _ in range(2))
+    d = lib.gated_linear_backward_desc(M, N, K, dy.ptr, dy.ld, x.ptr, x.ld, wg.ptr, wu.ptr, wg.ld, gate.ptr, up.ptr,
+                                       gate.ld, lib.DTYPES[dtype], trans_w=trans_w, act=lib.ACTIVATIONS[act], dx=dx.ptr,
+                                       lddx=dx.ld, dwg=dwg.ptr, dwu=dwu.ptr, lddw=dwg.ld)
+    lib.gated_linear_backward(d, scratch(lib, d))
+    a, s = act64(act, gate.f64())
+    e, u = dy.f64(), up.f64()
+    dg, du = e * u * s, e * a
+    ddg = (U[dtype] + 2.0 ** -20) * dg.abs() + 2.0 ** -20 * (e * u).abs() + TINY[dtype]
+    ddu = (U[dtype] + 2.0 ** -20) * du.abs() + 2.0 ** -20 * e.abs() + TINY[dtype]
+    zg, ag = product64(dg, gv.t())
+    zu, au = product64(du, uv.t())
+    want = zg + zu
+    within(dx.t, want, U[dtype] * want.abs() + ddg @ gv.t().abs() + ddu @ uv.t().abs() + 2 * (ag + au) + TINY[dtype], "dx")
+    normwise(dx.t, want, dtype, "dx", (dg, gv.t()), (du, uv.t()))
+    for got, v, dv, name in ((dwg, dg, ddg, "dwg"), (dwu, du, ddu, "dwu")):
+        want, acc = product64(v.t(), xv)
+        stored = got.t if trans_w else got.t.t()
+        within(stored, want, U[dtype] * want.abs() + dv.t() @ xv.abs() + acc + TINY[dtype], name)
+        normwise(stored, want, dtype, name, (v.t(), xv))
+        assert got.untouched_outside()
+    assert dx.untouched_outside()
+
+
+@pytest.mark.parametrize("N", [2688, 2944, 3200, 4736, 6272])  # 7, 6, 5, 4 and 3 shares of the sum on 148 SMs
+@pytest.mark.parametrize("M,K", [(100, 2560), (93, 2568), (200, 2600)])
+@pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
+def test_every_number_of_shares(lib, N, M, K, dtype):
+    """Sums split over clusters whose size is no power of two, in even and uneven shares."""
+    g = gen(N + M)
+    pad = -K % 16
+    x, (w,), xv, (wv,), xs, (ws,) = product_inputs(g, M, N, K, dtype, True, pad, 0)
+    y = Mat(M, N, "bf16")
+    lib.linear(lib.linear_desc(M, N, K, x.ptr, x.ld, w.ptr, w.ld, y.ptr, N, lib.DTYPES[dtype], y_dtype=lib.BF16, trans_w=True,
+                               x_scales=ptr(xs), w_scales=ptr(ws)))
+    z, dz = product64(xv, wv)
+    within(y.t, z, (U["bf16"] + 2.0 ** -23) * z.abs() + dz + TINY["bf16"], "linear")
+    assert y.untouched_outside()
+    half = N // 2  # the gated kernel's tiles are half as wide
+    x, (wg, wu), xv, (gv, uv), xs, (gs, us) = product_inputs(g, M, half, K, dtype, True, pad, 0, ("wg", "wu"))
+    y = Mat(M, half, "bf16")
+    lib.gated_linear(lib.gated_linear_desc(M, half, K, x.ptr, x.ld, wg.ptr, wu.ptr, wg.ld, y.ptr, half, lib.DTYPES[dtype],
+                                           y_dtype=lib.BF16, trans_w=True, act=lib.ACT_NONE, x_scales=ptr(xs),
+                                           wg_scales=ptr(gs), wu_scales=ptr(us)))
+    a, da = product64(xv, gv)
+    u, du = product64(xv, uv)
+    want = a * u
+    within(y.t, want, (U["bf16"] + 2.0 ** -23) * want.abs() + da * u.abs() + a.abs() * du + da * du + TINY["bf16"], "gated")
+    assert y.untouched_outside()
+
+
+@pytest.mark.parametrize("cols", ROW_LENGTHS)
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("pad", [0, 3])
+def test_nan_and_infinities_stay_in_their_rows_of_the_norm(lib, cols, dtype, pad):
+    """A NaN makes its row NaN, an infinity is NaN in its place and the rest of its row 0 (h rsqrt(inf)), in the
+    gradients both make the row of dx NaN; the rows beside them are what they are without."""
+    rows = 700
+    g = gen(cols)
+    x, w, dy = rand(g, rows, cols), 1 + rand(g, 1, cols, 0.1), rand(g, rows, cols)
+
+    def gradients(x):
+        X, DY, W, dx = (Mat(t.shape[0], cols, dtype, p, fill=t) for t, p in ((x, pad), (dy, pad), (w, 0), (x, pad)))
+        d = lib.rms_norm_backward_desc(rows, cols, DY.ptr, DY.ld, X.ptr, X.ld, W.ptr, dx.ptr, dx.ld, None, lib.DTYPES[dtype])
+        lib.rms_norm_backward(d)
+        return dx.t
+
+    clean, clean_dx = run_norm(lib, x, w, dtype, dtype, pad)[0], gradients(x)
+    bad = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    for r, c, v in ((1, 0, "nan"), (300, cols - 1, "nan"), (2, cols // 2, "inf"), (699, cols - 1, "-inf")):
+        x[r, c] = float(v)
+        bad[r] = True
+    y, dx = run_norm(lib, x, w, dtype, dtype, pad)[0], gradients(x)
+    assert torch.equal(y[~bad], clean[~bad]) and torch.equal(dx[~bad], clean_dx[~bad])
+    assert torch.isnan(y[[1, 300]]).all() and torch.isnan(dx[bad]).all()
+    for r, c in ((2, cols // 2), (699, cols - 1)):
+        assert torch.isnan(y[r, c]) and int((y[r] == 0).sum()) == cols - 1
+
+
+@pytest.mark.parametrize("out", ["bf16", "f32"])
+def test_wait_expiry_with_residual_copies_on_their_way(lib, monkeypatch, out):
+    """The large products' loads left out, the residual's not: the kernel waits for those before it leaves."""
+    M, N, K = 2048, 2560, 256
+    g = gen(9)
+    x, (w,), xv, (wv,), _, _ = product_inputs(g, M, N, K, "bf16", True, 0, 0)
+    y, res = Mat(M, N, out), Mat(M, N, out, fill=rand(g, M, N))
+    d = lib.linear_desc(M, N, K, x.ptr, K, w.ptr, K, y.ptr, N, lib.BF16, y_dtype=lib.DTYPES[out], trans_w=True,
+                        residual=res.ptr, ldr=N)
+    torch.cuda.synchronize()
+    monkeypatch.setenv("TTC_TEST_STALL", "linear")
+    lib.linear(d)
+    with pytest.raises(lib.TTCError) as e:
+        lib.synchronize()
+    assert e.value.code == lib.ERR_TIMEOUT
+    monkeypatch.delenv("TTC_TEST_STALL")
+    lib.linear(d)
+    lib.synchronize()
+    z, dz = product64(xv, wv)
+    want = z + res.f64()
+    within(y.t, want, (U[out] + 2.0 ** -22) * (want.abs() + res.f64().abs()) + dz + TINY[out], "y")
