@@ -352,6 +352,8 @@ int ttc_gemm_select_path(const ttc_gemm_desc* desc);
  * stream and holds nothing between calls. Calls that may overlap (different
  * streams, or captured graphs that are replayed side by side) take different
  * workspaces. Results do not depend on scheduling: no floating-point atomics.
+ * A result overlaps neither an operand nor another result, nor the workspace,
+ * except where a descriptor says so.
  *
  * Zero rows (rows or M = 0) are a valid call: gradients of weights and biases
  * are then zeros, everything else is left as it is. Descriptors are checked
@@ -442,8 +444,10 @@ int ttc_linear(const ttc_linear_desc* desc);
 int ttc_linear_workspace(const ttc_linear_desc* desc, size_t* bytes);
 
 /* Gradients of ttc_linear (F16, BF16): with dz = dy act'(pre), rounded to
- * dtype for the products,
- *   dx = dz W^T,  dw = x^T dz (stored as W is),  dbias = sum over rows of dz.
+ * dtype for the products (the tensor cores' operands have that type; over a whole
+ * matrix dx and dw are off by about sqrt(2) times what their own rounding leaves),
+ *   dx = dz W^T,  dw = x^T dz (stored as W is),
+ *   dbias = sum over rows of dz as it is before that rounding.
  * The residual's gradient is dy itself. Each of dx, dw, dbias is optional; x is
  * read for dw, w for dx, pre for act != NONE. */
 typedef struct {

@@ -233,6 +233,12 @@ def test_norm_of_far_rows_in_place(lib, rows, cols, dtype):
     lib.rms_norm(lib.rms_norm_desc(rows, cols, x.ptr, cols, w.ptr, x.ptr, cols, lib.DTYPES[dtype], eps=0.0,
                                    residual=res.ptr, ldr=cols, hidden=res.ptr, ldh=cols))
     assert torch.equal(x.t, want) and torch.equal(res.t, want_h)
+    # the other way round: hidden over x, y over the residual
+    x, res = (Mat(rows, cols, dtype, fill=far_rows(g, rows, cols)) for _ in range(2))
+    want, _, want_h = run_norm(lib, x.f64(), w.f64(), dtype, dtype, eps=0.0, residual=res.f64())
+    lib.rms_norm(lib.rms_norm_desc(rows, cols, x.ptr, cols, w.ptr, res.ptr, cols, lib.DTYPES[dtype], eps=0.0,
+                                   residual=res.ptr, ldr=cols, hidden=x.ptr, ldh=cols))
+    assert torch.equal(res.t, want) and torch.equal(x.t, want_h)
 
 
 @pytest.mark.parametrize("rows,cols", FAR)
@@ -246,12 +252,13 @@ def test_norm_gradients_of_rows_whose_squares_leave_fp32(lib, rows, cols, dtype,
     hid = Mat(rows, cols, dtype, pad, fill=far_rows(g, rows, cols))
     dy = Mat(rows, cols, dtype, pad, fill=rand(g, rows, cols))
     dh = Mat(rows, cols, dtype, pad, fill=rand(g, rows, cols)) if form == "dhidden" else None
-    w = Mat(1, cols, dtype, fill=1 + rand(g, 1, cols, 0.1))
-    dx, dw = Mat(rows, cols, dtype, pad), Mat(1, cols, dtype)
+    wt = "f32" if form == "dhidden" else dtype
+    w = Mat(1, cols, wt, fill=1 + rand(g, 1, cols, 0.1))
+    dx, dw = Mat(rows, cols, dtype, pad), Mat(1, cols, wt)
 
     def call(dx, dw):
         d = lib.rms_norm_backward_desc(rows, cols, dy.ptr, dy.ld, hid.ptr, hid.ld, w.ptr, dx.ptr, dx.ld, ptr(dw),
-                                       lib.DTYPES[dtype], eps=eps, dhidden=ptr(dh), lddh=cols)
+                                       lib.DTYPES[dtype], weight_dtype=lib.DTYPES[wt], eps=eps, dhidden=ptr(dh), lddh=cols)
         lib.rms_norm_backward(d, scratch(lib, d))
 
     call(dx, dw)
@@ -266,11 +273,16 @@ def test_norm_gradients_of_rows_whose_squares_leave_fp32(lib, rows, cols, dtype,
     within(dx.t, want, U[dtype] * want.abs() + rel * (first.abs() + spread) + 2.0 ** -23 * want.abs() + TINY[dtype], "dx")
     terms = e * unit
     relw = rel + (min(rows, rows / 148 + 2) + 700) * 2.0 ** -24
-    within(dw.t[0], terms.sum(0), U[dtype] * terms.sum(0).abs() + relw * terms.abs().sum(0) + TINY[dtype], "dweight")
+    within(dw.t[0], terms.sum(0), U[wt] * terms.sum(0).abs() + relw * terms.abs().sum(0) + TINY[wt], "dweight")
     assert dx.untouched_outside() and dw.untouched_outside()
     without = Mat(rows, cols, dtype, pad)
     call(without, None)
     assert torch.equal(without.t, dx.t)
+    if dh is not None:
+        kept = dh.t.clone()
+        call(dh, None)
+        assert torch.equal(dh.t, dx.t)
+        dh.t.copy_(kept)
     call(dy, None)
     assert torch.equal(dy.t, dx.t)
 

@@ -122,10 +122,15 @@ int check_gated_backward(const ttc_gated_linear_backward_desc& d) {
 // A block of 8 warps walks a band of rows of a 256-column stripe: a lane owns
 // 8 columns, a warp one row at a time, so that a column's sum for dbias stays
 // in a register. Memory bound: each value is read once and written once, 16
-// bytes per lane and access, a row's loads ahead of its arithmetic (as packed
-// registers: as floats, 72 and 88 us). 4096 x 8192 in bf16: 39 us with gelu (5.2
-// TB/s), 51 us for the gated pair with silu (6.6 TB/s); without the row ahead 47
-// and 73.
+// bytes per lane and access, a row's loads ahead of its arithmetic, as packed
+// registers. In bf16, buffers in turn so that none is still in L2: 4096 x 8192 with
+// gelu and dbias 40 us (5.0 TB/s), the gated pair with silu 56 us (6.0 TB/s); 8192 x
+// 16384 with gelu 145 us (5.5 TB/s), the pair of 4096 x 16384 107 us (6.3 TB/s).
+// Measured where these took 39 and 51: the row ahead as floats 72 and 88, without
+// it 47 and 73.
+//
+// What the products read of dz (dg, du) is rounded to their 16-bit type: a tensor-core
+// operand has no wider form of that speed. The column sums take the values before it.
 constexpr int kStripe = 256, kBandWarps = 8;
 // Rows of a block: 64, more when that would make over 256 bands of partial sums,
 // and fewer, down to one a warp, while that leaves SMs without two blocks: a

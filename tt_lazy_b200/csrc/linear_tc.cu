@@ -1200,7 +1200,7 @@ int plan_product(ProductParams& q, bool* pair) {
     // CTAs a tile would leave SMs idle (256 x 1024 x 512: 18.3 us with 8 tiles of
     // 256 rows, 6.2 with 64 tiles of 32). CTAs a tile: until the SMs have one
     // each, and two each for few rows, whose CTAs spend their time waiting for the
-    // weight (1 x 4096 x 16384: 24.2 us with 256 CTAs, 28.0 with 128; 64 x 4096 x
+    // weight (1 x 4096 x 16384: 24.2 us with 256 CTAs, 28.0 with 128, side by side; 64 x 4096 x
     // 4096: 13.1 us with 128, 15.8 with 256), while every share has at least
     // four k-blocks (two for a few rows, where joining the shares is quick). One CTA
     // an SM takes any number of shares whose clusters run at once (256 x 4608 x 4608:
@@ -1268,7 +1268,7 @@ int run_tiles(ProductSet<N>& set) {
     }
     // The ring: half an SM's shared memory where not all CTAs run at once otherwise
     // and that holds three stages, so that two meet on an SM and one's loads run
-    // under the other's start and end (4 x 16384 x 4096 gated: 45 us, 51 with the
+    // under the other's start and end (4 x 16384 x 4096 gated, side by side: 45 us, 51 with the
     // whole of it; 32 x 2048 x 8192 in 16 clusters of 8, of which 15 fit: 11.4 and
     // 22.4); else most of it.
     int at_once = 0;
