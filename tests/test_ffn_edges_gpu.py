@@ -461,3 +461,47 @@ def test_wait_expiry_with_residual_copies_on_their_way(lib, monkeypatch, out):
     z, dz = product64(xv, wv)
     want = z + res.f64()
     within(y.t, want, (U[out] + 2.0 ** -22) * (want.abs() + res.f64().abs()) + dz + TINY[out], "y")
+
+
+@pytest.mark.parametrize("rows,cols", FAR)
+@pytest.mark.parametrize("pad", [0, 3])
+def test_norm_rows_at_the_borders_of_the_range(lib, rows, cols, pad):
+    """fp32 rows whose sums of squares lie within a few roundings of the largest value and of 2^-90, on both sides:
+    each row is taken one way or the other, once, also where y and dx replace their inputs."""
+    g = gen(rows + 7 * cols)
+    # every element the same size, so that the sum is cols v^2; 41 steps of 2^-22 around each border
+    near = 1 + (torch.arange(rows, device="cuda", dtype=torch.float64) % 41 - 20) * 2.0 ** -22
+    border = torch.tensor([2.0 ** 128, 2.0 ** -90], device="cuda", dtype=torch.float64).repeat(rows // 2 + 1)[:rows]
+    sign = (torch.rand(rows, cols, generator=g, device="cuda") < 0.5).double() * 2 - 1
+    x = sign * (torch.sqrt(border / cols) * near).view(rows, 1)
+    X, Y = Mat(rows, cols, "f32", pad, fill=x), Mat(rows, cols, "f32", pad)
+    w = Mat(1, cols, "f32", fill=1 + rand(g, 1, cols, 0.1))
+    dy, dx, dw = Mat(rows, cols, "f32", pad, fill=rand(g, rows, cols)), Mat(rows, cols, "f32", pad), Mat(1, cols, "f32")
+    h, e, ww = X.f64(), dy.f64(), w.f64()
+    r = 1 / torch.sqrt((h * h).mean(dim=1, keepdim=True))
+    unit = h * r
+    want = unit * ww
+    rel = ((cols / 32 + 16) / 2 + 10) * 2.0 ** -24
+
+    def back(dx, dw):
+        d = lib.rms_norm_backward_desc(rows, cols, dy.ptr, dy.ld, X.ptr, X.ld, w.ptr, dx.ptr, dx.ld, ptr(dw), lib.F32, eps=0.0)
+        lib.rms_norm_backward(d, scratch(lib, d))
+
+    back(dx, dw)
+    first, spread = r * e * ww, r * unit.abs() * (e * ww * unit).abs().sum(1, keepdim=True) / cols
+    rel_dx = (1.5 * (cols / 32 + 16) + 20) * 2.0 ** -24
+    want_dx = first - r * unit * (e * ww * unit).sum(1, keepdim=True) / cols
+    within(dx.t, want_dx, U["f32"] * want_dx.abs() + rel_dx * (first.abs() + spread) + 2.0 ** -23 * want_dx.abs() + TINY["f32"], "dx")
+    relw = rel_dx + (min(rows, rows / 148 + 2) + 700) * 2.0 ** -24
+    terms = e * unit
+    within(dw.t[0], terms.sum(0), U["f32"] * terms.sum(0).abs() + relw * terms.abs().sum(0) + TINY["f32"], "dweight")
+    back(dy, None)
+    assert torch.equal(dy.t, dx.t)
+
+    def forward(y):
+        lib.rms_norm(lib.rms_norm_desc(rows, cols, X.ptr, X.ld, w.ptr, y.ptr, y.ld, lib.F32, eps=0.0))
+
+    forward(Y)
+    within(Y.t, want, (U["f32"] + rel) * want.abs() + TINY["f32"], "y")
+    forward(X)
+    assert torch.equal(X.t, Y.t)

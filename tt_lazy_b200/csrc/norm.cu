@@ -102,6 +102,10 @@ __device__ __forceinline__ void store_row(Y* row, int cols, Lane l, const float 
     }
 }
 
+template <class T>
+__device__ __forceinline__ float weight_at(const void* weight, bool f32, int c) {
+    return f32 ? static_cast<const float*>(weight)[c] : to_f32<T>(static_cast<const T*>(weight)[c]);
+}
 template <class T, bool VEC, int C>
 __device__ __forceinline__ void load_weight(const void* weight, bool f32, int cols, Lane l, float (&w)[C][kPer<T>]) {
 #pragma unroll
@@ -109,9 +113,7 @@ __device__ __forceinline__ void load_weight(const void* weight, bool f32, int co
 #pragma unroll
         for (int i = 0; i < kPer<T>; ++i) {
             const int k = column<T, VEC>(c, i, l);
-            w[c][i] = k >= cols ? 0.0f
-                      : f32     ? static_cast<const float*>(weight)[k]
-                                : to_f32<T>(static_cast<const T*>(weight)[k]);
+            w[c][i] = k >= cols ? 0.0f : weight_at<T>(weight, f32, k);
         }
 }
 
@@ -174,8 +176,8 @@ constexpr float kMinScale = 1.17549435e-38f;  // 2^-126
 
 // Squares of finite values can leave fp32: |h| from 2^64, and below 2^-63 where eps
 // does not cover them. The sums of such a row, infinite or next to nothing, are
-// taken again with the row times this power of two, exactly; 1 for any other row,
-// which pays a comparison. With it the squares of 2^30 values of 2^128 add up to
+// taken again with the row times this power of two, exactly; 1 for any other row.
+// With it the squares of 2^30 values of 2^128 add up to
 // 2^126, and values of which the sum of squares was below 2^-90 to at most 2^110.
 // F16 rows cannot get there.
 template <class T>
@@ -217,73 +219,6 @@ __device__ __forceinline__ RowPlace row_place(int cluster) {
 constexpr int kWarpRows = 4;  // rows of a block whose rows are one warp's
 constexpr int kMaxBlock = 256;
 
-// a and b over the block; MAX: b is a maximum.
-template <bool MAX>
-__device__ __forceinline__ float2 reduce_block(float a, float b) {
-    __shared__ float2 of_warp[32];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        a += __shfl_xor_sync(0xffffffffu, a, o);
-        const float x = __shfl_xor_sync(0xffffffffu, b, o);
-        b = MAX ? max_nan(b, x) : b + x;
-    }
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) of_warp[threadIdx.x >> 5] = make_float2(a, b);
-    __syncthreads();
-    float2 s = of_warp[0];
-    for (int i = 1; i < (int)blockDim.x / 32; ++i) {
-        s.x += of_warp[i].x;
-        s.y = MAX ? max_nan(s.y, of_warp[i].y) : s.y + of_warp[i].y;
-    }
-    return s;
-}
-
-// The rows of this block (of this cluster, by its first block) that need a
-// range_factor. The kernels pass over them, leaving every tensor as it is, and come
-// here at their end, so that the usual rows pay a comparison and few registers:
-// nothing to 5 % (gradients of 16384 x 4096 in bf16 94.6 -> 96.0 us, of 4096 x 16384
-// 125 -> 131; second sums inside the rows' loop spilled 70 bytes of that kernel, and
-// 64 rows of 40000 took 45 us instead of 30). `n` rows of the block at a time, as its
-// loop takes them.
-template <class T, class Y>
-__device__ __forceinline__ void late_rows(const NormParams& p, int n) {
-    auto weight = [&](int c) {
-        return p.weight_f32 ? static_cast<const float*>(p.weight)[c] : to_f32<T>(static_cast<const T*>(p.weight)[c]);
-    };
-    const long long step = (long long)(gridDim.x / p.cluster) * n;
-    for (long long base = (long long)(blockIdx.x / p.cluster) * n; base < p.rows; base += step)
-        for (long long r = base; r < min(base + n, p.rows); ++r) {
-            const T* x = static_cast<const T*>(p.x) + r * p.ldx;
-            const T* res = p.residual ? static_cast<const T*>(p.residual) + r * p.ldr : nullptr;
-            T* hid = p.hidden ? static_cast<T*>(p.hidden) + r * p.ldh : nullptr;
-            Y* y = static_cast<Y*>(p.y) + r * p.ldy;
-            auto row = [&](int c) { return res ? to_f32<T>(x[c]) + to_f32<T>(res[c]) : to_f32<T>(x[c]); };
-            float sum = 0.0f, top = 0.0f;
-            for (int c = threadIdx.x; c < p.cols; c += blockDim.x) sum += row(c) * row(c);
-            const float f = range_factor<T>(reduce_block<true>(sum, 0.0f).x, p.eps);
-            if (f == 1.0f) continue;
-            sum = 0.0f;
-            for (int c = threadIdx.x; c < p.cols; c += blockDim.x) {
-                const float h = row(c) * f;
-                sum += h * h;
-                if (sizeof(Y) == 1) top = max_nan(top, fabsf(h * weight(c)));
-            }
-            const float2 s = reduce_block<true>(sum, top);
-            const float k = rsqrtf(s.x / (float)p.cols + p.eps * f * f);
-            float inv = 1.0f;
-            if (sizeof(Y) == 1) {
-                const float scale = max_nan(s.y * k * (1.0f / 448.0f), kMinScale);
-                inv = 1.0f / scale;
-                if (threadIdx.x == 0) p.scales[r] = scale;
-            }
-            for (int c = threadIdx.x; c < p.cols; c += blockDim.x) {  // an element is read before it may be written over
-                const float h = row(c);
-                if (hid) hid[c] = from_f32<T>(h);
-                y[c] = from_f32<Y>(h * f * k * weight(c) * inv);
-            }
-        }
-}
-
 template <class T, class Y, bool VEC, bool ONE, int C>
 __global__ void __launch_bounds__(ONE ? 32 * kWarpRows : kMaxBlock) rms_norm_kernel(const __grid_constant__ NormParams p) {
     __shared__ float2 slots[2][kSlots];
@@ -301,7 +236,6 @@ __global__ void __launch_bounds__(ONE ? 32 * kWarpRows : kMaxBlock) rms_norm_ker
         if (res) load_row<T, VEC, C>(res + row * p.ldr, p.cols, l, rs);
     };
     fetch(r);
-    bool late = false;
     for (int parity = 0; r < p.rows; r += step, parity ^= 1) {
         float h[C][kPer<T>], sum = 0.0f, top = 0.0f;
 #pragma unroll
@@ -322,26 +256,34 @@ __global__ void __launch_bounds__(ONE ? 32 * kWarpRows : kMaxBlock) rms_norm_ker
         fetch(r + step);
         reduce_row<ONE, true>(sum, top, slots[parity], p.cluster);
         // All of the row is in registers now: x, residual, hidden and y may be the same memory.
-        const bool usual = range_factor<T>(sum, p.eps) == 1.0f;  // the same for all of the row's threads
-        late |= !usual;
-        if (p.hidden && usual) store_row<T, T, VEC, C>(static_cast<T*>(p.hidden) + r * p.ldh, p.cols, l, h);
-        float k = rsqrtf(sum / (float)p.cols + p.eps);
+        if (p.hidden) store_row<T, T, VEC, C>(static_cast<T*>(p.hidden) + r * p.ldh, p.cols, l, h);
+        float eps = p.eps;
+        if (const float f = range_factor<T>(sum, eps); f != 1.0f) {  // the same for all of the row's threads
+            eps = eps * f * f;
+            sum = top = 0.0f;
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int i = 0; i < kPer<T>; ++i) {
+                    h[c][i] *= f;
+                    sum += h[c][i] * h[c][i];
+                    if (sizeof(Y) == 1) top = max_nan(top, fabsf(h[c][i] * w[c][i]));
+                }
+            parity ^= 1;
+            reduce_row<ONE, true>(sum, top, slots[parity], p.cluster);
+        }
+        const float k = rsqrtf(sum / (float)p.cols + eps);
         float inv = 1.0f;
         if (sizeof(Y) == 1) {
             const float scale = max_nan(top * k * (1.0f / 448.0f), kMinScale);
             inv = 1.0f / scale;
-            if (l.t == 0 && usual) p.scales[r] = scale;
+            if (l.t == 0) p.scales[r] = scale;
         }
 #pragma unroll
         for (int c = 0; c < C; ++c)
 #pragma unroll
             for (int i = 0; i < kPer<T>; ++i) h[c][i] = h[c][i] * k * w[c][i] * inv;
-        if (usual) store_row<T, Y, VEC, C>(static_cast<Y*>(p.y) + r * p.ldy, p.cols, l, h);
-    }
-    if (ONE && !std::is_same<T, __half>::value) late = __syncthreads_or(late);
-    if (late) {
-        if (p.cluster > 1) cluster_sync();
-        if (blockIdx.x % p.cluster == 0) late_rows<T, Y>(p, ONE ? kWarpRows : 1);
+        store_row<T, Y, VEC, C>(static_cast<Y*>(p.y) + r * p.ldy, p.cols, l, h);
     }
 }
 
@@ -365,41 +307,32 @@ struct NormBackwardParams {
     int cluster;
 };
 
-// The gradients of such rows; `part` is the block's or cluster's row of the partials,
-// complete but for these.
+// The sums of a row times f = range_factor, and then its results, an element at a
+// time. The kernels leave the loop over the usual rows for such a row, so that it
+// takes no registers from them: nothing to 3 % (gradients of 16384 x 4096 in bf16 93.5
+// -> 95.1 us, of 8192 x 8192 109.5 -> 112.8, of 4096 x 16384 125.6 -> 130.4; with
+// the second sums inside the loop 70 bytes of it spilled). All of the row is read
+// before the reduction between the two, each thread's results where it alone reads.
 template <class T>
-__device__ __forceinline__ void late_rows(const NormBackwardParams& p, int n, float* part) {
-    auto weight = [&](int c) {
-        return p.weight_f32 ? static_cast<const float*>(p.weight)[c] : to_f32<T>(static_cast<const T*>(p.weight)[c]);
-    };
-    const long long step = (long long)(gridDim.x / p.cluster) * n;
-    for (long long base = (long long)(blockIdx.x / p.cluster) * n; base < p.rows; base += step)
-        for (long long r = base; r < min(base + n, p.rows); ++r) {
-            const T* dy = static_cast<const T*>(p.dy) + r * p.lddy;
-            const T* hid = static_cast<const T*>(p.hidden) + r * p.ldh;
-            const T* dh = p.dhidden ? static_cast<const T*>(p.dhidden) + r * p.lddh : nullptr;
-            T* dx = static_cast<T*>(p.dx) + r * p.lddx;
-            float sum = 0.0f, dot = 0.0f;
-            for (int c = threadIdx.x; c < p.cols; c += blockDim.x) sum += to_f32<T>(hid[c]) * to_f32<T>(hid[c]);
-            const float f = range_factor<T>(reduce_block<false>(sum, 0.0f).x, p.eps);
-            if (f == 1.0f) continue;
-            sum = 0.0f;
-            for (int c = threadIdx.x; c < p.cols; c += blockDim.x) {
-                const float h = to_f32<T>(hid[c]) * f;
-                sum += h * h;
-                dot += to_f32<T>(dy[c]) * weight(c) * h;
-            }
-            const float2 s = reduce_block<false>(sum, dot);
-            float rstd, k;
-            gradient_scalars(s.x, s.y, p.eps, p.cols, f, rstd, k);
-            for (int c = threadIdx.x; c < p.cols; c += blockDim.x) {
-                const float h = to_f32<T>(hid[c]), g = to_f32<T>(dy[c]);
-                float d = rstd * (g * weight(c) - h * k);
-                if (dh) d += to_f32<T>(dh[c]);
-                if (part) part[c] += g * (h * rstd);
-                dx[c] = from_f32<T>(d);
-            }
-        }
+__device__ __forceinline__ void far_sums(const T* dy, const T* hidden, const void* weight, int weight_f32, int cols, Lane l,
+                                         float f, float& sum, float& dot) {
+    sum = dot = 0.0f;
+#pragma unroll 1
+    for (int c = l.t; c < cols; c += l.tpr) {
+        const float h = to_f32<T>(hidden[c]) * f;
+        sum += h * h;
+        dot += to_f32<T>(dy[c]) * weight_at<T>(weight, weight_f32, c) * h;
+    }
+}
+
+template <class T>
+__device__ __forceinline__ void far_element(const T* hidden, const T* dy, const T* dhidden, T* dx, float w, float rstd, float k,
+                                            float& dw) {
+    const float h = to_f32<T>(*hidden), g = to_f32<T>(*dy);
+    float d = rstd * (g * w - h * k);
+    if (dhidden) d += to_f32<T>(*dhidden);
+    dw += g * (h * rstd);
+    *dx = from_f32<T>(d);
 }
 
 // The weight's gradient stays in registers over all of a block's rows and goes
@@ -425,84 +358,92 @@ __global__ void __launch_bounds__(ONE ? 32 * kWarpRows : kMaxBlock, ONE ? (C == 
         if (dh) load_row<T, VEC, C>(dh + row * p.lddh, p.cols, l, ds);
     };
     fetch(r);
-    bool late = false;
-    for (int parity = 0; r < p.rows; r += step, parity ^= 1) {
-        float sum = 0.0f, dot = 0.0f;
-        uint4 g[C], h[C], d[C];
+    for (int parity = 0; r < p.rows;) {
+        // The usual rows, up to one that needs a range_factor.
+        float f = 1.0f, sum, dot;
+        for (; r < p.rows; r += step, parity ^= 1) {
+            sum = dot = 0.0f;
+            uint4 g[C], h[C], d[C];
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            g[c] = gs[c];
-            h[c] = hs[c];
-            if (dh) d[c] = ds[c];
-            float hv[kPer<T>], gv[kPer<T>];
-            unpack<T>(h[c], hv);
-            unpack<T>(g[c], gv);
-#pragma unroll
-            for (int i = 0; i < kPer<T>; ++i) {
-                sum += hv[i] * hv[i];
-                dot += gv[i] * w[c][i] * hv[i];
-            }
-        }
-        fetch(r + step);
-        reduce_row<ONE, false>(sum, dot, slots[parity], p.cluster);
-        const bool usual = range_factor<T>(sum, p.eps) == 1.0f;  // the same for all of the row's threads
-        late |= !usual;
-        float rstd, k;
-        gradient_scalars(sum, dot, p.eps, p.cols, 1.0f, rstd, k);
-        if (!usual) rstd = 0.0f;  // nothing of it in dw
-        float out[C][kPer<T>];
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            float hv[kPer<T>], gv[kPer<T>];
-            unpack<T>(h[c], hv);
-            unpack<T>(g[c], gv);
-#pragma unroll
-            for (int i = 0; i < kPer<T>; ++i) {
-                out[c][i] = rstd * (gv[i] * w[c][i] - hv[i] * k);
-                dw[c][i] += gv[i] * (hv[i] * rstd);
-            }
-            if (dh) {
-                unpack<T>(d[c], gv);
-#pragma unroll
-                for (int i = 0; i < kPer<T>; ++i) out[c][i] += gv[i];
-            }
-        }
-        if (usual) store_row<T, T, VEC, C>(static_cast<T*>(p.dx) + r * p.lddx, p.cols, l, out);
-    }
-    float* part = p.partials ? p.partials + (long long)(blockIdx.x / p.cluster) * p.cols : nullptr;
-    if constexpr (!ONE) {
-        if (part) {
-#pragma unroll
-            for (int c = 0; c < C; ++c)
+            for (int c = 0; c < C; ++c) {
+                g[c] = gs[c];
+                h[c] = hs[c];
+                if (dh) d[c] = ds[c];
+                float hv[kPer<T>], gv[kPer<T>];
+                unpack<T>(h[c], hv);
+                unpack<T>(g[c], gv);
 #pragma unroll
                 for (int i = 0; i < kPer<T>; ++i) {
-                    const int col = column<T, VEC>(c, i, l);
-                    if (col < p.cols) part[col] = dw[c][i];
+                    sum += hv[i] * hv[i];
+                    dot += gv[i] * w[c][i] * hv[i];
                 }
+            }
+            fetch(r + step);
+            reduce_row<ONE, false>(sum, dot, slots[parity], p.cluster);
+            f = range_factor<T>(sum, p.eps);  // the same for all of the row's threads
+            if (f != 1.0f) break;
+            float rstd, k;
+            gradient_scalars(sum, dot, p.eps, p.cols, 1.0f, rstd, k);
+            float out[C][kPer<T>];
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                float hv[kPer<T>], gv[kPer<T>];
+                unpack<T>(h[c], hv);
+                unpack<T>(g[c], gv);
+#pragma unroll
+                for (int i = 0; i < kPer<T>; ++i) {
+                    out[c][i] = rstd * (gv[i] * w[c][i] - hv[i] * k);
+                    dw[c][i] += gv[i] * hv[i] * rstd;
+                }
+                if (dh) {
+                    unpack<T>(d[c], gv);
+#pragma unroll
+                    for (int i = 0; i < kPer<T>; ++i) out[c][i] += gv[i];
+                }
+            }
+            store_row<T, T, VEC, C>(static_cast<T*>(p.dx) + r * p.lddx, p.cols, l, out);
         }
-        if (late) {  // the same for all blocks of the cluster
-            if (p.cluster > 1) cluster_sync();
-            __syncthreads();
-            if (blockIdx.x % p.cluster == 0) late_rows<T>(p, 1, part);
-        }
+        if (f == 1.0f) break;
+        // That row, once more from memory.
+        far_sums<T>(dy + r * p.lddy, hid + r * p.ldh, p.weight, p.weight_f32, p.cols, l, f, sum, dot);
+        parity ^= 1;
+        reduce_row<ONE, false>(sum, dot, slots[parity], p.cluster);
+        float rstd, k;
+        gradient_scalars(sum, dot, p.eps, p.cols, f, rstd, k);
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < kPer<T>; ++i)
+                if (const int col = column<T, VEC>(c, i, l); col < p.cols)
+                    far_element(hid + r * p.ldh + col, dy + r * p.lddy + col, dh ? dh + r * p.lddh + col : nullptr,
+                                static_cast<T*>(p.dx) + r * p.lddx + col, w[c][i], rstd, k, dw[c][i]);
+        r += step;
+        parity ^= 1;
+        fetch(r);
+    }
+    if (!p.partials) return;
+    float* part = p.partials + (long long)(blockIdx.x / p.cluster) * p.cols;
+    if constexpr (!ONE) {
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < kPer<T>; ++i) {
+                const int col = column<T, VEC>(c, i, l);
+                if (col < p.cols) part[col] = dw[c][i];
+            }
     } else {  // the block's warps side by side, added in order
         __shared__ float rows[kWarpRows][32 * C * kPer<T>];
-        if (part) {
 #pragma unroll
-            for (int c = 0; c < C; ++c)
+        for (int c = 0; c < C; ++c)
 #pragma unroll
-                for (int i = 0; i < kPer<T>; ++i) rows[threadIdx.x / 32][column<T, VEC>(c, i, l)] = dw[c][i];
+            for (int i = 0; i < kPer<T>; ++i) rows[threadIdx.x / 32][column<T, VEC>(c, i, l)] = dw[c][i];
+        __syncthreads();
+        for (int col = threadIdx.x; col < p.cols; col += 32 * kWarpRows) {
+            float s = rows[0][col];
+#pragma unroll
+            for (int k = 1; k < kWarpRows; ++k) s += rows[k][col];
+            part[col] = s;
         }
-        late = __syncthreads_or(late);
-        if (part) {
-            for (int col = threadIdx.x; col < p.cols; col += 32 * kWarpRows) {
-                float s = rows[0][col];
-#pragma unroll
-                for (int k = 1; k < kWarpRows; ++k) s += rows[k][col];
-                part[col] = s;
-            }
-        }
-        if (late) late_rows<T>(p, kWarpRows, part);  // a thread's columns are the same there
     }
 }
 
@@ -528,7 +469,7 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 template <class T, int C, int MAX>
 __global__ void __launch_bounds__(MAX, 512 / MAX) rms_norm_backward_ring_kernel(const __grid_constant__ RingParams q) {
     extern __shared__ __align__(16) uint8_t ring[];
-    __shared__ float2 slots[2][MAX / 32];
+    __shared__ float2 slots[3][MAX / 32];  // two that rows use in turn, one for sums taken again
     __shared__ alignas(8) uint64_t bars[kMaxStages];
     const NormBackwardParams& p = q.p;
     const int t = threadIdx.x, threads = blockDim.x, n = p.cols / kPer<T>;  // chunks of a row
@@ -616,35 +557,8 @@ __global__ void __launch_bounds__(MAX, 512 / MAX) rms_norm_backward_ring_kernel(
     };
     add_up(0);
     __syncthreads();
-    bool late = false;
     int s = 0;  // this row's stage
-    for (int i = 0; i < mine; ++i) {
-        const long long r = blockIdx.x + (long long)i * gridDim.x;
-        float2 total = totals(i & 1);
-        if (i + 1 < mine) add_up((i + 1) & 1);
-        float rstd, k2;
-        gradient_scalars(total.x, total.y, p.eps, p.cols, 1.0f, rstd, k2);
-        const bool usual = range_factor<T>(total.x, p.eps) == 1.0f;  // the same for all threads
-        late |= !usual;
-        if (!usual) rstd = 0.0f;  // nothing of it in dw
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            float g[kPer<T>], h[kPer<T>], wv[kPer<T>], out[1][kPer<T>];
-            chunk(s, 0, c, g);
-            chunk(s, 1, c, h);
-            weight(c, wv);
-#pragma unroll
-            for (int k = 0; k < kPer<T>; ++k) {
-                out[0][k] = rstd * (g[k] * wv[k] - h[k] * k2);
-                dw[c][k] += g[k] * (h[k] * rstd);
-            }
-            if (p.dhidden) {
-                chunk(s, 2, c, g);
-#pragma unroll
-                for (int k = 0; k < kPer<T>; ++k) out[0][k] += g[k];
-            }
-            if (usual) store_row<T, T, true, 1>(static_cast<T*>(p.dx) + r * p.lddx, p.cols, Lane{c * threads + t, 0}, out);
-        }
+    auto end_row = [&](int i) {
         __syncthreads();
         // After a wait that ran out the stage may still be filled, so nothing more is
         // sent for: its barrier must not be armed again, nor its buffer written.
@@ -653,24 +567,72 @@ __global__ void __launch_bounds__(MAX, 512 / MAX) rms_norm_backward_ring_kernel(
             ++issued;
         }
         if (++s == q.stages) s = 0;
+    };
+    for (int i = 0; i < mine; ++i) {
+        // The usual rows, up to one that needs a range_factor.
+        float f = 1.0f;
+        for (; i < mine; ++i) {
+            const long long r = blockIdx.x + (long long)i * gridDim.x;
+            const float2 total = totals(i & 1);
+            if (i + 1 < mine) add_up((i + 1) & 1);
+            f = range_factor<T>(total.x, p.eps);  // the same for all threads
+            if (f != 1.0f) break;
+            float rstd, k2;
+            gradient_scalars(total.x, total.y, p.eps, p.cols, 1.0f, rstd, k2);
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                float g[kPer<T>], h[kPer<T>], wv[kPer<T>], out[1][kPer<T>];
+                chunk(s, 0, c, g);
+                chunk(s, 1, c, h);
+                weight(c, wv);
+#pragma unroll
+                for (int k = 0; k < kPer<T>; ++k) {
+                    out[0][k] = rstd * (g[k] * wv[k] - h[k] * k2);
+                    dw[c][k] += g[k] * h[k] * rstd;
+                }
+                if (p.dhidden) {
+                    chunk(s, 2, c, g);
+#pragma unroll
+                    for (int k = 0; k < kPer<T>; ++k) out[0][k] += g[k];
+                }
+                store_row<T, T, true, 1>(static_cast<T*>(p.dx) + r * p.lddx, p.cols, Lane{c * threads + t, 0}, out);
+            }
+            end_row(i);
+        }
+        if (f == 1.0f) break;
+        // That row, still in its stage.
+        const T* dy = reinterpret_cast<const T*>(ring + s * stage_bytes);
+        float2 a;
+        far_sums<T>(dy, dy + p.cols, p.weight, p.weight_f32, p.cols, Lane{t, threads}, f, a.x, a.y);
+        put_sums(a.x, a.y, 2);
+        __syncthreads();  // these slots are not written again before the barrier at the end of the row
+        a = totals(2);
+        float rstd, k2;
+        gradient_scalars(a.x, a.y, p.eps, p.cols, f, rstd, k2);
+        T* dx = static_cast<T*>(p.dx) + (blockIdx.x + (long long)i * gridDim.x) * p.lddx;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int k = 0; k < kPer<T>; ++k)
+                if (const int col = (c * threads + t) * kPer<T> + k; col < p.cols)
+                    far_element(dy + p.cols + col, dy + col, p.dhidden ? dy + 2 * p.cols + col : nullptr, dx + col,
+                                weight_at<T>(p.weight, p.weight_f32, col), rstd, k2, dw[c][k]);
+        end_row(i);
     }
     if (failed) *(volatile int*)q.status = 1;
     if (t == 0 && failed)  // never leave with copies in flight: the last rows that were sent for
         for (int i = max(0, issued - q.stages); i < issued; ++i)
             mbar_wait(smem_u32(&bars[i % q.stages]), (uint32_t)(i / q.stages) & 1, q.wait_limit);
-    float* part = p.partials ? p.partials + (long long)blockIdx.x * p.cols : nullptr;
+    if (!p.partials) return;
+    float* part = p.partials + (long long)blockIdx.x * p.cols;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
         const int k = (c * threads + t) * kPer<T>;
-        if (part && k < p.cols) {
+        if (k < p.cols) {
 #pragma unroll
             for (int i = 0; i < kPer<T>; i += 4)
                 *reinterpret_cast<float4*>(part + k + i) = make_float4(dw[c][i], dw[c][i + 1], dw[c][i + 2], dw[c][i + 3]);
         }
-    }
-    if (late) {
-        __syncthreads();
-        late_rows<T>(p, 1, part);
     }
 }
 
@@ -681,11 +643,8 @@ constexpr int kWide = 1024;
 template <class T, class Y>
 __global__ void __launch_bounds__(kWide) rms_norm_wide_kernel(const __grid_constant__ NormParams p) {
     __shared__ float2 slots[2][kSlots];
-    auto weight = [&](int c) {
-        return p.weight_f32 ? static_cast<const float*>(p.weight)[c] : to_f32<T>(static_cast<const T*>(p.weight)[c]);
-    };
+    auto weight = [&](int c) { return weight_at<T>(p.weight, p.weight_f32, c); };
     int parity = 0;
-    bool late = false;
     for (long long r = blockIdx.x; r < p.rows; r += gridDim.x, parity ^= 1) {
         const T* x = static_cast<const T*>(p.x) + r * p.ldx;
         const T* res = p.residual ? static_cast<const T*>(p.residual) + r * p.ldr : nullptr;
@@ -698,18 +657,35 @@ __global__ void __launch_bounds__(kWide) rms_norm_wide_kernel(const __grid_const
             if (sizeof(Y) == 1) top = max_nan(top, fabsf(h * weight(c)));
         }
         reduce_row<false, true>(sum, top, slots[parity], 1);
-        const bool usual = range_factor<T>(sum, p.eps) == 1.0f;  // the same for all threads
-        late |= !usual;
-        if (!usual) continue;
-        const float k = rsqrtf(sum / (float)p.cols + p.eps);
-        float inv = 1.0f;
-        if (sizeof(Y) == 1) {
-            const float scale = max_nan(top * k * (1.0f / 448.0f), kMinScale);
-            inv = 1.0f / scale;
-            if (threadIdx.x == 0) p.scales[r] = scale;
-        }
         Y* y = static_cast<Y*>(p.y) + r * p.ldy;
         T* hid = p.hidden ? static_cast<T*>(p.hidden) + r * p.ldh : nullptr;
+        auto quantise = [&](float k) {  // 1 / scale
+            if (sizeof(Y) != 1) return 1.0f;
+            const float scale = max_nan(top * k * (1.0f / 448.0f), kMinScale);
+            if (threadIdx.x == 0) p.scales[r] = scale;
+            return 1.0f / scale;
+        };
+        if (const float f = range_factor<T>(sum, p.eps); f != 1.0f) {  // the same for all threads
+            auto row = [&](int c) { return res ? to_f32<T>(x[c]) + to_f32<T>(res[c]) : to_f32<T>(x[c]); };
+            sum = top = 0.0f;
+#pragma unroll 1
+            for (int c = threadIdx.x; c < p.cols; c += kWide) {
+                const float h = row(c) * f;
+                sum += h * h;
+                if (sizeof(Y) == 1) top = max_nan(top, fabsf(h * weight(c)));
+            }
+            parity ^= 1;
+            reduce_row<false, true>(sum, top, slots[parity], 1);
+            const float k = rsqrtf(sum / (float)p.cols + p.eps * f * f), inv = quantise(k);
+#pragma unroll 1
+            for (int c = threadIdx.x; c < p.cols; c += kWide) {
+                const float h = row(c);
+                if (hid) hid[c] = from_f32<T>(h);
+                y[c] = from_f32<Y>(h * f * k * weight(c) * inv);
+            }
+            continue;
+        }
+        const float k = rsqrtf(sum / (float)p.cols + p.eps), inv = quantise(k);
 #pragma unroll 4
         for (int c = threadIdx.x; c < p.cols; c += kWide) {  // an element is read before it may be written over
             float h = to_f32<T>(x[c]);
@@ -718,20 +694,16 @@ __global__ void __launch_bounds__(kWide) rms_norm_wide_kernel(const __grid_const
             y[c] = from_f32<Y>(h * k * weight(c) * inv);
         }
     }
-    if (late) late_rows<T, Y>(p, 1);
 }
 
 template <class T>
-__global__ void __launch_bounds__(kWide) rms_norm_backward_wide_kernel(const __grid_constant__ NormBackwardParams p) {
+__global__ void __launch_bounds__(kWide, 1) rms_norm_backward_wide_kernel(const __grid_constant__ NormBackwardParams p) {
     __shared__ float2 slots[2][kSlots];
     float* part = p.partials ? p.partials + (long long)blockIdx.x * p.cols : nullptr;
     if (part)
         for (int c = threadIdx.x; c < p.cols; c += kWide) part[c] = 0.0f;  // a thread owns its columns throughout
-    auto weight = [&](int c) {
-        return p.weight_f32 ? static_cast<const float*>(p.weight)[c] : to_f32<T>(static_cast<const T*>(p.weight)[c]);
-    };
+    auto weight = [&](int c) { return weight_at<T>(p.weight, p.weight_f32, c); };
     int parity = 0;
-    bool late = false;
     for (long long r = blockIdx.x; r < p.rows; r += gridDim.x, parity ^= 1) {
         const T* dy = static_cast<const T*>(p.dy) + r * p.lddy;
         const T* hid = static_cast<const T*>(p.hidden) + r * p.ldh;
@@ -745,11 +717,19 @@ __global__ void __launch_bounds__(kWide) rms_norm_backward_wide_kernel(const __g
             dot += to_f32<T>(dy[c]) * weight(c) * h;
         }
         reduce_row<false, false>(sum, dot, slots[parity], 1);
-        const bool usual = range_factor<T>(sum, p.eps) == 1.0f;  // the same for all threads
-        late |= !usual;
-        if (!usual) continue;
-        const float rstd = rsqrtf(sum / (float)p.cols + p.eps);
-        const float k = dot * rstd * rstd / (float)p.cols;
+        float rstd, k;
+        if (const float f = range_factor<T>(sum, p.eps); f != 1.0f) {  // the same for all threads
+            far_sums<T>(dy, hid, p.weight, p.weight_f32, p.cols, Lane{(int)threadIdx.x, kWide}, f, sum, dot);
+            parity ^= 1;
+            reduce_row<false, false>(sum, dot, slots[parity], 1);
+            gradient_scalars(sum, dot, p.eps, p.cols, f, rstd, k);
+            float none = 0.0f;
+#pragma unroll 1
+            for (int c = threadIdx.x; c < p.cols; c += kWide)
+                far_element(hid + c, dy + c, dh ? dh + c : nullptr, dx + c, weight(c), rstd, k, part ? part[c] : none);
+            continue;
+        }
+        gradient_scalars(sum, dot, p.eps, p.cols, 1.0f, rstd, k);
 #pragma unroll 4
         for (int c = threadIdx.x; c < p.cols; c += kWide) {
             const float h = to_f32<T>(hid[c]), g = to_f32<T>(dy[c]);
@@ -759,7 +739,6 @@ __global__ void __launch_bounds__(kWide) rms_norm_backward_wide_kernel(const __g
             dx[c] = from_f32<T>(d);
         }
     }
-    if (late) late_rows<T>(p, 1, part);
 }
 
 // out[c] = sum over b < n of partials[b][c]: 32 columns a block, 32 threads a
@@ -960,7 +939,6 @@ template <class T>
 int launch_ring(const NormBackwardParams& p, const RingShape& s, int& blocks) {
     RingParams q;
     q.p = p;
-    q.p.cluster = 1;  // a block a row, however long
     q.stages = s.stages;
     q.row_bytes = p.cols * (int)sizeof(T);
     q.stall = stall_test("norm") ? 1 : 0;
