@@ -919,8 +919,8 @@ int launch_norm_type(const NormParams& p, int y_dtype, const RowShape& s, bool v
 // another kernel takes them. As many blocks an SM as have registers (96 a thread)
 // and a ring of three rows each. In us, register kernel / this one, both before they
 // looked for rows that leave fp32's range: 16384 x 4096 bf16 94 / 103, 8192 x 8192
-// bf16 133 / 108 (now 113), 4096 x 16384 bf16 143 / 125 (now 131), 16384 x 2048 f32
-// 92 / 84 (85), 8192 x 8192 f32 231 / 187 (191). 16-bit rows up to 512 chunks have
+// bf16 133 / 108 (now 113), 4096 x 16384 bf16 143 / 125 (now 130), 16384 x 2048 f32
+// 92 / 84 (85), 8192 x 8192 f32 231 / 187 (194). 16-bit rows up to 512 chunks have
 // twice the arithmetic a byte and more rows on an SM with the register kernel.
 struct RingShape {
     int threads, chunks, stages, per_sm;
